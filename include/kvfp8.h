@@ -399,6 +399,32 @@ int kvfp8_skinny_linear_rope(const void* x_dev, int dtype, int64_t x_stride, int
                              const void* sin_table_dev, int table_dtype, int64_t table_rows, void* out_dev,
                              int64_t out_stride, void* stream);
 
+/*
+ * Log probabilities of given tokens, entropy and the most probable tokens of logit rows
+ * (f32/f16/bf16, unit element stride, row_stride elements between rows; float32 sums):
+ *   logprobs[r] = ln p(tokens[r]), 0 for a token outside [0, vocab) (int32/int64);
+ *   entropy[r]  = -sum p ln p;  stats[r] = (max, ln sum e^(x - max)), for the backward;
+ *   top_logprobs, top_tokens [rows, top]: the largest logits, ties to the lowest index.
+ * A row of -inf alone: log probabilities -inf, entropy 0. NaN or +inf in a row: NaN.
+ * top 0..64, at most vocab (its outputs may be NULL when 0); vocab below 2^30.
+ * stats: [rows, 2], 8-byte aligned. No reference counterpart (it samples the argmax,
+ * reference src/torch_llm/inference/sampling.py).
+ */
+int kvfp8_token_logprobs(const void* logits_dev, int dtype, int64_t row_stride, int64_t rows, int64_t vocab,
+                         const void* tokens_dev, int tok_dtype, int32_t top, float* logprobs_dev,
+                         float* entropy_dev, float* stats_dev, float* top_logprobs_dev, int64_t* top_tokens_dev,
+                         void* stream);
+
+/*
+ * Gradient of the logits (their dtype, [rows, vocab] contiguous, one rounding) from those of the
+ * log probabilities and the entropies (float32 [rows], either may be NULL) and the forward's
+ * entropy and stats. A row of -inf alone gets zeros.
+ */
+int kvfp8_token_logprobs_backward(const void* logits_dev, int dtype, int64_t row_stride, int64_t rows, int64_t vocab,
+                                  const void* tokens_dev, int tok_dtype, const float* entropy_dev,
+                                  const float* stats_dev, const float* grad_logprobs_dev,
+                                  const float* grad_entropy_dev, void* grad_logits_dev, void* stream);
+
 /* Human-readable name of a return code (negative KVFP8_E* or positive hipError_t). */
 const char* kvfp8_strerror(int code);
 
