@@ -41,6 +41,7 @@ _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _DECODE_ARGS = [_P, _INT, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _INT, _P, _P, _I64, _I32, _P, _I64, _I64,
                 _P, _INT, _P, _INT, ctypes.c_float, _P, _P, _I64, _P]
+_PREFIX_ARGS = [_P, _INT, _P, _INT, _P, _INT, _I32]
 SIGNATURES = {
     "kvfp8_quantize_append": (_INT, [_P, _P, _INT, _I64, _I64, _I64, _I64, _P, _INT, _P, _INT,
                                      _I64, _I32, _I32, _I64, _I32, _P, _P, _P, _P, _P]),
@@ -70,6 +71,11 @@ SIGNATURES = {
     "kvfp8_prefill_backward_workspace_bytes": (_I64, [_INT, _I64, _I32, _I32, _I32, _I32, _I32, _INT]),
     "kvfp8_prefill_attention_backward": (_INT, [_P, _P, _P, _P, _P, _P, _INT, _I64, _I32, _I32, _I32, _P, _INT, _I32,
                                                 _I32, ctypes.c_float, _P, _P, _P, _P, _I64, _P]),
+    "kvfp8_shared_prefix_workspace_bytes": (_I64, [_I64, _I32, _I32, _I32, _I32, _I64, _I32, _INT, _INT]),
+    "kvfp8_shared_prefix_decode": (_INT, _DECODE_ARGS + _PREFIX_ARGS),
+    "kvfp8_shared_prefix_prefill": (_INT, [_P, _INT, _I64, _I32, _I32, _I32, _P, _P, _INT, _P, _P, _I64, _I32, _P, _I64,
+                                           _I64] + _PREFIX_ARGS + [_P, _INT, _I32, _I32, ctypes.c_float, _P, _P, _P,
+                                                                   _I64, _P]),
     "kvfp8_token_logprobs": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _INT, _I32, _P, _P, _P, _P, _P, _P]),
     "kvfp8_token_logprobs_backward": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _INT, _P, _P, _P, _P, _P, _P]),
     "kvfp8_timing_enable": (_INT, [_I32]),

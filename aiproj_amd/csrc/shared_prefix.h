@@ -1,0 +1,76 @@
+// Shared pieces of the shared-prefix attention kernels: arguments, the lookup of a row's group, and
+// the softmax states that the kernels leave for the merge.
+#pragma once
+
+#include "kvfp8_decode_common.h"
+
+namespace kvfp8 {
+
+// Rows of q are the sequences' new tokens (decode form: row = sequence, `d.slots`/`d.ctx` name its own
+// pages) or packed prompt tokens (prompt form: `cu` delimits the sequences; out and lse hold the
+// attention over the prompts themselves). Group g holds sequences [starts[g], starts[g + 1]); its
+// prefix is the first p_lens[g] tokens on block-table row p_slots[g].
+struct PrefixArgs {
+    DecodeArgs d;
+    int64_t rows;
+    const void* p_slots;
+    const void* p_lens;
+    const void* p_starts;
+    int32_t p_slots64, p_lens64, p_starts64;
+    int32_t groups;
+    const void* cu;             // null: decode form
+    int32_t cu64;
+    int32_t seqs;
+    int32_t max_len;            // prompt form: rows of a sequence past it are left alone
+    int32_t splits;             // states per row, [splits][rows][Hq] in d.part_*
+    float* lse;                 // prompt form [rows, Hq]
+};
+
+// Prefix tokens of group g, clipped to what the block table addresses; 0 for a slot outside it.
+__device__ __forceinline__ int64_t group_tokens(const PrefixArgs& a, int g, int64_t* slot_out) {
+    const int64_t slot = load_i(a.p_slots, a.p_slots64, g);
+    const int64_t raw = load_i(a.p_lens, a.p_lens64, g);
+    const int64_t cap = a.d.bt_width * a.d.block_size;
+    *slot_out = slot;
+    if (slot < 0 || slot >= a.d.bt_rows || raw < 0) return 0;
+    return raw < cap ? raw : cap;
+}
+
+// Last i in [0, n) with p[i] <= x (0 where there is none), p not decreasing.
+__device__ __forceinline__ int last_at_most(const void* p, int is64, int n, int64_t x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (load_i(p, is64, mid) <= x) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// The group of sequence b, -1 where it is in none.
+__device__ __forceinline__ int group_of_seq(const PrefixArgs& a, int64_t b) {
+    if (a.groups <= 0) return -1;
+    const int g = last_at_most(a.p_starts, a.p_starts64, a.groups, b);
+    return load_i(a.p_starts, a.p_starts64, g) <= b && b < load_i(a.p_starts, a.p_starts64, g + 1) ? g : -1;
+}
+
+// The sequence of a row; -1 for a prompt row of no sequence or past max_len of its own.
+__device__ __forceinline__ int64_t seq_of_row(const PrefixArgs& a, int64_t row) {
+    if (a.cu == nullptr) return row;
+    const int b = last_at_most(a.cu, a.cu64, a.seqs, row);
+    const int64_t s0 = load_i(a.cu, a.cu64, b);
+    return s0 <= row && row < load_i(a.cu, a.cu64, b + 1) && row - s0 < a.max_len ? b : -1;
+}
+
+// Tokens [lo, hi) of split s of n, in units of `step` tokens.
+__device__ __forceinline__ void split_range(int64_t n, int step, int splits, int s, int64_t* lo, int64_t* hi) {
+    const int64_t units = (n + step - 1) / step;
+    *lo = units * s / splits * step;
+    const int64_t end = units * (s + 1) / splits * step;
+    *hi = end < n ? end : n;
+}
+
+__device__ __forceinline__ int64_t prefix_part(const PrefixArgs& a, int64_t row, int s, int hq) {
+    return (s * a.rows + row) * a.d.num_q_heads + hq;
+}
+
+}  // namespace kvfp8

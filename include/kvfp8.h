@@ -400,6 +400,53 @@ int kvfp8_skinny_linear_rope(const void* x_dev, int dtype, int64_t x_stride, int
                              int64_t out_stride, void* stream);
 
 /*
+ * Paged decode attention for a batch whose sequences share prefixes: sequence b attends the tokens of
+ * its group's prefix and then its own,
+ *   out[b, hq, :] = softmax_t( q[b, hq, :] . khat[t, :] * sm_scale ) @ vhat,
+ * t over both. Group g holds the sequences [prefix_starts[g], prefix_starts[g + 1]) (groups + 1
+ * entries, not decreasing); its prefix is the first prefix_lengths[g] tokens on the block-table row
+ * prefix_slots[g], read once for the whole group. Sequences of no group attend their own tokens
+ * only. Own tokens, cache, block table and errors as kvfp8_paged_decode (slots and context_lengths
+ * count own tokens). All index arrays int32/int64 on the device. head_dim 1..512, any batch with
+ * batch * num_q_heads below 2^31.
+ *   workspace: kvfp8_shared_prefix_workspace_bytes(batch, ..., prompt = 0) bytes, 256-byte aligned, any
+ *   contents.
+ * No reference counterpart: there every sequence reads its own pages
+ * (reference src/torch_llm/kernals/decode_attention.py:39-550).
+ */
+int64_t kvfp8_shared_prefix_workspace_bytes(int64_t rows, int32_t num_q_heads, int32_t num_kv_heads,
+                                            int32_t head_dim, int32_t groups, int64_t bt_width, int32_t block_size,
+                                            int kv_dtype, int prompt);
+int kvfp8_shared_prefix_decode(const void* q_dev, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, int32_t batch,
+                               int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, const void* k_cache_dev,
+                               const void* v_cache_dev, int kv_dtype, const float* k_scales_dev,
+                               const float* v_scales_dev, int64_t num_blocks, int32_t block_size,
+                               const int32_t* block_table_dev, int64_t bt_rows, int64_t bt_width,
+                               const void* slots_dev, int slots_dtype, const void* context_lengths_dev, int ctx_dtype,
+                               float sm_scale, void* out_dev, void* workspace_dev, int64_t workspace_bytes,
+                               void* stream, const void* prefix_slots_dev, int prefix_slots_dtype,
+                               const void* prefix_lengths_dev, int prefix_lengths_dtype,
+                               const void* prefix_starts_dev, int prefix_starts_dtype, int32_t groups);
+
+/*
+ * The prompt form: joins the attention of packed prompt rows over their groups' prefixes (in the cache)
+ * to that over the prompts themselves. q [rows, Hq, D] contiguous; cu_seqlens [batch + 1], batch and
+ * max_seq_len as in kvfp8_prefill_attention, whose out and lse are read and rewritten in place: out in
+ * q's dtype, lse float32 the natural log of the joint denominator. Rows of no sequence, of no group or
+ * past max_seq_len stay as they are. Groups count sequences. Workspace with prompt = 1.
+ */
+int kvfp8_shared_prefix_prefill(const void* q_dev, int q_dtype, int64_t rows, int32_t num_q_heads,
+                                int32_t num_kv_heads, int32_t head_dim, const void* k_cache_dev,
+                                const void* v_cache_dev, int kv_dtype, const float* k_scales_dev,
+                                const float* v_scales_dev, int64_t num_blocks, int32_t block_size,
+                                const int32_t* block_table_dev, int64_t bt_rows, int64_t bt_width,
+                                const void* prefix_slots_dev, int prefix_slots_dtype, const void* prefix_lengths_dev,
+                                int prefix_lengths_dtype, const void* prefix_starts_dev, int prefix_starts_dtype,
+                                int32_t groups, const void* cu_seqlens_dev, int cu_dtype, int32_t batch,
+                                int32_t max_seq_len, float scale, void* out_dev, float* lse_dev, void* workspace_dev,
+                                int64_t workspace_bytes, void* stream);
+
+/*
  * Log probabilities of given tokens, entropy and the most probable tokens of logit rows
  * (f32/f16/bf16, unit element stride, row_stride elements between rows; float32 sums):
  *   logprobs[r] = ln p(tokens[r]), 0 for a token outside [0, vocab) (int32/int64);
