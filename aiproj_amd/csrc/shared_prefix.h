@@ -73,4 +73,21 @@ __device__ __forceinline__ int64_t prefix_part(const PrefixArgs& a, int64_t row,
     return (s * a.rows + row) * a.d.num_q_heads + hq;
 }
 
+// The matrix-core path: whether its prefix kernel takes these types and sizes (cache and q pointers are
+// checked by the call), and where its workspace holds what (byte offsets).
+bool prefix_mfma_supported(int32_t head_dim, int32_t block_size, int q_dtype, int kv_dtype);
+
+struct PrefixMfmaPlan {
+    int32_t splits;
+    int64_t states;
+    int64_t own_plan, seq_m, seq_l, seq_acc;      // decode form: the decode kernel's workspace, whole states
+    int64_t part_m, part_l, part_acc;             // the prefix's states
+    int64_t bytes;
+};
+PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t groups,
+                                int64_t bt_width, int32_t block_size, int q_dtype, bool prompt);
+
+template <int QT>
+hipError_t launch_prefix_mfma(PrefixArgs a, int kv_dtype, const PrefixMfmaPlan& p, void* workspace, hipStream_t s);
+
 }  // namespace kvfp8

@@ -7,9 +7,11 @@
 // and states of disjoint sets join exactly: M = max(m1, m2), l = l1 e^(m1 - M) + l2 e^(m2 - M), acc
 // likewise; the output is acc / l, 0 for a row without tokens. States are float32, scores base 2.
 //
-// prefix_generic_kernel takes every cache, head size (up to 512) and page size: one wave per (row, q
+// The matrix-core kernels are in shared_prefix_mfma.hip. prefix_generic_kernel takes every cache, head size (up to 512) and page size: one wave per (row, q
 // head, split of the row's tokens), on the vector ALU.
 #include "shared_prefix.h"
+
+#include "kvfp8_decode_mfma.h"
 
 namespace kvfp8 {
 
@@ -325,6 +327,42 @@ int run_generic(PrefixArgs& a, const PrefixPlan& p, int q_dtype, int kv_dtype, v
     }
 }
 
+// Whether a call runs on the matrix cores: the prefix kernel takes it and, in the decode form, the decode
+// kernel its own tokens.
+bool mfma_shape(int64_t rows, int32_t hq, int32_t hkv, int32_t d, int32_t groups, int64_t bt_width, int32_t bs, int q_dtype,
+                int kv_dtype, bool prompt) {
+    if (!prefix_mfma_supported(d, bs, q_dtype, kv_dtype)) return false;
+    // Workgroups are counted in int32, and a launch has fewer than 2^32 threads.
+    if (rows * hq / 16 + (int64_t)groups * hkv >= (1 << 22)) return false;
+    return prompt || mfma_decode_supported((int32_t)rows, hq, hkv, d, bt_width, bs, kv_dtype);
+}
+
+template <int QT>
+int run(PrefixArgs& a, int kv_dtype, void* workspace, int64_t workspace_bytes, hipStream_t s) {
+    const bool prompt = a.cu != nullptr;
+    const bool aligned = (((uintptr_t)a.d.k_cache | (uintptr_t)a.d.v_cache | (uintptr_t)a.d.out) & 15) == 0;
+    if (aligned && a.d.bt_rows < ((int64_t)1 << 26) &&
+        mfma_shape(a.rows, a.d.num_q_heads, a.d.num_kv_heads, a.d.head_dim, a.groups, a.d.bt_width, a.d.block_size, QT, kv_dtype,
+                   prompt)) {
+        const PrefixMfmaPlan p = prefix_mfma_plan(a.rows, a.d.num_q_heads, a.d.num_kv_heads, a.d.head_dim, a.groups,
+                                                  a.d.bt_width, a.d.block_size, QT, prompt);
+        if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return KVFP8_EWORKSPACE;
+        return (int)launch_prefix_mfma<QT>(a, kv_dtype, p, workspace, s);
+    }
+    const PrefixPlan p = make_plan(a.rows, a.d.num_q_heads, a.d.head_dim, a.d.bt_width, a.d.block_size, prompt);
+    if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return KVFP8_EWORKSPACE;
+    return run_generic(a, p, QT, kv_dtype, workspace, s);
+}
+
+int run(PrefixArgs& a, int q_dtype, int kv_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    switch (q_dtype) {
+        case KVFP8_F32: return run<KVFP8_F32>(a, kv_dtype, workspace, workspace_bytes, s);
+        case KVFP8_F16: return run<KVFP8_F16>(a, kv_dtype, workspace, workspace_bytes, s);
+        default: return run<KVFP8_BF16>(a, kv_dtype, workspace, workspace_bytes, s);
+    }
+}
+
 }  // namespace
 
 }  // namespace kvfp8
@@ -337,7 +375,16 @@ extern "C" int64_t kvfp8_shared_prefix_workspace_bytes(int64_t rows, int32_t num
     if (rows <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || groups < 0 || bt_width <= 0 ||
         block_size <= 0)
         return 0;
-    return make_plan(rows, num_q_heads, head_dim, bt_width, block_size, prompt != 0).bytes;
+    // The larger of what the paths need that a call of these shapes may take (its pointers decide).
+    int64_t bytes = make_plan(rows, num_q_heads, head_dim, bt_width, block_size, prompt != 0).bytes;
+    if (num_q_heads % num_kv_heads == 0)
+        for (const int q_dtype : {KVFP8_F32, KVFP8_F16, KVFP8_BF16})
+            if (mfma_shape(rows, num_q_heads, num_kv_heads, head_dim, groups, bt_width, block_size, q_dtype, kv_dtype, prompt != 0)) {
+                const int64_t need = prefix_mfma_plan(rows, num_q_heads, num_kv_heads, head_dim, groups, bt_width, block_size,
+                                                      q_dtype, prompt != 0).bytes;
+                bytes = bytes > need ? bytes : need;
+            }
+    return bytes;
 }
 
 extern "C" int kvfp8_shared_prefix_decode(
@@ -360,9 +407,7 @@ extern "C" int kvfp8_shared_prefix_decode(
     a.d.ctx = context_lengths;
     a.d.slots64 = slots_dtype == KVFP8_I64;
     a.d.ctx64 = ctx_dtype == KVFP8_I64;
-    const PrefixPlan p = make_plan(batch, num_q_heads, head_dim, bt_width, block_size, false);
-    if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return KVFP8_EWORKSPACE;
-    return run_generic(a, p, q_dtype, kv_dtype, workspace, reinterpret_cast<hipStream_t>(stream));
+    return run(a, q_dtype, kv_dtype, workspace, workspace_bytes, stream);
 }
 
 extern "C" int kvfp8_shared_prefix_prefill(
@@ -388,7 +433,5 @@ extern "C" int kvfp8_shared_prefix_prefill(
     a.seqs = batch;
     a.max_len = max_seq_len;
     a.lse = lse;
-    const PrefixPlan p = make_plan(rows, num_q_heads, head_dim, bt_width, block_size, true);
-    if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return KVFP8_EWORKSPACE;
-    return run_generic(a, p, q_dtype, kv_dtype, workspace, reinterpret_cast<hipStream_t>(stream));
+    return run(a, q_dtype, kv_dtype, workspace, workspace_bytes, stream);
 }

@@ -120,4 +120,6 @@ def test_workspace_size_depends_on_shapes_only():
     fn = _native.lib().kvfp8_shared_prefix_workspace_bytes
     for prompt in (0, 1):
         assert fn(4, 8, 2, 64, 1, 64, 16, _native.E4M3FN, prompt) == fn(4, 8, 2, 64, 1, 64, 16, _native.E4M3FN, prompt) >= 0
+        # A batch without groups, down to fewer pairs than a row block holds.
+        assert fn(1, 2, 2, 64, 0, 64, 16, _native.E4M3FN, prompt) >= 0
     assert fn(0, 8, 2, 64, 1, 64, 16, _native.E4M3FN, 0) == 0
