@@ -78,37 +78,11 @@ __device__ __forceinline__ f32x4_t mma(const Opnd<kSplit>& a, const Opnd<kSplit>
     return c;
 }
 
-// The element is passed by value: clang's __builtin_bit_cast applied directly to an
-// element of an ext_vector_type reads element 0.
-__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
-
 __device__ __forceinline__ uint32_t bf16_bits(float x) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x);
 }
 __device__ __forceinline__ uint32_t f16_bits(float x) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x);
-}
-
-// Maximum over lanes l, l ^ 16, l ^ 32 and l ^ 48. Each permlane swap leaves the
-// values of a lane pair (l, l ^ 16), then (l, l ^ 32), in the two results, so
-// their maximum is the pair's in every lane; no LDS round trip.
-__device__ __forceinline__ float max_across_rows(float x) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const float y = fmaxf(as_float(a[0]), as_float(a[1]));
-    const uint32_t v = __builtin_bit_cast(uint32_t, y);
-    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return fmaxf(as_float(b[0]), as_float(b[1]));
-}
-
-// Sum over the same four lanes (equal in all four: float addition commutes).
-__device__ __forceinline__ float sum_across_rows(float x) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const float y = as_float(a[0]) + as_float(a[1]);
-    const uint32_t v = __builtin_bit_cast(uint32_t, y);
-    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return as_float(b[0]) + as_float(b[1]);
 }
 
 // Eight floats -> operand (bf16, or f16 for f16 inputs; split for float32).
@@ -514,18 +488,6 @@ __device__ __forceinline__ bool fa_item(const PrefillArgs& a, const FaSchedule& 
         it.n_kv = (min(L, r0 + a.rows) + kKeys - 1) / kKeys;
         return true;
     }
-}
-
-// c += a b over 16 dims (lane l: A[l % 16][4 (l / 16) + i], B likewise).
-template <bool kF16>
-__device__ __forceinline__ f32x4_t mma16_half(uint2 a, uint2 b, f32x4_t c) {
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-    if constexpr (kF16)
-        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0,
-                                                         0, 0);
 }
 
 // x c + y with the product rounded: 0 where y is the negated rounded product, whatever its size.

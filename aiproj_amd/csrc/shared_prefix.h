@@ -23,6 +23,7 @@ struct PrefixArgs {
     int32_t seqs;
     int32_t max_len;            // prompt form: rows of a sequence past it are left alone
     int32_t splits;             // states per row, [splits][rows][Hq] in d.part_*
+    int32_t split_step;         // tokens that a split's bounds are multiples of
     float* lse;                 // prompt form [rows, Hq]
 };
 
@@ -78,7 +79,8 @@ __device__ __forceinline__ int64_t prefix_part(const PrefixArgs& a, int64_t row,
 bool prefix_mfma_supported(int32_t head_dim, int32_t block_size, int q_dtype, int kv_dtype);
 
 struct PrefixMfmaPlan {
-    int32_t splits;
+    bool wide;                                    // blocks of 256 rows that share their tokens through LDS
+    int32_t splits, split_step;
     int64_t states;
     int64_t own_plan, seq_m, seq_l, seq_acc;      // decode form: the decode kernel's workspace, whole states
     int64_t part_m, part_l, part_acc;             // the prefix's states
@@ -86,6 +88,17 @@ struct PrefixMfmaPlan {
 };
 PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t groups,
                                 int64_t bt_width, int32_t block_size, int q_dtype, bool prompt);
+
+// Workgroups of a prefix kernel.
+struct PrefixGrid {
+    int32_t blocks;                   // row blocks, at most
+    int32_t total;                    // workgroups: blocks x KV heads x splits
+    int32_t per_xcd;                  // total / 8, rounded up
+};
+
+constexpr int kWideRows = 256;
+template <int QT>
+hipError_t launch_prefix_wide(const PrefixArgs& a, int kv_dtype, const PrefixGrid& g, int q_vec, hipStream_t s);
 
 template <int QT>
 hipError_t launch_prefix_mfma(PrefixArgs a, int kv_dtype, const PrefixMfmaPlan& p, void* workspace, hipStream_t s);

@@ -14,8 +14,7 @@
 // Operand types: bf16 q over e4m3fn codes bf16 throughout; f16 q multiplies codes widened to f16 (exact),
 // its P' enters as two bf16 parts (an f16 P' would lose scales outside f16's range); float32 q and its P'
 // as three bf16 parts; bf16 and f16 caches with q of their type are operands as they are.
-#include "decode_mfma_kernels.h"
-#include "shared_prefix.h"
+#include "shared_prefix_blocks.h"
 
 namespace kvfp8 {
 
@@ -24,7 +23,6 @@ namespace {
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kXcds = 8;              // workgroups are dispatched round-robin over the XCDs
 
 template <int QT, int ES>
 struct Kinds {
@@ -57,61 +55,6 @@ struct PrefixStep {
     uint32_t v[8][C * ES];            // token 4 (l / 16) + i % 4 of tile i / 4, 4 C elements at 4 C (l % 16)
     float sc;                         // e4m3fn: lane l holds the [k|v][tile A|B][token l % 16] scale
 };
-
-struct PrefixGrid {
-    int32_t blocks;                   // row blocks, at most
-    int32_t total;                    // workgroups: blocks x KV heads x splits
-    int32_t per_xcd;                  // total / 8, rounded up
-};
-
-// A row block: rows [rs, re) of q in group g, from pair r0 on.
-struct RowBlock {
-    int32_t g;
-    int64_t rs, re;
-    int64_t r0;
-};
-
-// First q row of group boundary i (entry i of starts).
-__device__ __forceinline__ int64_t group_row(const PrefixArgs& a, int i) {
-    int64_t b = load_i(a.p_starts, a.p_starts64, i);
-    const int64_t seqs = a.cu == nullptr ? a.rows : a.seqs;
-    b = b < 0 ? 0 : (b > seqs ? seqs : b);
-    if (a.cu == nullptr) return b;
-    const int64_t row = load_i(a.cu, a.cu64, b);
-    return row < 0 ? 0 : (row > a.rows ? a.rows : row);
-}
-
-// Row block `index` of the groups' blocks in their order; false past the last one. Whole waves.
-__device__ __forceinline__ bool find_block(const PrefixArgs& a, int32_t index, int rows_per_block, int heads, RowBlock& out) {
-    const int lane = threadIdx.x & 63;
-    int64_t left = index;
-    for (int g0 = 0; g0 < a.groups; g0 += 64) {
-        const int g = g0 + lane;
-        int64_t rs = 0, re = 0;
-        if (g < a.groups) {
-            rs = group_row(a, g);
-            re = group_row(a, g + 1);
-        }
-        const int64_t blocks = re > rs ? ((re - rs) * heads + rows_per_block - 1) / rows_per_block : 0;
-        int64_t incl = blocks;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int64_t y = __shfl_up((long long)incl, off);
-            if (lane >= off) incl += y;
-        }
-        const uint64_t over = __ballot(incl > left);
-        if (over != 0) {
-            const int at = __builtin_ctzll(over);
-            out.g = g0 + at;
-            out.rs = uniform64(__shfl((long long)rs, at));
-            out.re = uniform64(__shfl((long long)re, at));
-            out.r0 = uniform64((left - __shfl((long long)(incl - blocks), at)) * rows_per_block);
-            return true;
-        }
-        left -= __shfl((long long)incl, 63);
-    }
-    return false;
-}
 
 template <int C, int ES>
 __device__ __forceinline__ void load_prefix_step(PrefixStep<C, ES>& s, const DecodeArgs& d, int h, const TileRef& ta,
@@ -314,27 +257,16 @@ prefix_mfma_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
     constexpr int kVals = 4 * NB + 2;
     __shared__ float4 stage_all[kWaves][16];
     __shared__ float merge[kWaves / 2][kVals][64];
-    // Each XCD takes one run of (split, KV head, row block): the blocks of one head and split meet their
-    // tokens in the same L2.
-    const int32_t index = (int32_t)(blockIdx.x % kXcds) * grid.per_xcd + (int32_t)(blockIdx.x / kXcds);
-    if (index >= grid.total || (int32_t)(blockIdx.x / kXcds) >= grid.per_xcd) return;
-    const int32_t unit = index / grid.blocks, block = index - unit * grid.blocks;
-    const int h = unit % a.d.num_kv_heads, split = unit / a.d.num_kv_heads;
+    PrefixItem it;
+    if (!prefix_item(a, grid, 16 * RT, it)) return;
+    const RowBlock& rb = it.rb;
+    const int h = it.h, split = it.split;
     const int G = a.d.num_q_heads / a.d.num_kv_heads;
-    RowBlock rb;
-    if (!find_block(a, block, 16 * RT, G, rb)) return;
-    int64_t slot;
-    const int64_t tokens = group_tokens(a, rb.g, &slot);
-    int64_t lo, hi;
-    split_range(tokens, 32, a.splits, split, &lo, &hi);
-    if (lo >= hi) return;
-    lo = uniform64(lo);
-    hi = uniform64(hi);
-    const int32_t* table = a.d.block_table + uniform64(slot) * a.d.bt_width;
+    const int64_t lo = it.lo, hi = it.hi, pairs = it.pairs;
+    const int32_t* table = it.table;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int m16 = lane & 15, j = lane >> 4;
     const int D = a.d.head_dim;
-    const int64_t pairs = (rb.re - rb.rs) * G;
 
     auto issue = [&](PrefixStep<C, ES>& dst, int64_t t0, TileRef& ra, TileRef& rb2) __attribute__((always_inline)) {
         auto ref = [&](int64_t tok) __attribute__((always_inline)) {
@@ -561,7 +493,7 @@ prefix_mfma_join_kernel(PrefixArgs a, MfmaArgs own) {
 #pragma unroll 4
         for (int s = po; s < a.splits; s += kPass) {
             int64_t lo, hi;
-            split_range(tokens, 32, a.splits, s, &lo, &hi);
+            split_range(tokens, a.split_step, a.splits, s, &lo, &hi);
             if (lo < hi) add_state(a.d.part_m, a.d.part_l, a.d.part_acc, prefix_part(a, row, s, hq));
         }
     }
@@ -586,6 +518,9 @@ prefix_mfma_join_kernel(PrefixArgs a, MfmaArgs own) {
 // ------------------------------------------------------------------ host
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Pairs of an average group from which blocks of 256 rows are taken.
+constexpr int64_t kWidePairs = 128;
 
 template <int C, int QT> constexpr int kTiles = C == 2 || QT == KVFP8_F32 ? 1 : 2;
 
@@ -614,9 +549,12 @@ hipError_t launch_join(const PrefixArgs& a, const MfmaArgs& own, hipStream_t s) 
     return hipGetLastError();
 }
 
-int tiles_of(int32_t head_dim, int q_dtype) { return head_dim > 64 || q_dtype == KVFP8_F32 ? 1 : 2; }
+int rows_per_block(int32_t head_dim, int q_dtype, bool wide) {
+    return wide ? kWideRows : (head_dim > 64 || q_dtype == KVFP8_F32 ? 16 : 32);
+}
 
-int64_t row_blocks(int64_t rows, int32_t heads, int32_t groups, int tiles) { return rows * heads / (16 * tiles) + groups; }
+// At most this many row blocks: every group may leave its last one unfilled.
+int64_t row_blocks(int64_t rows, int32_t heads, int32_t groups, int per_block) { return rows * heads / per_block + groups; }
 
 }  // namespace
 
@@ -629,10 +567,13 @@ bool prefix_mfma_supported(int32_t head_dim, int32_t block_size, int q_dtype, in
 PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t groups,
                                 int64_t bt_width, int32_t block_size, int q_dtype, bool prompt) {
     PrefixMfmaPlan p;
-    const int64_t columns = row_blocks(rows, num_q_heads / num_kv_heads, groups, tiles_of(head_dim, q_dtype)) * num_kv_heads;
-    // One workgroup per CU, each with at least a step for every wave of the longest prefix.
+    const int heads = num_q_heads / num_kv_heads;
+    p.wide = q_dtype != KVFP8_F32 && groups > 0 && rows * heads / groups >= kWidePairs;
+    p.split_step = p.wide ? 64 : 32;
+    const int64_t columns = row_blocks(rows, heads, groups, rows_per_block(head_dim, q_dtype, p.wide)) * num_kv_heads;
+    // One workgroup per CU, each with at least 256 tokens of the longest prefix.
     int64_t splits = columns > 0 ? (device_cus() + columns / 2) / columns : 1;      // no group: no column
-    const int64_t most = bt_width * block_size / (32 * kWaves);
+    const int64_t most = bt_width * block_size / 256;
     splits = splits < most ? splits : most;
     p.splits = (int32_t)(splits < 1 ? 1 : splits);
     p.states = prompt && p.splits == 1 ? 0 : rows * num_q_heads * p.splits;
@@ -659,6 +600,7 @@ template <int QT>
 hipError_t launch_prefix_mfma(PrefixArgs a, int kv_dtype, const PrefixMfmaPlan& p, void* workspace, hipStream_t s) {
     char* ws = reinterpret_cast<char*>(workspace);
     a.splits = p.splits;
+    a.split_step = p.split_step;
     a.d.part_m = reinterpret_cast<float*>(ws + p.part_m);
     a.d.part_l = reinterpret_cast<float*>(ws + p.part_l);
     a.d.part_acc = reinterpret_cast<float*>(ws + p.part_acc);
@@ -680,13 +622,16 @@ hipError_t launch_prefix_mfma(PrefixArgs a, int kv_dtype, const PrefixMfmaPlan& 
     }
     if (a.groups > 0) {
         PrefixGrid g;
-        g.blocks = (int32_t)row_blocks(a.rows, a.d.num_q_heads / a.d.num_kv_heads, a.groups, tiles_of(a.d.head_dim, QT));
+        g.blocks = (int32_t)row_blocks(a.rows, a.d.num_q_heads / a.d.num_kv_heads, a.groups,
+                                       rows_per_block(a.d.head_dim, QT, p.wide));
         const int64_t total = (int64_t)g.blocks * a.d.num_kv_heads * p.splits;
         g.total = (int32_t)total;
         g.per_xcd = (int32_t)((total + kXcds - 1) / kXcds);
         const int64_t q_size = QT == KVFP8_F32 ? 4 : 2;
         const int q_vec = (uintptr_t)a.d.q % 16 == 0 && a.d.q_stride_b * q_size % 16 == 0 && a.d.q_stride_h * q_size % 16 == 0;
-        const hipError_t err = launch_prefix_kv<QT>(a, kv_dtype, g, q_vec, s);
+        hipError_t err;
+        if constexpr (QT == KVFP8_F32) err = launch_prefix_kv<QT>(a, kv_dtype, g, q_vec, s);
+        else err = p.wide ? launch_prefix_wide<QT>(a, kv_dtype, g, q_vec, s) : launch_prefix_kv<QT>(a, kv_dtype, g, q_vec, s);
         if (err != hipSuccess) return err;
     }
     if (a.cu == nullptr) return launch_join<QT, true>(a, own, s);

@@ -29,6 +29,7 @@ BATCHES = {
     "alone": ([7, 0, 40], [], [], 0),
     "long": ([2, 600, 0], [5003], [3], 0),
     "many": ([(7 * i) % 50 for i in range(75)], [129, 31, 512], [40, 1, 30], 2),
+    "crowded": ([(5 * i) % 23 for i in range(140)], [1000, 45], [100, 37], 1),
 }
 
 
