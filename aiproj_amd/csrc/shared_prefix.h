@@ -23,7 +23,7 @@ struct PrefixArgs {
     int32_t seqs;
     int32_t max_len;            // prompt form: rows of a sequence past it are left alone
     int32_t splits;             // states per row, [splits][rows][Hq] in d.part_*
-    int32_t split_step;         // tokens that a split's bounds are multiples of
+    int32_t step_shift;         // splits hold whole steps of 1 << step_shift tokens
     float* lse;                 // prompt form [rows, Hq]
 };
 
@@ -62,13 +62,13 @@ __device__ __forceinline__ int64_t seq_of_row(const PrefixArgs& a, int64_t row) 
     return s0 <= row && row < load_i(a.cu, a.cu64, b + 1) && row - s0 < a.max_len ? b : -1;
 }
 
-// Tokens [lo, hi) of split s of n, in units of `step` tokens.
-__device__ __forceinline__ void split_range(int64_t n, int step, int splits, int s, int64_t* lo, int64_t* hi) {
-    const int64_t units = (n + step - 1) / step;
-    *lo = units * s / splits * step;
-    const int64_t end = units * (s + 1) / splits * step;
-    *hi = end < n ? end : n;
+// Tokens per split of n tokens: equal runs of whole steps (1 << step_shift tokens), the last ones shorter
+// or empty. Splits from split_count on are empty.
+__device__ __forceinline__ int64_t split_tokens(int64_t n, int step_shift, int splits) {
+    const uint32_t steps = (uint32_t)((n + (1 << step_shift) - 1) >> step_shift);
+    return (int64_t)((steps + splits - 1) / (uint32_t)splits) << step_shift;
 }
+__device__ __forceinline__ int split_count(int64_t n, int64_t per) { return n > 0 ? (int)((uint32_t)(n + per - 1) / (uint32_t)per) : 0; }
 
 __device__ __forceinline__ int64_t prefix_part(const PrefixArgs& a, int64_t row, int s, int hq) {
     return (s * a.rows + row) * a.d.num_q_heads + hq;
@@ -80,7 +80,7 @@ bool prefix_mfma_supported(int32_t head_dim, int32_t block_size, int q_dtype, in
 
 struct PrefixMfmaPlan {
     bool wide;                                    // blocks of 256 rows that share their tokens through LDS
-    int32_t splits, split_step;
+    int32_t splits, step_shift;
     int64_t states;
     int64_t own_plan, seq_m, seq_l, seq_acc;      // decode form: the decode kernel's workspace, whole states
     int64_t part_m, part_l, part_acc;             // the prefix's states

@@ -79,8 +79,8 @@ prefix_generic_kernel(PrefixArgs a) {
         else if (prefix == 0) continue;                  // out and lse stand
         const int32_t* p_table = a.d.block_table + p_slot * a.d.bt_width;
         const int32_t* o_table = a.d.block_table + o_slot * a.d.bt_width;
-        int64_t lo, hi;
-        split_range(prefix + own, 64, a.splits, split, &lo, &hi);
+        const int64_t per = split_tokens(prefix + own, a.step_shift, a.splits);
+        const int64_t lo = split * per, hi = min(lo + per, prefix + own);
         const int h = hq / (a.d.num_q_heads / hkv);
         float* q = q_lds[wave];
         for (int d = lane; d < D; d += 64)
@@ -315,6 +315,7 @@ int shared_args(PrefixArgs& a, const void* q, int q_dtype, int64_t q_stride_t, i
 
 int run_generic(PrefixArgs& a, const PrefixPlan& p, int q_dtype, int kv_dtype, void* workspace, hipStream_t s) {
     a.splits = p.splits;
+    a.step_shift = 6;
     const size_t states = (size_t)a.rows * a.d.num_q_heads * p.splits;
     char* ws = reinterpret_cast<char*>(workspace);
     a.d.part_m = reinterpret_cast<float*>(ws);

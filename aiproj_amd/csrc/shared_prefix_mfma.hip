@@ -259,17 +259,16 @@ prefix_mfma_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
     __shared__ float merge[kWaves / 2][kVals][64];
     PrefixItem it;
     if (!prefix_item(a, grid, 16 * RT, it)) return;
-    const RowBlock& rb = it.rb;
     const int h = it.h, split = it.split;
-    const int G = a.d.num_q_heads / a.d.num_kv_heads;
-    const int64_t lo = it.lo, hi = it.hi, pairs = it.pairs;
+    const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
+    const int32_t lo = it.lo, hi = it.hi;
     const int32_t* table = it.table;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int m16 = lane & 15, j = lane >> 4;
     const int D = a.d.head_dim;
 
-    auto issue = [&](PrefixStep<C, ES>& dst, int64_t t0, TileRef& ra, TileRef& rb2) __attribute__((always_inline)) {
-        auto ref = [&](int64_t tok) __attribute__((always_inline)) {
+    auto issue = [&](PrefixStep<C, ES>& dst, int32_t t0, TileRef& ra, TileRef& rb2) __attribute__((always_inline)) {
+        auto ref = [&](int32_t tok) __attribute__((always_inline)) {
             // Wave-uniform scalar load of the table: its wait leaves the loads in flight alone.
             const int64_t addr = uniform64((int64_t)(uintptr_t)(table + (tok >> a.d.bs_shift)));
             const int64_t phys = *(const_i32_ptr)(uintptr_t)addr;
@@ -282,17 +281,17 @@ prefix_mfma_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
     };
     PrefixStep<C, ES> buf0, buf1;
     TileRef r0a, r0b, r1a, r1b;
-    const int64_t stride = 32 * kWaves;
-    int64_t tok = lo + 32 * wave;
+    const int32_t stride = 32 * kWaves;
+    int32_t tok = lo + 32 * wave;
     if (tok < hi) issue(buf0, tok, r0a, r0b);
 
     // Q^T operands: column l % 16 of tile rt is pair r0 + 16 rt + l % 16 (rows past the last repeat it).
     OpT<K::kF16> q[RT][K::kQParts][2 * C];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int64_t pair = min(rb.r0 + 16 * rt + m16, pairs - 1);
-        const int64_t t = pair / G;
-        const T* src = reinterpret_cast<const T*>(a.d.q) + (rb.rs + t) * a.d.q_stride_b + (h * G + (pair - t * G)) * a.d.q_stride_h;
+        const int32_t pair = min(it.r0 + 16 * rt + m16, it.pairs - 1);
+        const int32_t t = (uint32_t)pair / (uint32_t)G;
+        const T* src = reinterpret_cast<const T*>(a.d.q) + (int64_t)(it.rs + t) * a.d.q_stride_b + (h * G + (pair - t * G)) * a.d.q_stride_h;
 #pragma unroll
         for (int kb = 0; kb < 2 * C; ++kb) {
             const int dim = ES == 1 ? 64 * (kb >> 1) + 16 * j + 8 * (kb & 1) : 32 * kb + 8 * j;
@@ -338,9 +337,9 @@ prefix_mfma_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
         st.m[rt] = kNegInf;
         st.l[rt] = 0.0f;
     }
-    auto compute = [&](const PrefixStep<C, ES>& cur, int64_t t0, const TileRef& ra, const TileRef& rb2) __attribute__((always_inline)) {
-        const int lim_a = ra.valid ? (int)min((int64_t)16, hi - t0) : 0;
-        const int lim_b = rb2.valid ? (int)min((int64_t)16, hi - t0 - 16) : 0;
+    auto compute = [&](const PrefixStep<C, ES>& cur, int32_t t0, const TileRef& ra, const TileRef& rb2) __attribute__((always_inline)) {
+        const int lim_a = ra.valid ? min(16, hi - t0) : 0;
+        const int lim_b = rb2.valid ? min(16, hi - t0 - 16) : 0;
         prefix_step<C, QT, ES, RT>(st, cur, q, stage_all[wave], lane, lim_a, lim_b, a.d.score_scale);
     };
     while (tok < hi) {
@@ -390,10 +389,11 @@ prefix_mfma_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
         float l = st.l[rt] + __shfl_xor(st.l[rt], 16);
         l += __shfl_xor(l, 32);
         float m = st.m[rt];
-        const int64_t pair = rb.r0 + 16 * rt + m16;
-        if (pair >= pairs) continue;
-        const int64_t t = pair / G, row = rb.rs + t;
-        const int hq = h * G + (int)(pair - t * G);
+        const int32_t pair = it.r0 + 16 * rt + m16;
+        if (pair >= it.pairs) continue;
+        const int32_t t = (uint32_t)pair / (uint32_t)G;
+        const int64_t row = it.rs + t;
+        const int hq = h * G + (pair - t * G);
         if (a.cu != nullptr && a.splits == 1) {
             // The prompt form's only state of the row: joined with out and lse at once.
             if (seq_of_row(a, row) < 0) continue;
@@ -444,10 +444,10 @@ prefix_mfma_join_kernel(PrefixArgs a, MfmaArgs own) {
     using T = typename Elem<QT>::T;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int D = a.d.head_dim;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
-    if (unit >= a.rows * a.d.num_q_heads) return;
-    const int64_t row = unit / a.d.num_q_heads;
-    const int hq = (int)(unit - row * a.d.num_q_heads);
+    const int32_t unit = (int32_t)blockIdx.x * 4 + wave;      // below 2^26
+    if (unit >= (int32_t)a.rows * a.d.num_q_heads) return;
+    const int32_t row = (uint32_t)unit / (uint32_t)a.d.num_q_heads;
+    const int32_t hq = unit - row * a.d.num_q_heads;
     const int64_t seq = seq_of_row(a, row);
     if (seq < 0) return;
     const int g = group_of_seq(a, seq);
@@ -478,7 +478,7 @@ prefix_mfma_join_kernel(PrefixArgs a, MfmaArgs own) {
             const int64_t total = own.plan[a.d.batch], groups = own.plan[a.d.batch + 1];
             const int32_t w0 = uniform(group_of(t0, total, groups)), w1 = uniform(group_of(t1 - 1, total, groups));
             if (w0 == w1) {
-                if (po == 0) add_state(own.seq_m, own.seq_l, own.seq_acc, row * a.d.num_q_heads + hq);
+                if (po == 0) add_state(own.seq_m, own.seq_l, own.seq_acc, unit);
             } else {
                 const int32_t cut0 = floor_div((int64_t)w0 * total, groups) < t0 ? 1 : 0;
 #pragma unroll 4
@@ -488,21 +488,16 @@ prefix_mfma_join_kernel(PrefixArgs a, MfmaArgs own) {
             }
         }
     }
-    if (tokens > 0) {
-        // Splits without tokens left no state.
+    // Splits without tokens left no state.
+    const int held = split_count(tokens, split_tokens(tokens, a.step_shift, a.splits));
 #pragma unroll 4
-        for (int s = po; s < a.splits; s += kPass) {
-            int64_t lo, hi;
-            split_range(tokens, a.split_step, a.splits, s, &lo, &hi);
-            if (lo < hi) add_state(a.d.part_m, a.d.part_l, a.d.part_acc, prefix_part(a, row, s, hq));
-        }
-    }
+    for (int s = po; s < held; s += kPass) add_state(a.d.part_m, a.d.part_l, a.d.part_acc, prefix_part(a, row, s, hq));
 #pragma unroll
     for (int off = kLanes; off < 64; off <<= 1)
         add(__shfl_xor(mr, off), __shfl_xor(den, off),
             make_float4(__shfl_xor(num.x, off), __shfl_xor(num.y, off), __shfl_xor(num.z, off), __shfl_xor(num.w, off)));
     if (po != 0 || 4 * (lane % kLanes) >= D) return;
-    const int64_t at = row * a.d.num_q_heads + hq;
+    const int64_t at = unit;
     T* out = reinterpret_cast<T*>(a.d.out) + at * D + 4 * d4;
     if constexpr (!kOwn) {
         add(a.lse[at] * kLog2e, 1.0f,
@@ -569,7 +564,7 @@ PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_k
     PrefixMfmaPlan p;
     const int heads = num_q_heads / num_kv_heads;
     p.wide = q_dtype != KVFP8_F32 && groups > 0 && rows * heads / groups >= kWidePairs;
-    p.split_step = p.wide ? 64 : 32;
+    p.step_shift = p.wide ? 6 : 5;
     const int64_t columns = row_blocks(rows, heads, groups, rows_per_block(head_dim, q_dtype, p.wide)) * num_kv_heads;
     // One workgroup per CU, each with at least 256 tokens of the longest prefix.
     int64_t splits = columns > 0 ? (device_cus() + columns / 2) / columns : 1;      // no group: no column
@@ -600,7 +595,7 @@ template <int QT>
 hipError_t launch_prefix_mfma(PrefixArgs a, int kv_dtype, const PrefixMfmaPlan& p, void* workspace, hipStream_t s) {
     char* ws = reinterpret_cast<char*>(workspace);
     a.splits = p.splits;
-    a.split_step = p.split_step;
+    a.step_shift = p.step_shift;
     a.d.part_m = reinterpret_cast<float*>(ws + p.part_m);
     a.d.part_l = reinterpret_cast<float*>(ws + p.part_l);
     a.d.part_acc = reinterpret_cast<float*>(ws + p.part_acc);

@@ -11,8 +11,16 @@
 // The vector ALU bounds it: nine operations a score, one of them the exponential at a quarter rate.
 //
 // LDS rows are 16-byte chunks at position chunk ^ (row % chunks per row), so that the 16 rows of an operand
-// read lie in different bank groups. Two buffers: block g + 1 is written while g is read, its bytes were
-// loaded into registers during g - 1.
+// read lie in different bank groups.
+//
+// Waves w and w + 4 share a SIMD and alternate between a phase on the matrix cores (PV of block g - 1, QK of
+// block g) and one on the vector ALU (softmax of block g), half a step apart, with a barrier after each phase:
+//   phase 2 g       waves 0..3: PV(g - 1), QK(g)    waves 4..7: softmax(g - 1)
+//   phase 2 g + 1   waves 0..3: softmax(g)          waves 4..7: PV(g - 1), QK(g)
+// so K(g) and V(g - 1) are read in phases 2 g and 2 g + 1. In its matrix phase of step g a wave moves its part of
+// K(g + 1) and V(g) from registers to the buffers that K(g - 1) and V(g - 2) have left, and issues the loads of
+// K(g + 2) and V(g + 1). Scales and counts (softmax(g) of waves 4..7 reads them in phase 2 g + 2, when waves 0..3
+// write those of g + 2) have four buffers.
 #include "mfma_tiles.h"
 #include "shared_prefix_blocks.h"
 
@@ -61,73 +69,83 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
     constexpr int TILES = LOADS >= 4 ? 2 : 1;            // tiles a wave loads from
     __shared__ __attribute__((aligned(16))) uint8_t lds_k[2][kKeys * ROW];
     __shared__ __attribute__((aligned(16))) uint8_t lds_v[2][kKeys * ROW];
-    __shared__ __attribute__((aligned(16))) float lds_scale[2][2][kKeys];
-    __shared__ __attribute__((aligned(16))) int32_t lds_count[2][4];      // tokens of each tile that count
+    __shared__ __attribute__((aligned(16))) float lds_scale[4][2][kKeys];
+    __shared__ __attribute__((aligned(16))) int32_t lds_count[4][4];      // tokens of each tile that count
 
     PrefixItem it;
     if (!prefix_item(a, grid, kWideRows, it)) return;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int m16 = lane & 15, j = lane >> 4;
-    const int G = a.d.num_q_heads / a.d.num_kv_heads, h = it.h;
-    const int32_t blocks = (int32_t)((it.hi - it.lo + kKeys - 1) / kKeys);
-    const int64_t r0 = it.rb.r0 + 32 * wave;             // first pair of the wave
+    const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
+    const int h = it.h;
+    const int32_t blocks = (it.hi - it.lo + kKeys - 1) / kKeys;
+    const int32_t r0 = it.r0 + 32 * wave;                // first pair of the wave
     const bool active = r0 < it.pairs;
 
     // Row and tensor of load i of this thread; the tile of its wave's rows.
-    auto slot_of = [&](int i) __attribute__((always_inline)) { return (int)threadIdx.x + kWideThreads * i; };
-    auto row_of = [&](int i) __attribute__((always_inline)) { return slot_of(i) % PER / SLOTS; };
+    auto row_of = [&](int i) __attribute__((always_inline)) { return ((int)threadIdx.x + kWideThreads * i) % PER / SLOTS; };
     auto wave_row = [&](int i) __attribute__((always_inline)) { return (64 * wave + kWideThreads * i) % PER / SLOTS; };
     const int run = threadIdx.x % SLOTS;
     const int64_t row_bytes = (int64_t)a.d.num_kv_heads * kD * ES;
-    // Scales: lanes 0..15 of a wave load those of the rows it loads (head size 64: 16 rows of one tensor,
-    // else 8 rows of both).
-    const int s_tensor = kD == 64 ? wave >> 2 : (lane >> 3) & 1;
-    const int s_row = kD == 64 ? 16 * (wave & 3) + m16 : 8 * wave + (lane & 7);
+    // Scales: 16 lanes of a wave load those of the rows of K that it loads and of the same rows of V (head size 64:
+    // 16 rows, lanes 0..31 of the waves that load K).
+    constexpr bool kByWave = LOADS == 1;                 // waves 0..3 load K, 4..7 V
+    const int s_tensor = kByWave ? (lane >> 4) & 1 : (lane >> 3) & 1;
+    const int s_row = kByWave ? 16 * (wave & 3) + m16 : 8 * wave + (lane & 7);
+    const bool s_mine = kByWave ? wave < 4 && lane < 32 : lane < 16;
+    const bool loads_v = kByWave && wave >= 4;
 
-    // The page of the tile of load i in block g; -1 past the prefix.
+    // The page of the tile of load i in block g; past the prefix one of its own (no branch), which counts nothing.
     auto fetch_page = [&](int32_t g, int i) __attribute__((always_inline)) -> int32_t {
-        const int64_t tok = it.lo + (int64_t)g * kKeys + (wave_row(i) & ~15);
-        if (tok >= it.hi) return -1;
-        const int64_t addr = uniform64((int64_t)(uintptr_t)(it.table + (tok >> a.d.bs_shift)));
+        const int32_t tok = it.lo + g * kKeys + (wave_row(i) & ~15);
+        const int64_t addr = uniform64((int64_t)(uintptr_t)(it.table + ((tok < it.hi ? tok : it.lo) >> a.d.bs_shift)));
         return *(const_i32_ptr)(uintptr_t)addr;
+    };
+    int32_t page[TILES];
+    auto fetch = [&](int32_t g) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < TILES; ++u) page[u] = fetch_page(g, u);
     };
     u32x4_t raw[LOADS];
     float scale = 0.0f;
-    int32_t count[TILES];                                // tokens that count in the wave's tiles
-    auto issue = [&](int32_t g, const int32_t (&page)[TILES]) __attribute__((always_inline)) {
-        const int64_t t0 = it.lo + (int64_t)g * kKeys;
-        int64_t base[TILES];                             // first cache row of the tile
+    int64_t base[TILES];                                 // first cache row of the wave's tiles: of the K block in flight
+    int32_t count_k[TILES], count_v[TILES];              // tokens that count in them, of the K and the V block in flight
+    auto locate = [&](int32_t g) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < TILES; ++u) {
-            const int64_t tok = t0 + (wave_row(u) & ~15);
+            const int32_t tok = it.lo + g * kKeys + (wave_row(u) & ~15);
             const bool ok = page[u] >= 0 && page[u] < a.d.num_blocks && tok < it.hi;
-            count[u] = ok ? (int32_t)min((int64_t)16, it.hi - tok) : 0;
+            count_k[u] = ok ? min(16, it.hi - tok) : 0;
             base[u] = ok ? (int64_t)page[u] * a.d.block_size + (tok & (a.d.block_size - 1)) : 0;
         }
+    };
+    auto is_v = [&](int i) __attribute__((always_inline)) { return kByWave ? loads_v : kWideThreads * i >= PER; };
+    auto issue = [&](bool v) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int u = i % TILES;
-            const bool v = slot_of(i) >= PER;
+            if (is_v(i) != v) continue;
             const uint8_t* src = reinterpret_cast<const uint8_t*>(v ? a.d.v_cache : a.d.k_cache) +
-                                 (base[u] + (row_of(i) & 15)) * row_bytes + h * kD * ES + 16 * (run < RUNS ? run : 0);
+                                 (base[i % TILES] + (row_of(i) & 15)) * row_bytes + h * kD * ES + 16 * (run < RUNS ? run : 0);
             raw[i] = *reinterpret_cast<const u32x4_t*>(src);
         }
-        if constexpr (ES == 1) {
-            const int64_t row = base[0] + (s_row & 15);
-            scale = (s_tensor ? a.d.v_scales : a.d.k_scales)[row * a.d.num_kv_heads + h];
+        if (v) {
+#pragma unroll
+            for (int u = 0; u < TILES; ++u) count_v[u] = count_k[u];
+        } else if constexpr (ES == 1) {
+            scale = (s_tensor ? a.d.v_scales : a.d.k_scales)[(base[0] + (s_row & 15)) * a.d.num_kv_heads + h];
         }
     };
     // Rows that do not count become zeros (their bytes may be anything).
-    auto publish = [&](int buf) __attribute__((always_inline)) {
+    auto publish = [&](bool v, int buf, int32_t g) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
+            if (is_v(i) != v) continue;
             const int row = row_of(i);
-            const bool live = (row & 15) < count[i % TILES];
-            uint8_t* dst = (slot_of(i) >= PER ? lds_v[buf] : lds_k[buf]) + row * ROW;
+            const bool live = (row & 15) < (v ? count_v : count_k)[i % TILES];
+            uint8_t* dst = (v ? lds_v[buf] : lds_k[buf]) + row * ROW;
             if (run >= RUNS) continue;
             if constexpr (ES == 1) {
                 u32x4_t x[2];
-                const bool v = slot_of(i) >= PER;        // wave-uniform
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     const uint32_t c = live ? raw[i][w] : 0u;
@@ -146,13 +164,14 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
                 *reinterpret_cast<u32x4_t*>(dst + 16 * (run ^ (row % CPR))) = live ? raw[i] : u32x4_t{0u, 0u, 0u, 0u};
             }
         }
+        if (v) return;
         if constexpr (ES == 1) {
-            const float x = (s_row & 15) < count[0] ? scale : 0.0f;
-            if (lane < 16) lds_scale[buf][s_tensor][s_row] = s_tensor ? x : x * a.d.score_scale;
+            const float x = (s_row & 15) < count_k[0] ? scale : 0.0f;
+            if (s_mine) lds_scale[g & 3][s_tensor][s_row] = s_tensor ? x : x * a.d.score_scale;
         }
 #pragma unroll
         for (int u = 0; u < TILES; ++u)
-            if (lane == 0 && wave_row(u) % 16 == 0) lds_count[buf][wave_row(u) / 16] = count[u];
+            if (lane == 0 && !loads_v && wave_row(u) % 16 == 0) lds_count[g & 3][wave_row(u) / 16] = count_k[u];
     };
 
     // Q^T operands: lane (row 16 qt + l % 16, l / 16) holds dims 32 s + 8 (l / 16) .. + 7 (pairs past the last
@@ -162,9 +181,9 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
     auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int qt = 0; qt < 2; ++qt) {
-            const int64_t pair = min(r0 + 16 * qt + m16, it.pairs - 1);
-            const int64_t t = pair / G;
-            const T* src = reinterpret_cast<const T*>(a.d.q) + (it.rb.rs + t) * a.d.q_stride_b + (h * G + (pair - t * G)) * a.d.q_stride_h;
+            const int32_t pair = min(r0 + 16 * qt + m16, it.pairs - 1);
+            const int32_t t = (uint32_t)pair / (uint32_t)G;
+            const T* src = reinterpret_cast<const T*>(a.d.q) + (int64_t)(it.rs + t) * a.d.q_stride_b + (h * G + (pair - t * G)) * a.d.q_stride_h;
             auto element2 = [&](int d) __attribute__((always_inline)) { return (uint32_t)src[d] | ((uint32_t)src[d + 1] << 16); };
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
@@ -204,11 +223,10 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
         l[qt] = 0.0f;
     }
 
-    auto compute = [&](auto buf_c) __attribute__((always_inline)) {
+    f32x4_t sacc[4][2];
+    auto qk = [&](auto buf_c) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value;
         lds_u8* const kl = (lds_u8*)&lds_k[buf][0];
-        lds_u8* const vl = (lds_u8*)&lds_v[buf][0];
-        f32x4_t sacc[4][2];
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -226,14 +244,17 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
                 for (int qt = 0; qt < 2; ++qt) sacc[kt][qt] = mma16_half<kF16>(kop, qhalf[qt], sacc[kt][qt]);
             }
         }
+    };
+    // P'^T operands; pp holds tokens 16 (2 pp + i / 4) + 4 j + i % 4.
+    u32x4_t pop[2][kParts][2];
+    auto softmax = [&](int32_t g) __attribute__((always_inline)) {
+        const float(*scales)[kKeys] = lds_scale[g & 3];
         // Scaled scores (score i of a row: token 16 (i / 4) + 4 j + i % 4).
-        float4 vs[4];
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
             float4 ks = make_float4(a.d.score_scale, a.d.score_scale, a.d.score_scale, a.d.score_scale);
             if constexpr (ES == 1) {
-                ks = *reinterpret_cast<const float4*>(&lds_scale[buf][0][16 * kt + 4 * j]);
-                vs[kt] = *reinterpret_cast<const float4*>(&lds_scale[buf][1][16 * kt + 4 * j]);
+                ks = *reinterpret_cast<const float4*>(&scales[0][16 * kt + 4 * j]);
             }
 #pragma unroll
             for (int qt = 0; qt < 2; ++qt) {
@@ -243,7 +264,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
                 sacc[kt][qt][3] *= ks.w;
             }
         }
-        const int4 counts = *reinterpret_cast<const int4*>(&lds_count[buf][0]);
+        const int4 counts = *reinterpret_cast<const int4*>(&lds_count[g & 3][0]);
         const int n[4] = {uniform(counts.x), uniform(counts.y), uniform(counts.z), uniform(counts.w)};
         if (n[0] + n[1] + n[2] + n[3] < kKeys) {         // wave-uniform
 #pragma unroll
@@ -269,62 +290,50 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
             }
             neg_m[qt] = m[qt] == kNegInf ? 0.0f : -m[qt];
         }
-        // P'^T operands; pp holds tokens 16 (2 pp + i / 4) + 4 j + i % 4. The second half's probabilities are
-        // computed between the products of the first.
-        u32x4_t pop[2][kParts][2];
-        float pr[2][16];
-        auto prob = [&](int qt, int i) __attribute__((always_inline)) {
-            const float p = __builtin_amdgcn_exp2f(sacc[i / 4][qt][i % 4] + neg_m[qt]);
-            l[qt] += p;
-            if constexpr (ES == 1) {
-                const float4 v = vs[i / 4];
-                pr[qt][i] = p * (i % 4 == 0 ? v.x : i % 4 == 1 ? v.y : i % 4 == 2 ? v.z : v.w);
-            } else {
-                pr[qt][i] = p;
-            }
-        };
-        auto pack_half = [&](int pp) __attribute__((always_inline)) {
 #pragma unroll
-            for (int qt = 0; qt < 2; ++qt)
+        for (int kt = 0; kt < 4; ++kt) {
+            f32x4_t vs = {1.0f, 1.0f, 1.0f, 1.0f};
+            if constexpr (ES == 1) vs = *reinterpret_cast<const f32x4_t*>(&scales[1][16 * kt + 4 * j]);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float x0 = pr[qt][8 * pp + 2 * w], x1 = pr[qt][8 * pp + 2 * w + 1];
-                    const uint32_t top = pack2<kF16V>(x0, x1);
-                    pop[qt][0][pp][w] = top;
-                    if constexpr (kParts == 2)
-                        pop[qt][1][pp][w] = pack2<false>(x0 - bits_f32(top << 16), x1 - bits_f32(top & 0xFFFF0000u));
+            for (int qt = 0; qt < 2; ++qt) {
+                float x[4];
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    const float p = __builtin_amdgcn_exp2f(sacc[kt][qt][jj] + neg_m[qt]);
+                    l[qt] += p;
+                    x[jj] = ES == 1 ? p * vs[jj] : p;
                 }
-        };
-        auto pv = [&](int pp, int nb) __attribute__((always_inline)) {
-            u32x4_t av;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vl + v_off[nb] + 16 * (2 * pp + half) * ROW));
-                const uint2 w = __builtin_bit_cast(uint2, x);
-                av[2 * half] = w.x;
-                av[2 * half + 1] = w.y;
+                for (int w = 0; w < 2; ++w) {
+                    const uint32_t top = pack2<kF16V>(x[2 * w], x[2 * w + 1]);
+                    pop[qt][0][kt >> 1][2 * (kt & 1) + w] = top;
+                    if constexpr (kParts == 2)
+                        pop[qt][1][kt >> 1][2 * (kt & 1) + w] =
+                            pack2<false>(x[2 * w] - bits_f32(top << 16), x[2 * w + 1] - bits_f32(top & 0xFFFF0000u));
+                }
             }
-#pragma unroll
-            for (int qt = 0; qt < 2; ++qt)
-#pragma unroll
-                for (int part = 0; part < kParts; ++part) o[qt][nb] = mma16<kF16V>(av, pop[qt][part][pp], o[qt][nb]);
-        };
-#pragma unroll
-        for (int qt = 0; qt < 2; ++qt)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) prob(qt, i);
-        pack_half(0);
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            pv(0, nb);
-#pragma unroll
-            for (int qt = 0; qt < 2; ++qt)
-#pragma unroll
-                for (int u = 8 * nb / NB; u < 8 * (nb + 1) / NB; ++u) prob(qt, 8 + u);
         }
-        pack_half(1);
+    };
+    auto pv = [&](auto buf_c) __attribute__((always_inline)) {
+        constexpr int buf = decltype(buf_c)::value;
+        lds_u8* const vl = (lds_u8*)&lds_v[buf][0];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) pv(1, nb);
+        for (int pp = 0; pp < 2; ++pp)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                u32x4_t av;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vl + v_off[nb] + 16 * (2 * pp + half) * ROW));
+                    const uint2 w = __builtin_bit_cast(uint2, x);
+                    av[2 * half] = w.x;
+                    av[2 * half + 1] = w.y;
+                }
+#pragma unroll
+                for (int qt = 0; qt < 2; ++qt)
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part) o[qt][nb] = mma16<kF16V>(av, pop[qt][part][pp], o[qt][nb]);
+            }
     };
 
     // A barrier that waits for this wave's LDS operations and leaves its loads in flight.
@@ -334,35 +343,87 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
         __builtin_amdgcn_s_barrier();
         __asm__ volatile("" ::: "memory");
     };
-    int32_t page[TILES];
-    auto fetch = [&](int32_t g) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < TILES; ++u) page[u] = fetch_page(g, u);
-    };
     fetch(0);
-    issue(0, page);
+    locate(0);
+    issue(false);
+    issue(true);
     fetch(1);
     load_q();
-    publish(0);
-    if (blocks > 1) issue(1, page);
+    publish(false, 0, 0);
+    locate(1);
+    issue(false);
     fetch(2);
     barrier();
-    // Step g: block g + 1's bytes go from registers to the other buffer (its last readers passed the barrier of
-    // step g - 1), block g + 2's loads are issued, block g is used; the barrier publishes g + 1.
-    auto step = [&](int32_t g, auto buf_c) __attribute__((always_inline)) {
-        if (g + 1 < blocks) {
-            publish(1 - decltype(buf_c)::value);
-            if (g + 2 < blocks) {
-                issue(g + 2, page);
-                fetch(g + 3);
+    constexpr std::integral_constant<int, 0> b0{};
+    constexpr std::integral_constant<int, 1> b1{};
+    // The matrix phase of step g (buffer of K(g), V(g): g % 2). Past the last block the staging moves rows that count
+    // nothing, so that there is no branch around it.
+    // Operand reads run ahead of the products by up to 16 (an LDS read under this load takes some 200 cycles, a
+    // product 16); left alone, the compiler reads each operand right before its use.
+    constexpr int kReads = 4 * NB + 4 * KS + (kHalf ? 4 : 0), kProducts = 4 * NB * kParts + 8 * KS + (kHalf ? 8 : 0);
+    constexpr int kAhead = 16, kPace = (kProducts - kAhead) / ((kReads - kAhead) / 2);
+    auto matrix = [&](int32_t g, auto buf_c, bool first) __attribute__((always_inline)) {
+        constexpr std::integral_constant<int, 1 - decltype(buf_c)::value> other{};
+        publish(true, decltype(buf_c)::value, g);
+        publish(false, other.value, g + 1);
+        issue(true);
+        locate(g + 2);
+        issue(false);
+        fetch(g + 3);
+        if (!active) return;
+        if (first) {
+            qk(buf_c);
+            return;
+        }
+        pv(other);
+        qk(buf_c);
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);              // LDS reads
+#pragma unroll
+        for (int i = 0; i < (kReads - kAhead) / 2; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, kPace, 0);           // matrix products
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
+    };
+    // Both halves run the same 2 * blocks barriers.
+    if (wave < 4) {
+        matrix(0, b0, true);
+        barrier();
+        if (active) softmax(0);
+        barrier();
+        for (int32_t g = 1; g < blocks; g += 2) {
+            matrix(g, b1, false);
+            barrier();
+            if (active) softmax(g);
+            barrier();
+            if (g + 1 < blocks) {
+                matrix(g + 1, b0, false);
+                barrier();
+                if (active) softmax(g + 1);
+                barrier();
             }
         }
-        if (active) compute(buf_c);
+    } else {
         barrier();
-    };
-    for (int32_t g = 0; g < blocks; g += 2) {
-        step(g, std::integral_constant<int, 0>{});
-        if (g + 1 < blocks) step(g + 1, std::integral_constant<int, 1>{});
+        matrix(0, b0, true);
+        barrier();
+        for (int32_t g = 1; g < blocks; g += 2) {
+            if (active) softmax(g - 1);
+            barrier();
+            matrix(g, b1, false);
+            barrier();
+            if (g + 1 < blocks) {
+                if (active) softmax(g);
+                barrier();
+                matrix(g + 1, b0, false);
+                barrier();
+            }
+        }
+        if (active) softmax(blocks - 1);
+    }
+    if (active) {
+        if ((blocks & 1) != 0) pv(b0);
+        else pv(b1);
     }
     if (!active) return;
 
@@ -370,10 +431,11 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) {
         const float lt = sum_across_rows(l[qt]);
-        const int64_t pair = r0 + 16 * qt + m16;
+        const int32_t pair = r0 + 16 * qt + m16;
         if (pair >= it.pairs) continue;
-        const int64_t t = pair / G, row = it.rb.rs + t;
-        const int hq = h * G + (int)(pair - t * G);
+        const int32_t t = (uint32_t)pair / (uint32_t)G;
+        const int64_t row = it.rs + t;
+        const int hq = h * G + (pair - t * G);
         if (a.cu != nullptr && a.splits == 1) {
             // The prompt form's only state of the row: joined with out and lse at once.
             if (seq_of_row(a, row) < 0) continue;
