@@ -24,16 +24,4 @@ int64_t mfma_workspace_layout(int32_t batch, int32_t num_q_heads, int32_t num_kv
 template <int QT>
 hipError_t launch_mfma_decode(const DecodeArgs& a, int kv_dtype, void* workspace, hipStream_t stream, int phases);
 
-// Softmax states of whole sequences: m and l [batch, Hq], acc [batch, Hq, D].
-struct DecodeStates {
-    float* m;
-    float* l;
-    float* acc;
-};
-
-// The split kernel without outputs: a sequence that one workgroup holds leaves its state in `out`, a cut
-// one its pieces in the workspace (see combine_mfma_kernel for where). bf16 caches with bf16 q only.
-template <int QT>
-hipError_t launch_mfma_states(const DecodeArgs& a, int kv_dtype, void* workspace, const DecodeStates& out, hipStream_t stream);
-
 }  // namespace kvfp8

@@ -22,7 +22,8 @@ struct PrefixArgs {
     int32_t cu64;
     int32_t seqs;
     int32_t max_len;            // prompt form: rows of a sequence past it are left alone
-    int32_t splits;             // states per row, [splits][rows][Hq] in d.part_*
+    int32_t splits;             // states per row of its prefix, and of its own tokens (matrix-core path, decode
+    int32_t own_splits;         // form) behind them: [splits + own_splits][rows][Hq] in d.part_*
     int32_t step_shift;         // splits hold whole steps of 1 << step_shift tokens
     float* lse;                 // prompt form [rows, Hq]
 };
@@ -79,26 +80,30 @@ __device__ __forceinline__ int64_t prefix_part(const PrefixArgs& a, int64_t row,
 bool prefix_mfma_supported(int32_t head_dim, int32_t block_size, int q_dtype, int kv_dtype);
 
 struct PrefixMfmaPlan {
-    bool wide;                                    // blocks of 256 rows that share their tokens through LDS
-    int32_t splits, step_shift;
-    int64_t states;
-    int64_t own_plan, seq_m, seq_l, seq_acc;      // decode form: the decode kernel's workspace, whole states
-    int64_t part_m, part_l, part_acc;             // the prefix's states
-    int64_t bytes;
+    int32_t rows;                     // pairs per row block: 16, 128 or 256
+    int32_t blocks;                   // row blocks, at most
+    int32_t splits, step_shift;       // of a prefix
+    int32_t own_groups, own_heads, own_blocks, own_splits;        // decode form, as in PrefixGrid
+    int64_t states;                   // float32 states: m at 0, l and acc at these byte offsets
+    int64_t part_l, part_acc, bytes;
 };
 PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t groups,
                                 int64_t bt_width, int32_t block_size, int q_dtype, bool prompt);
 
-// Workgroups of a prefix kernel.
+// Workgroups of the launch that leaves states: those of the prefixes, then those of the own tokens.
 struct PrefixGrid {
     int32_t blocks;                   // row blocks, at most
-    int32_t total;                    // workgroups: blocks x KV heads x splits
+    int32_t total;                    // items of the prefixes: blocks x KV heads x splits
     int32_t per_xcd;                  // total / 8, rounded up
+    int32_t prefix_groups;            // workgroups of the prefixes, 8 per_xcd
+    int32_t own_groups;               // workgroups of the own tokens
+    int32_t own_heads;                // KV heads of one of them
+    int32_t own_blocks;               // blocks of 16 q heads of a KV head
+    int32_t q_vec;                    // q rows are 16-byte aligned
 };
 
-constexpr int kWideRows = 256;
 template <int QT>
-hipError_t launch_prefix_wide(const PrefixArgs& a, int kv_dtype, const PrefixGrid& g, int q_vec, hipStream_t s);
+hipError_t launch_prefix_wide(const PrefixArgs& a, int kv_dtype, int rows, const PrefixGrid& g, hipStream_t s);
 
 template <int QT>
 hipError_t launch_prefix_mfma(PrefixArgs a, int kv_dtype, const PrefixMfmaPlan& p, void* workspace, hipStream_t s);

@@ -11,8 +11,6 @@
 // head, split of the row's tokens), on the vector ALU.
 #include "shared_prefix.h"
 
-#include "kvfp8_decode_mfma.h"
-
 namespace kvfp8 {
 
 namespace {
@@ -158,7 +156,7 @@ prefix_generic_kernel(PrefixArgs a) {
 // One wave per (row, q head) joins the states of its splits (and, in the prompt form, out and lse).
 template <int QT, int ND>
 __global__ void __launch_bounds__(64 * kGenWaves)
-prefix_join_kernel(PrefixArgs a) {
+prefix_generic_join_kernel(PrefixArgs a) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int D = a.d.head_dim;
     const int64_t units = a.rows * a.d.num_q_heads;
@@ -241,7 +239,7 @@ hipError_t launch_generic_nd(const PrefixArgs& a, hipStream_t s) {
     const int64_t pairs = a.rows * a.d.num_q_heads;
     const hipError_t err = launch_units(prefix_generic_kernel<KVT, QT, ND>, pairs * a.splits, a, s);
     if (err != hipSuccess || a.splits == 1) return err;
-    return launch_units(prefix_join_kernel<QT, ND>, pairs, a, s);
+    return launch_units(prefix_generic_join_kernel<QT, ND>, pairs, a, s);
 }
 
 template <int KVT, int QT>
@@ -328,14 +326,12 @@ int run_generic(PrefixArgs& a, const PrefixPlan& p, int q_dtype, int kv_dtype, v
     }
 }
 
-// Whether a call runs on the matrix cores: the prefix kernel takes it and, in the decode form, the decode
-// kernel its own tokens.
-bool mfma_shape(int64_t rows, int32_t hq, int32_t hkv, int32_t d, int32_t groups, int64_t bt_width, int32_t bs, int q_dtype,
-                int kv_dtype, bool prompt) {
+// Whether a call runs on the matrix cores.
+bool mfma_shape(int64_t rows, int32_t hq, int32_t hkv, int32_t d, int32_t groups, int32_t bs, int q_dtype, int kv_dtype) {
     if (!prefix_mfma_supported(d, bs, q_dtype, kv_dtype)) return false;
-    // Workgroups are counted in int32, and a launch has fewer than 2^32 threads.
-    if (rows * hq / 16 + (int64_t)groups * hkv >= (1 << 22)) return false;
-    return prompt || mfma_decode_supported((int32_t)rows, hq, hkv, d, bt_width, bs, kv_dtype);
+    // Workgroups (at most a row block of 16 pairs and one of own tokens each, or some hundreds) are counted in int32,
+    // and a launch has fewer than 2^32 threads.
+    return rows * hq < ((int64_t)1 << 22) && (int64_t)groups * hkv < ((int64_t)1 << 21);
 }
 
 template <int QT>
@@ -343,8 +339,7 @@ int run(PrefixArgs& a, int kv_dtype, void* workspace, int64_t workspace_bytes, h
     const bool prompt = a.cu != nullptr;
     const bool aligned = (((uintptr_t)a.d.k_cache | (uintptr_t)a.d.v_cache | (uintptr_t)a.d.out) & 15) == 0;
     if (aligned && a.d.bt_rows < ((int64_t)1 << 26) &&
-        mfma_shape(a.rows, a.d.num_q_heads, a.d.num_kv_heads, a.d.head_dim, a.groups, a.d.bt_width, a.d.block_size, QT, kv_dtype,
-                   prompt)) {
+        mfma_shape(a.rows, a.d.num_q_heads, a.d.num_kv_heads, a.d.head_dim, a.groups, a.d.block_size, QT, kv_dtype)) {
         const PrefixMfmaPlan p = prefix_mfma_plan(a.rows, a.d.num_q_heads, a.d.num_kv_heads, a.d.head_dim, a.groups,
                                                   a.d.bt_width, a.d.block_size, QT, prompt);
         if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return KVFP8_EWORKSPACE;
@@ -380,7 +375,7 @@ extern "C" int64_t kvfp8_shared_prefix_workspace_bytes(int64_t rows, int32_t num
     int64_t bytes = make_plan(rows, num_q_heads, head_dim, bt_width, block_size, prompt != 0).bytes;
     if (num_q_heads % num_kv_heads == 0)
         for (const int q_dtype : {KVFP8_F32, KVFP8_F16, KVFP8_BF16})
-            if (mfma_shape(rows, num_q_heads, num_kv_heads, head_dim, groups, bt_width, block_size, q_dtype, kv_dtype, prompt != 0)) {
+            if (mfma_shape(rows, num_q_heads, num_kv_heads, head_dim, groups, block_size, q_dtype, kv_dtype)) {
                 const int64_t need = prefix_mfma_plan(rows, num_q_heads, num_kv_heads, head_dim, groups, bt_width, block_size,
                                                       q_dtype, prompt != 0).bytes;
                 bytes = bytes > need ? bytes : need;

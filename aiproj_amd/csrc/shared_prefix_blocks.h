@@ -1,7 +1,7 @@
 // Row blocks of the shared-prefix kernels: which rows, tokens and KV head a workgroup takes.
 #pragma once
 
-#include "decode_mfma_kernels.h"
+#include "paged_operands.h"
 #include "shared_prefix.h"
 
 namespace kvfp8 {
@@ -10,15 +10,16 @@ namespace {
 
 constexpr int kXcds = 8;              // workgroups are dispatched round-robin over the XCDs
 
-// What a workgroup does: pairs (token of q, q head of a KV head) of a group from r0 on, against the tokens
-// [lo, hi) of its prefix.
+// What a workgroup does: pairs (token of q, q head of a KV head) of a group or sequence from r0 on, against the
+// tokens [lo, hi) of its prefix or own pages.
 struct PrefixItem {
-    int32_t h, split;
+    int32_t h;                        // (first) KV head
+    int32_t part;                     // where the states go
     int32_t rs;                       // first q row of the group
     int32_t pairs;                    // its pairs
     int32_t r0;                       // first pair of the block
     int32_t lo, hi;
-    const int32_t* table;             // block-table row of the prefix
+    const int32_t* table;             // block-table row
 };
 
 // First q row of group boundary i (entry i of starts).
@@ -39,8 +40,8 @@ __device__ __forceinline__ bool prefix_item(const PrefixArgs& a, const PrefixGri
     const int32_t index = (int32_t)(blockIdx.x % kXcds) * grid.per_xcd + local;
     if (index >= grid.total || local >= grid.per_xcd) return false;
     const int32_t unit = (uint32_t)index / (uint32_t)grid.blocks;
-    it.split = (uint32_t)unit / (uint32_t)a.d.num_kv_heads;
-    it.h = unit - it.split * a.d.num_kv_heads;
+    it.part = (uint32_t)unit / (uint32_t)a.d.num_kv_heads;
+    it.h = unit - it.part * a.d.num_kv_heads;
     const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
     int32_t left = index - unit * grid.blocks;
     const int lane = threadIdx.x & 63;
@@ -67,7 +68,7 @@ __device__ __forceinline__ bool prefix_item(const PrefixArgs& a, const PrefixGri
             it.r0 = (left - __builtin_amdgcn_readlane(incl - blocks, at)) * rows_per_block;
             const int32_t n = __builtin_amdgcn_readlane(tokens, at);
             const int64_t per = split_tokens(n, a.step_shift, a.splits);
-            const int64_t lo = it.split * per;
+            const int64_t lo = it.part * per;
             if (lo >= n) return false;
             it.lo = uniform((int32_t)lo);
             it.hi = uniform((int32_t)min(lo + per, (int64_t)n));
@@ -78,6 +79,33 @@ __device__ __forceinline__ bool prefix_item(const PrefixArgs& a, const PrefixGri
         left -= __builtin_amdgcn_readlane(incl, 63);
     }
     return false;
+}
+
+// Own tokens: block of 16 q heads, KV heads and split of a sequence. Neighbouring workgroups take the heads of the
+// same tokens.
+__device__ __forceinline__ bool own_item(const PrefixArgs& a, const PrefixGrid& grid, PrefixItem& it) {
+    uint32_t index = blockIdx.x - grid.prefix_groups;
+    const uint32_t head_groups = (uint32_t)a.d.num_kv_heads / (uint32_t)grid.own_heads;
+    uint32_t rest = index / head_groups;
+    it.h = (int32_t)(index - rest * head_groups) * grid.own_heads;
+    index = rest;
+    rest = index / (uint32_t)a.own_splits;
+    const int32_t split = (int32_t)(index - rest * (uint32_t)a.own_splits);
+    index = rest;
+    rest = index / (uint32_t)grid.own_blocks;
+    it.r0 = 16 * (int32_t)(index - rest * (uint32_t)grid.own_blocks);
+    it.rs = (int32_t)rest;
+    it.pairs = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
+    it.part = a.splits + split;
+    int64_t slot;
+    const int32_t n = (int32_t)seq_tokens(a.d, it.rs, &slot);
+    const int64_t per = split_tokens(n, 5, a.own_splits);
+    const int64_t lo = split * per;
+    if (lo >= n) return false;
+    it.lo = uniform((int32_t)lo);
+    it.hi = uniform((int32_t)min(lo + per, (int64_t)n));
+    it.table = a.d.block_table + uniform64(slot) * a.d.bt_width;
+    return true;
 }
 
 }  // namespace

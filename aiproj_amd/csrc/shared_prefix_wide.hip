@@ -1,6 +1,6 @@
-// Shared prefixes for many rows: blocks of 256 (row, q head) pairs against a prefix, gfx950.
+// Shared prefixes for many rows: blocks of 256 or 128 (row, q head) pairs against a prefix, gfx950.
 //
-// A workgroup takes one (row block, KV head, split of the prefix). Its eight waves hold 32 rows each and
+// A workgroup takes one (row block, KV head, split of the prefix). Its eight or four waves hold 32 rows each and
 // share the prefix's tokens through LDS in blocks of 64: the codes are widened to 16 bits once per
 // workgroup on their way there (exact), instead of once per wave, and the tokens' bytes cross L2 once per
 // 256 rows. Per block and wave (MFMA 16x16x32, layouts in mfma_tiles.h):
@@ -13,7 +13,7 @@
 // LDS rows are 16-byte chunks at position chunk ^ (row % chunks per row), so that the 16 rows of an operand
 // read lie in different bank groups.
 //
-// Waves w and w + 4 share a SIMD and alternate between a phase on the matrix cores (PV of block g - 1, QK of
+// The two halves of the waves alternate between a phase on the matrix cores (PV of block g - 1, QK of
 // block g) and one on the vector ALU (softmax of block g), half a step apart, with a barrier after each phase:
 //   phase 2 g       waves 0..3: PV(g - 1), QK(g)    waves 4..7: softmax(g - 1)
 //   phase 2 g + 1   waves 0..3: softmax(g)          waves 4..7: PV(g - 1), QK(g)
@@ -21,19 +21,15 @@
 // K(g + 1) and V(g) from registers to the buffers that K(g - 1) and V(g - 2) have left, and issues the loads of
 // K(g + 2) and V(g + 1). Scales and counts (softmax(g) of waves 4..7 reads them in phase 2 g + 2, when waves 0..3
 // write those of g + 2) have four buffers.
-#include "mfma_tiles.h"
-#include "shared_prefix_blocks.h"
+#include "shared_prefix_narrow.h"
 
 namespace kvfp8 {
 
 namespace {
 
 constexpr float kLn2 = 0.693147180559945309f;
-constexpr int kWideWaves = 8;
-constexpr int kWideThreads = 64 * kWideWaves;
 constexpr int kKeys = 64;             // tokens per block
 constexpr float kLag = 8.0f;          // log2 of how far a row's maximum may exceed its reference
-static_assert(kWideRows == 32 * kWideWaves, "32 rows per wave");
 
 typedef __attribute__((address_space(3))) const uint8_t lds_u8;
 typedef __attribute__((address_space(3))) const u32x4_t lds_u32x4;
@@ -48,32 +44,54 @@ __device__ __forceinline__ uint32_t widen2(uint32_t x) {
     else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, kHi));
 }
 
-template <int kD, int QT, int ES>
-__global__ void __launch_bounds__(kWideThreads)
-prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
+template <int kD>
+struct WideLds {
+    static constexpr int kRow = kD <= 64 ? 128 : 256;    // bytes of an LDS row
+    uint8_t k[2][kKeys * kRow];
+    uint8_t v[2][kKeys * kRow];
+    float scale[4][2][kKeys];
+    int32_t count[4][4];                                 // tokens of each tile that count
+};
+
+// NW waves, 32 rows each.
+template <int kD, int QT, int ES, int NW>
+__global__ void __launch_bounds__(64 * NW)
+prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
     static_assert(kD % 16 == 0 && kD >= 64 && kD <= 128 && (ES == 1 || kD % 64 == 0), "head sizes of this kernel");
     using T = typename Elem<QT>::T;
     constexpr bool kF16 = QT == KVFP8_F16;               // K and Q^T operands
     constexpr bool kF16V = kF16 && ES == 2;              // V^T and P operands; f16 q over codes: two bf16 parts of P
     constexpr int kParts = kF16 && ES == 1 ? 2 : 1;
-    constexpr int CPR = kD <= 64 ? 8 : 16;               // 16-byte chunks of an LDS row
-    constexpr int ROW = CPR * 16;
+    constexpr int kThreads = 64 * NW;
+    constexpr int ROW = WideLds<kD>::kRow;
+    constexpr int CPR = ROW / 16;                        // 16-byte chunks of an LDS row
     constexpr int NB = kD / 16, KS = kD / 32;
     constexpr bool kHalf = kD % 32 != 0;                 // and one step of 16 dims
     // Staging: a row of K or V is `SLOTS` runs of 16 bytes of cache; slot x of the block's 2 x 64 x SLOTS goes to
-    // thread x % 512. A wave's rows of one load lie in one 16-token tile, so its page is wave-uniform.
+    // thread x % kThreads. A wave's rows of one load lie in one 16-token tile, so its page is wave-uniform.
     constexpr int SLOTS = ES == 1 ? CPR / 2 : CPR;
     constexpr int RUNS = kD * ES / 16;                   // of them used
     constexpr int PER = kKeys * SLOTS;                   // slots per tensor
-    constexpr int LOADS = 2 * PER / kWideThreads;
-    constexpr int TILES = LOADS >= 4 ? 2 : 1;            // tiles a wave loads from
-    __shared__ __attribute__((aligned(16))) uint8_t lds_k[2][kKeys * ROW];
-    __shared__ __attribute__((aligned(16))) uint8_t lds_v[2][kKeys * ROW];
-    __shared__ __attribute__((aligned(16))) float lds_scale[4][2][kKeys];
-    __shared__ __attribute__((aligned(16))) int32_t lds_count[4][4];      // tokens of each tile that count
+    constexpr int LOADS = 2 * PER / kThreads;
+    constexpr int TILES = LOADS > 1 ? LOADS / 2 : 1;     // loads of K, each from a tile of its own, then those of V
+    constexpr int RPW = 64 / SLOTS;                      // rows of one load of a wave
+    union Lds {
+        WideLds<kD> wide;
+        NarrowLds<(kD <= 64 ? 1 : 2), NW> narrow;
+    };
+    __shared__ __attribute__((aligned(16))) Lds lds;
+    if ((int32_t)blockIdx.x >= grid.prefix_groups) {
+        PrefixItem own;
+        if (own_item(a, grid, own)) narrow_run<(kD <= 64 ? 1 : 2), QT, ES, NW>(a, own, grid.own_heads, grid.q_vec, lds.narrow);
+        return;
+    }
+    auto& lds_k = lds.wide.k;
+    auto& lds_v = lds.wide.v;
+    auto& lds_scale = lds.wide.scale;
+    auto& lds_count = lds.wide.count;
 
     PrefixItem it;
-    if (!prefix_item(a, grid, kWideRows, it)) return;
+    if (!prefix_item(a, grid, 32 * NW, it)) return;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int m16 = lane & 15, j = lane >> 4;
     const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
@@ -83,17 +101,15 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
     const bool active = r0 < it.pairs;
 
     // Row and tensor of load i of this thread; the tile of its wave's rows.
-    auto row_of = [&](int i) __attribute__((always_inline)) { return ((int)threadIdx.x + kWideThreads * i) % PER / SLOTS; };
-    auto wave_row = [&](int i) __attribute__((always_inline)) { return (64 * wave + kWideThreads * i) % PER / SLOTS; };
+    auto row_of = [&](int i) __attribute__((always_inline)) { return ((int)threadIdx.x + kThreads * i) % PER / SLOTS; };
+    auto wave_row = [&](int i) __attribute__((always_inline)) { return (64 * wave + kThreads * i) % PER / SLOTS; };
     const int run = threadIdx.x % SLOTS;
     const int64_t row_bytes = (int64_t)a.d.num_kv_heads * kD * ES;
-    // Scales: 16 lanes of a wave load those of the rows of K that it loads and of the same rows of V (head size 64:
-    // 16 rows, lanes 0..31 of the waves that load K).
-    constexpr bool kByWave = LOADS == 1;                 // waves 0..3 load K, 4..7 V
-    const int s_tensor = kByWave ? (lane >> 4) & 1 : (lane >> 3) & 1;
-    const int s_row = kByWave ? 16 * (wave & 3) + m16 : 8 * wave + (lane & 7);
-    const bool s_mine = kByWave ? wave < 4 && lane < 32 : lane < 16;
-    const bool loads_v = kByWave && wave >= 4;
+    // Scales: 2 RPW lanes of a wave that loads K load those of its rows, of K and of V.
+    constexpr bool kByWave = LOADS == 1;                 // the first half of the waves loads K, the other V
+    const bool loads_v = kByWave && wave >= NW / 2;
+    const int s_tensor = (lane / RPW) & 1, s_row = lane % RPW;
+    const bool s_mine = !loads_v && lane < 2 * RPW;
 
     // The page of the tile of load i in block g; past the prefix one of its own (no branch), which counts nothing.
     auto fetch_page = [&](int32_t g, int i) __attribute__((always_inline)) -> int32_t {
@@ -107,7 +123,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
         for (int u = 0; u < TILES; ++u) page[u] = fetch_page(g, u);
     };
     u32x4_t raw[LOADS];
-    float scale = 0.0f;
+    float scale[TILES];
     int64_t base[TILES];                                 // first cache row of the wave's tiles: of the K block in flight
     int32_t count_k[TILES], count_v[TILES];              // tokens that count in them, of the K and the V block in flight
     auto locate = [&](int32_t g) __attribute__((always_inline)) {
@@ -119,7 +135,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
             base[u] = ok ? (int64_t)page[u] * a.d.block_size + (tok & (a.d.block_size - 1)) : 0;
         }
     };
-    auto is_v = [&](int i) __attribute__((always_inline)) { return kByWave ? loads_v : kWideThreads * i >= PER; };
+    auto is_v = [&](int i) __attribute__((always_inline)) { return kByWave ? loads_v : kThreads * i >= PER; };
     auto issue = [&](bool v) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
@@ -132,7 +148,9 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
 #pragma unroll
             for (int u = 0; u < TILES; ++u) count_v[u] = count_k[u];
         } else if constexpr (ES == 1) {
-            scale = (s_tensor ? a.d.v_scales : a.d.k_scales)[(base[0] + (s_row & 15)) * a.d.num_kv_heads + h];
+#pragma unroll
+            for (int u = 0; u < TILES; ++u)
+                scale[u] = (s_tensor ? a.d.v_scales : a.d.k_scales)[(base[u] + (wave_row(u) & 15) + s_row) * a.d.num_kv_heads + h];
         }
     };
     // Rows that do not count become zeros (their bytes may be anything).
@@ -166,8 +184,11 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
         }
         if (v) return;
         if constexpr (ES == 1) {
-            const float x = (s_row & 15) < count_k[0] ? scale : 0.0f;
-            if (s_mine) lds_scale[g & 3][s_tensor][s_row] = s_tensor ? x : x * a.d.score_scale;
+#pragma unroll
+            for (int u = 0; u < TILES; ++u) {
+                const float x = (wave_row(u) & 15) + s_row < count_k[u] ? scale[u] : 0.0f;
+                if (s_mine) lds_scale[g & 3][s_tensor][wave_row(u) + s_row] = s_tensor ? x : x * a.d.score_scale;
+            }
         }
 #pragma unroll
         for (int u = 0; u < TILES; ++u)
@@ -188,12 +209,12 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const int d = 32 * s + 8 * j;
-                if (q_vec) qop[qt][s] = *reinterpret_cast<const u32x4_t*>(src + d);
+                if (grid.q_vec) qop[qt][s] = *reinterpret_cast<const u32x4_t*>(src + d);
                 else qop[qt][s] = u32x4_t{element2(d), element2(d + 2), element2(d + 4), element2(d + 6)};
             }
             if constexpr (kHalf) {
                 const int d = 32 * KS + 4 * j;
-                if (q_vec) qhalf[qt] = *reinterpret_cast<const uint2*>(src + d);
+                if (grid.q_vec) qhalf[qt] = *reinterpret_cast<const uint2*>(src + d);
                 else qhalf[qt] = make_uint2(element2(d), element2(d + 2));
             }
         }
@@ -386,7 +407,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
         __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
     };
     // Both halves run the same 2 * blocks barriers.
-    if (wave < 4) {
+    if (wave < NW / 2) {
         matrix(0, b0, true);
         barrier();
         if (active) softmax(0);
@@ -461,7 +482,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
             if (j == 0) a.lse[at] = (mu + __builtin_log2f(den)) * kLn2;
             continue;
         }
-        const int64_t pi = prefix_part(a, row, it.split, hq);
+        const int64_t pi = prefix_part(a, row, it.part, hq);
         if (j == 0) {
             a.d.part_m[pi] = m[qt];
             a.d.part_l[pi] = lt;
@@ -474,26 +495,28 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid, int q_vec) {
 }
 
 template <int kD, int QT, int ES>
-hipError_t launch_wide(const PrefixArgs& a, const PrefixGrid& g, int q_vec, hipStream_t s) {
-    hipLaunchKernelGGL((prefix_wide_kernel<kD, QT, ES>), dim3((unsigned)(kXcds * g.per_xcd)), dim3(kWideThreads), 0, s, a, g, q_vec);
+hipError_t launch_wide(const PrefixArgs& a, int rows, const PrefixGrid& g, hipStream_t s) {
+    const dim3 grid((unsigned)(g.prefix_groups + g.own_groups));
+    if (rows == 256) hipLaunchKernelGGL((prefix_wide_kernel<kD, QT, ES, 8>), grid, dim3(512), 0, s, a, g);
+    else hipLaunchKernelGGL((prefix_wide_kernel<kD, QT, ES, 4>), grid, dim3(256), 0, s, a, g);
     return hipGetLastError();
 }
 
 }  // namespace
 
 template <int QT>
-hipError_t launch_prefix_wide(const PrefixArgs& a, int kv_dtype, const PrefixGrid& g, int q_vec, hipStream_t s) {
-    if (kv_dtype != KVFP8_E4M3FN) return a.d.head_dim == 64 ? launch_wide<64, QT, 2>(a, g, q_vec, s) : launch_wide<128, QT, 2>(a, g, q_vec, s);
+hipError_t launch_prefix_wide(const PrefixArgs& a, int kv_dtype, int rows, const PrefixGrid& g, hipStream_t s) {
+    if (kv_dtype != KVFP8_E4M3FN) return a.d.head_dim == 64 ? launch_wide<64, QT, 2>(a, rows, g, s) : launch_wide<128, QT, 2>(a, rows, g, s);
     switch (a.d.head_dim) {
-        case 64: return launch_wide<64, QT, 1>(a, g, q_vec, s);
-        case 80: return launch_wide<80, QT, 1>(a, g, q_vec, s);
-        case 96: return launch_wide<96, QT, 1>(a, g, q_vec, s);
-        case 112: return launch_wide<112, QT, 1>(a, g, q_vec, s);
-        default: return launch_wide<128, QT, 1>(a, g, q_vec, s);
+        case 64: return launch_wide<64, QT, 1>(a, rows, g, s);
+        case 80: return launch_wide<80, QT, 1>(a, rows, g, s);
+        case 96: return launch_wide<96, QT, 1>(a, rows, g, s);
+        case 112: return launch_wide<112, QT, 1>(a, rows, g, s);
+        default: return launch_wide<128, QT, 1>(a, rows, g, s);
     }
 }
 
-template hipError_t launch_prefix_wide<KVFP8_F16>(const PrefixArgs&, int, const PrefixGrid&, int, hipStream_t);
-template hipError_t launch_prefix_wide<KVFP8_BF16>(const PrefixArgs&, int, const PrefixGrid&, int, hipStream_t);
+template hipError_t launch_prefix_wide<KVFP8_F16>(const PrefixArgs&, int, int, const PrefixGrid&, hipStream_t);
+template hipError_t launch_prefix_wide<KVFP8_BF16>(const PrefixArgs&, int, int, const PrefixGrid&, hipStream_t);
 
 }  // namespace kvfp8
