@@ -117,6 +117,63 @@ static PyObject* py_kvfp8_store_append(PyObject* self, PyObject* const* args, Py
     return PyLong_FromLong(rc);
 }
 
+/* kvfp8_shared_prefix_decode: the decode arguments, then the 7 of the prefixes. */
+static PyObject* py_kvfp8_shared_prefix_decode(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+    (void)self;
+    int64_t iv[DECODE_N + 7];
+    float scale = 0.0f;
+    if (!parse(args, nargs, DECODE_N + 7, 22, iv, &scale, "kvfp8_shared_prefix_decode")) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = kvfp8_shared_prefix_decode(DECODE_ARGS, PTR(27), (int)iv[28], PTR(29), (int)iv[30], PTR(31), (int)iv[32],
+                                    (int32_t)iv[33]);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+/* kvfp8_shared_prefix_prefill: 33 arguments, the scale at 27. */
+static PyObject* py_kvfp8_shared_prefix_prefill(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+    (void)self;
+    int64_t iv[33];
+    float scale = 0.0f;
+    if (!parse(args, nargs, 33, 27, iv, &scale, "kvfp8_shared_prefix_prefill")) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = kvfp8_shared_prefix_prefill(PTR(0), (int)iv[1], iv[2], (int32_t)iv[3], (int32_t)iv[4], (int32_t)iv[5], PTR(6),
+                                     PTR(7), (int)iv[8], (const float*)PTR(9), (const float*)PTR(10), iv[11],
+                                     (int32_t)iv[12], (const int32_t*)PTR(13), iv[14], iv[15], PTR(16), (int)iv[17],
+                                     PTR(18), (int)iv[19], PTR(20), (int)iv[21], (int32_t)iv[22], PTR(23), (int)iv[24],
+                                     (int32_t)iv[25], (int32_t)iv[26], scale, PTR(28), (float*)PTR(29), PTR(30), iv[31],
+                                     PTR(32));
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+/* kvfp8_token_logprobs: 14 arguments; its backward: 13. */
+static PyObject* py_kvfp8_token_logprobs(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+    (void)self;
+    int64_t iv[14];
+    if (!parse(args, nargs, 14, -1, iv, NULL, "kvfp8_token_logprobs")) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = kvfp8_token_logprobs(PTR(0), (int)iv[1], iv[2], iv[3], iv[4], PTR(5), (int)iv[6], (int32_t)iv[7], (float*)PTR(8),
+                              (float*)PTR(9), (float*)PTR(10), (float*)PTR(11), (int64_t*)PTR(12), PTR(13));
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+static PyObject* py_kvfp8_token_logprobs_backward(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+    (void)self;
+    int64_t iv[13];
+    if (!parse(args, nargs, 13, -1, iv, NULL, "kvfp8_token_logprobs_backward")) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = kvfp8_token_logprobs_backward(PTR(0), (int)iv[1], iv[2], iv[3], iv[4], PTR(5), (int)iv[6], (const float*)PTR(7),
+                                       (const float*)PTR(8), (const float*)PTR(9), (const float*)PTR(10), PTR(11), PTR(12));
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
 static PyMethodDef methods[] = {
     {"kvfp8_paged_decode", (PyCFunction)(void (*)(void))py_kvfp8_paged_decode, METH_FASTCALL, NULL},
     {"kvfp8_paged_decode_split", (PyCFunction)(void (*)(void))py_kvfp8_paged_decode_split, METH_FASTCALL, NULL},
@@ -124,6 +181,10 @@ static PyMethodDef methods[] = {
     {"kvfp8_append_paged_decode", (PyCFunction)(void (*)(void))py_kvfp8_append_paged_decode, METH_FASTCALL, NULL},
     {"kvfp8_quantize_append", (PyCFunction)(void (*)(void))py_kvfp8_quantize_append, METH_FASTCALL, NULL},
     {"kvfp8_store_append", (PyCFunction)(void (*)(void))py_kvfp8_store_append, METH_FASTCALL, NULL},
+    {"kvfp8_shared_prefix_decode", (PyCFunction)(void (*)(void))py_kvfp8_shared_prefix_decode, METH_FASTCALL, NULL},
+    {"kvfp8_shared_prefix_prefill", (PyCFunction)(void (*)(void))py_kvfp8_shared_prefix_prefill, METH_FASTCALL, NULL},
+    {"kvfp8_token_logprobs", (PyCFunction)(void (*)(void))py_kvfp8_token_logprobs, METH_FASTCALL, NULL},
+    {"kvfp8_token_logprobs_backward", (PyCFunction)(void (*)(void))py_kvfp8_token_logprobs_backward, METH_FASTCALL, NULL},
     {NULL, NULL, 0, NULL},
 };
 

@@ -14,13 +14,15 @@
 // alternatives of -inf at indices 0, 1, .. and gradient 0. NaN or +inf anywhere gives NaN
 // (alternatives: NaN counts as the largest value).
 //
-// One workgroup per row. Pass 1 keeps (m, S, sum e^d d) per thread, online, and the thread's largest
-// value. Alternatives: each wave finds the `top`-th largest of its 64 thread maxima by a search over
-// the bits of the value (ballots); the largest such bound over the waves is one that at least
-// `top` entries of the row reach. Pass 2 collects the entries that reach it in LDS and ranks them by
-// counting. Rows with more such entries than the list holds (long runs of equal logits), and rows
-// with NaN, are searched entry by entry instead.
-#include "kvfp8_common.h"
+// One workgroup per row. Rows of up to 131072 16-bit entries (65536 of float32) stay in registers: every load is
+// issued at once, the maximum is known before the first exponential, and the row is read once. Longer rows
+// keep (m, S, sum e^d d) per thread online and are read again for the alternatives.
+//
+// Alternatives: each wave finds the `top`-th largest of its 64 thread maxima by a search over the bits of the
+// value (ballots); the largest such bound over the waves is one that at least `top` entries of the row
+// reach. The entries that reach it are collected in LDS and ranked by counting. Rows with more such entries
+// than the list holds (long runs of equal logits), and rows with NaN, are searched entry by entry instead.
+#include "mfma_tiles.h"
 
 namespace kvfp8 {
 
@@ -82,21 +84,41 @@ __device__ __forceinline__ uint64_t entry_key(uint32_t value, int32_t index) {
     return ((uint64_t)value << 32) | (uint32_t)~index;
 }
 
+// DPP lane permutations inside rows of 16 lanes; together they reach all 16.
+constexpr int kDppXor1 = 0xB1;          // quad_perm [1, 0, 3, 2]
+constexpr int kDppXor2 = 0x4E;          // quad_perm [2, 3, 0, 1]
+constexpr int kDppHalfMirror = 0x141;   // lane i <-> 7 - i within each 8 lanes
+constexpr int kDppMirror = 0x140;       // lane i <-> 15 - i within each row
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return bits_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_bits(x), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, dpp<kDppXor1>(x));
+    x = fmaxf(x, dpp<kDppXor2>(x));
+    x = fmaxf(x, dpp<kDppHalfMirror>(x));
+    return fmaxf(x, dpp<kDppMirror>(x));
+}
+__device__ __forceinline__ float row_sum(float x) {
+    x += dpp<kDppXor1>(x);
+    x += dpp<kDppXor2>(x);
+    x += dpp<kDppHalfMirror>(x);
+    return x + dpp<kDppMirror>(x);
+}
+__device__ __forceinline__ float wave_max(float x) { return max_across_rows(row_max(x)); }
+__device__ __forceinline__ float wave_sum(float x) { return sum_across_rows(row_sum(x)); }
+
+__device__ __forceinline__ float first_lane(float x) { return bits_f32((uint32_t)__builtin_amdgcn_readfirstlane((int)f32_bits(x))); }
+
 struct Sums {
     float m, s, t;      // max, sum e^(x - m), sum e^(x - m) (x - m)
 };
 
-// The state with its maximum moved up to m (finite or -inf, at least s.m).
+// The state with its maximum moved up to m (finite or -inf, at least a.m).
 __device__ __forceinline__ Sums moved(Sums a, float m) {
     const float d = a.m == kNegInf ? 0.0f : a.m - m;     // an empty state has s = t = 0
     const float f = __builtin_amdgcn_exp2f(d * kLog2e);
     return Sums{m, a.s * f, (a.t + d * a.s) * f};
-}
-__device__ __forceinline__ Sums joined(Sums a, Sums b) {
-    const float m = fmaxf(a.m, b.m);
-    a = moved(a, m);
-    b = moved(b, m);
-    return Sums{m, a.s + b.s, a.t + b.t};
 }
 
 // Adds e^d and e^d d of d = x - m. Below -200 e^d is 0, and d is kept finite for the product.
@@ -107,7 +129,16 @@ __device__ __forceinline__ void add_entry(Sums& a, float x, float m) {
     a.t += e * fmaxf(d, -200.0f);
 }
 
-template <int DT, int NT>
+// Two entries of -inf (one of float32).
+template <int DT>
+constexpr uint32_t kNegInfBits = DT == KVFP8_F32 ? 0xFF800000u : (DT == KVFP8_BF16 ? 0xFF80FF80u : 0xFC00FC00u);
+// Lowest bit of the wave's search for a bound: the values' own last bit, or 20 bits of float32 (a bound that is
+// a little low only lets more entries into the list).
+template <int DT>
+constexpr int kLastBit = DT == KVFP8_BF16 ? 16 : (DT == KVFP8_F16 ? 13 : 12);
+
+// R: vectors of 16 bytes a thread holds; 0: the row is read in passes.
+template <int DT, int NT, int R>
 __global__ void __launch_bounds__(NT)
 token_logprobs_kernel(LogprobArgs a) {
     using T = typename Elem<DT>::T;
@@ -121,81 +152,151 @@ token_logprobs_kernel(LogprobArgs a) {
     const int64_t row = a.row0 + blockIdx.x;
     const T* x = reinterpret_cast<const T*>(a.x) + row * a.stride;
     const int32_t vectors = a.vocab / kPer, rest = a.vocab - vectors * kPer;
+    const int64_t token = a.tokens64 ? reinterpret_cast<const int64_t*>(a.tokens)[row]
+                                     : (int64_t)reinterpret_cast<const int32_t*>(a.tokens)[row];
+    const bool given = token >= 0 && token < a.vocab;
 
-    Sums st = {kNegInf, 0.0f, 0.0f};
-    uint32_t best = 0;
-    for (int32_t i = tid; i < vectors; i += NT) {
-        float v[kPer];
-        unpack<DT>(reinterpret_cast<const Vec16<T>*>(x)[i].w, v);
-        float mx = v[0];
+    uint32_t raw[R > 0 ? R : 1][4];
+    if constexpr (R > 0) {
 #pragma unroll
-        for (int e = 1; e < kPer; ++e) mx = fmaxf(mx, v[e]);
-        if (mx > st.m) st = moved(st, mx);
+        for (int r = 0; r < R; ++r) {
+            const int32_t i = r * NT + tid;
+            if (i < vectors) {
+                const Vec16<T> v = reinterpret_cast<const Vec16<T>*>(x)[i];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) raw[r][w] = v.w[w];
+            } else {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) raw[r][w] = kNegInfBits<DT>;
+            }
+        }
+    }
+    // The entries behind the last whole vector, one a thread.
+    const float tail = tid < rest ? Elem<DT>::load(x[vectors * kPer + tid]) : kNegInf;
+    const float chosen = tid == 0 && given ? Elem<DT>::load(x[token]) : 0.0f;
+    if (tid == 0) listed = 0;
+
+    // Between the passes over the registers: the words stay packed (else every unpacked value is kept).
+    auto keep_packed = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) __asm__ volatile("" : "+v"(raw[r][w]));
+    };
+    Sums st = {kNegInf, 0.0f, 0.0f};
+    float best = tail;                                    // this thread's largest value
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float v[kPer];
+            unpack<DT>(raw[r], v);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) best = fmaxf(best, v[e]);
+        }
+        st.m = wave_max(best);
+        keep_packed();
         const float m = st.m == kNegInf ? 0.0f : st.m;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) add_entry(st, v[e], m);
-    }
-    if (tid < rest) {
-        const float v = Elem<DT>::load(x[vectors * kPer + tid]);
-        if (v > st.m) st = moved(st, v);
-        add_entry(st, v, st.m == kNegInf ? 0.0f : st.m);
+        for (int r = 0; r < R; ++r) {
+            float v[kPer];
+            unpack<DT>(raw[r], v);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) add_entry(st, v[e], m);
+        }
+        if (tid < rest) add_entry(st, tail, m);
+    } else {
+        for (int32_t i = tid; i < vectors; i += NT) {
+            float v[kPer];
+            unpack<DT>(reinterpret_cast<const Vec16<T>*>(x)[i].w, v);
+            float mx = v[0];
+#pragma unroll
+            for (int e = 1; e < kPer; ++e) mx = fmaxf(mx, v[e]);
+            if (mx > st.m) st = moved(st, mx);
+            const float m = st.m == kNegInf ? 0.0f : st.m;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) add_entry(st, v[e], m);
+        }
+        if (tid < rest) {
+            if (tail > st.m) st = moved(st, tail);
+            add_entry(st, tail, st.m == kNegInf ? 0.0f : st.m);
+        }
+        best = fmaxf(best, st.m);
+        st = moved(st, wave_max(st.m));
     }
     if (a.top > 0) {
         // The wave's bound: the top-th largest thread maximum (0 where fewer threads hold entries).
-        best = tid < vectors || tid < rest ? ordered(st.m) : 0u;
+        const uint32_t key = tid < vectors || tid < rest ? ordered(best) : 0u;
         uint32_t bound = 0;
-        for (int bit = 31; bit >= (DT == KVFP8_BF16 ? 16 : 0); --bit) {
+        for (int bit = 31; bit >= kLastBit<DT>; --bit) {
             const uint32_t trial = bound | (1u << bit);
-            if (__popcll(__ballot(best >= trial)) >= a.top) bound = trial;
+            if (__popcll(__ballot(key >= trial)) >= a.top) bound = trial;
         }
         if (lane == 0) wave_bound[wave] = bound;
-        if (tid == 0) listed = 0;
     }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1)
-        st = joined(st, Sums{__shfl_xor(st.m, off), __shfl_xor(st.s, off), __shfl_xor(st.t, off)});
+    st.s = wave_sum(st.s);
+    st.t = wave_sum(st.t);
     if (lane == 0) wave_sums[wave] = st;
     __syncthreads();
-    st = wave_sums[0];
-    uint32_t bound = a.top > 0 ? wave_bound[0] : 0u;
-    for (int w = 1; w < kWaves; ++w) {
-        st = joined(st, wave_sums[w]);
-        if (a.top > 0) bound = max(bound, wave_bound[w]);
-    }
-    const bool empty = st.m == kNegInf && st.s == 0.0f;      // every entry is -inf
+    // Every row of 16 lanes joins the waves' states, one a lane; all take lane 0's result (a fused multiply in the sums
+    // rounds differently per lane, and the alternatives are written by threads in order of arrival).
+    const bool holds = (lane & 15) < kWaves;
+    st = holds ? wave_sums[lane & (kWaves - 1)] : Sums{kNegInf, 0.0f, 0.0f};
+    st = moved(st, row_max(st.m));
+    st.s = first_lane(row_sum(st.s));
+    st.t = first_lane(row_sum(st.t));
+    const bool empty = st.m == kNegInf && st.s == 0.0f;  // every entry is -inf
     const float log_s = empty ? kNegInf : __builtin_logf(st.s);
     if (tid == 0) {
-        const int64_t token = a.tokens64 ? reinterpret_cast<const int64_t*>(a.tokens)[row]
-                                         : (int64_t)reinterpret_cast<const int32_t*>(a.tokens)[row];
-        float lp = 0.0f;
-        if (token >= 0 && token < a.vocab) lp = empty ? kNegInf : (Elem<DT>::load(x[token]) - st.m) - log_s;
-        a.logprobs[row] = lp;
+        a.logprobs[row] = !given ? 0.0f : (empty ? kNegInf : (chosen - st.m) - log_s);
         a.entropy[row] = empty ? 0.0f : log_s - st.t / st.s;
         a.stats[row] = make_float2(st.m, log_s);
     }
     if (a.top == 0) return;
 
+    uint32_t bound = holds ? wave_bound[lane & (kWaves - 1)] : 0u;
+#pragma unroll
+    for (int w = 1; w < 16; w <<= 1) bound = max(bound, (uint32_t)__shfl_xor((int)bound, w));
     auto emit = [&](int32_t rank, uint64_t key) {
         const float v = from_ordered((uint32_t)(key >> 32));
         a.top_logprobs[row * a.top + rank] = empty ? kNegInf : (v - st.m) - log_s;
         a.top_tokens[row * a.top + rank] = (int64_t)(int32_t)~(uint32_t)key;
     };
-    // Every entry whose value reaches the bound, once.
-    auto scan = [&](auto&& visit) {
+    // Every entry of this thread, with its index.
+    auto scan_memory = [&](auto&& visit) __attribute__((always_inline)) {
         for (int32_t i = tid; i < vectors; i += NT) {
             float v[kPer];
             unpack<DT>(reinterpret_cast<const Vec16<T>*>(x)[i].w, v);
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) visit(ordered(v[e]), i * kPer + e);
+            for (int e = 0; e < kPer; ++e) visit(v[e], i * kPer + e);
         }
-        if (tid < rest) visit(ordered(Elem<DT>::load(x[vectors * kPer + tid])), vectors * kPer + tid);
+        if (tid < rest) visit(tail, vectors * kPer + tid);
+    };
+    auto scan = [&](auto&& visit) __attribute__((always_inline)) {
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int32_t i = r * NT + tid;
+                if (i < vectors) {
+                    float v[kPer];
+                    unpack<DT>(raw[r], v);
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) visit(v[e], i * kPer + e);
+                }
+            }
+            if (tid < rest) visit(tail, vectors * kPer + tid);
+        } else {
+            scan_memory(visit);
+        }
     };
     const bool clean = st.s == st.s;         // no NaN and no +inf
-    if (clean)
-        scan([&](uint32_t value, int32_t index) {
-            if (value >= bound) {
+    keep_packed();
+    // (Shortened to its upper bits, the order of -inf is that of no value.)
+    const float least = bound <= 0x007FFFFFu ? kNegInf : from_ordered(bound);
+    if (clean && best >= least)
+        scan([&](float v, int32_t index) {
+            if (v >= least) {
                 const int32_t at = atomicAdd(&listed, 1);
-                if (at < kList) list[at] = entry_key(value, index);
+                if (at < kList) list[at] = entry_key(ordered(v), index);
             }
         });
     __syncthreads();
@@ -214,8 +315,8 @@ token_logprobs_kernel(LogprobArgs a) {
     uint64_t last = 0;
     for (int32_t r = 0; r < a.top; ++r) {
         uint64_t mine = 0;
-        scan([&](uint32_t value, int32_t index) {
-            const uint64_t key = entry_key(value, index);
+        scan_memory([&](float v, int32_t index) {
+            const uint64_t key = entry_key(ordered(v), index);
             if ((r == 0 || key < last) && key > mine) mine = key;
         });
 #pragma unroll
@@ -307,14 +408,23 @@ bool aligned(const void* p, int dtype) { return (uintptr_t)p % (dtype == KVFP8_F
 // A launch has fewer than 2^32 threads: rows go in runs of this many workgroups.
 constexpr int64_t kMaxGroups = (int64_t)1 << 21;
 
+template <int DT, int NT, int R>
+void launch_rows(const LogprobArgs& a, int64_t rows, hipStream_t s) {
+    hipLaunchKernelGGL((token_logprobs_kernel<DT, NT, R>), dim3((unsigned)rows), dim3(NT), 0, s, a);
+}
+
 template <int DT>
 hipError_t launch_logprobs(LogprobArgs a, int64_t rows, hipStream_t s) {
+    const int64_t vectors = a.vocab / (DT == KVFP8_F32 ? 4 : 8);
     for (a.row0 = 0; a.row0 < rows; a.row0 += kMaxGroups) {
-        const dim3 grid((unsigned)(rows - a.row0 < kMaxGroups ? rows - a.row0 : kMaxGroups));
-        if (a.vocab <= 8192)
-            hipLaunchKernelGGL((token_logprobs_kernel<DT, 256>), grid, dim3(256), 0, s, a);
-        else
-            hipLaunchKernelGGL((token_logprobs_kernel<DT, 1024>), grid, dim3(1024), 0, s, a);
+        const int64_t n = rows - a.row0 < kMaxGroups ? rows - a.row0 : kMaxGroups;
+        if (vectors <= 256) launch_rows<DT, 256, 1>(a, n, s);
+        else if (vectors <= 1024) launch_rows<DT, 256, 4>(a, n, s);
+        else if (vectors <= 2048) launch_rows<DT, 1024, 2>(a, n, s);
+        else if (vectors <= 4096) launch_rows<DT, 1024, 4>(a, n, s);
+        else if (vectors <= 8192) launch_rows<DT, 1024, 8>(a, n, s);
+        else if (vectors <= 16384) launch_rows<DT, 1024, 16>(a, n, s);
+        else launch_rows<DT, 1024, 0>(a, n, s);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }

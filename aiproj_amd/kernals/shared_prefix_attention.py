@@ -62,22 +62,28 @@ def _check_prefix(prefix, what: str):
 def _check_cache(cache, block_table, d: int, hq: int, what: str):
     """(k, v, k_scales, v_scales, block table) of a paged cache, contiguous."""
     k, v = cache.k, cache.v
-    scales = (cache.k_scales, cache.v_scales) if cache.quantized else (None, None)
-    if k.ndim != 4 or k.shape != v.shape or k.shape[3] != d or hq % k.shape[2]:
+    shape, block_size = k.shape, cache.block_size
+    if len(shape) != 4 or shape != v.shape or shape[3] != d or hq % shape[2]:
         raise ValueError(f"{what}: cache rows [num_blocks, block_size, Hkv, D] that match q [.., Hq, D]")
-    if k.shape[1] != cache.block_size or cache.block_size & (cache.block_size - 1):
+    if shape[1] != block_size or block_size & (block_size - 1):
         raise ValueError(f"{what}: block size must be the cache's and a power of two")
     if block_table.ndim != 2 or block_table.dtype != t.int32:
         raise ValueError(f"{what}: the block table is an int32 matrix")
     if v.dtype != k.dtype:
         raise ValueError(f"{what}: k and v share one dtype")
-    if cache.quantized and (k.dtype != t.float8_e4m3fn or any(s.dtype != t.float32 or s.shape != k.shape[:3] for s in scales)):
-        raise ValueError(f"{what}: a quantized cache holds float8_e4m3fn and float32 scales per row")
-    if not cache.quantized and k.dtype not in _Q_DTYPES:
+    contiguous = k.is_contiguous() and v.is_contiguous()
+    k_scales = v_scales = None
+    if cache.quantized:
+        k_scales, v_scales = cache.k_scales, cache.v_scales
+        if (k.dtype != t.float8_e4m3fn or k_scales.dtype != t.float32 or v_scales.dtype != t.float32
+                or k_scales.shape != shape[:3] or v_scales.shape != shape[:3]):
+            raise ValueError(f"{what}: a quantized cache holds float8_e4m3fn and float32 scales per row")
+        contiguous = contiguous and k_scales.is_contiguous() and v_scales.is_contiguous()
+    elif k.dtype not in _Q_DTYPES:
         raise ValueError(f"{what}: unsupported cache dtype {k.dtype}")
-    if any(x is not None and not x.is_contiguous() for x in (k, v, *scales)):
+    if not contiguous:
         raise ValueError(f"{what}: cache tensors must be contiguous")
-    return k, v, *scales, block_table if block_table.is_contiguous() else block_table.contiguous()
+    return k, v, k_scales, v_scales, block_table if block_table.is_contiguous() else block_table.contiguous()
 
 
 @functools.lru_cache(maxsize=256)
@@ -106,16 +112,16 @@ def shared_prefix_decode_attention(q: t.Tensor, paged_kv_cache, cache_batch_cont
     if q.stride(-1) != 1:
         q = q.contiguous()
     num_blocks, block_size, hkv, _ = k.shape
-    kv_code, stream = _native.dtype_code(k.dtype), _native.stream_handle(device)
-    nbytes = _workspace_bytes(b, hq, hkv, d, len(p_slots), table.shape[1], block_size, kv_code, 0)
-    workspace = _workspace(device, stream, nbytes)
+    bt_rows, bt_width = table.shape
+    groups, code = p_slots.shape[0], _native.TORCH_TO_CODE
+    kv_code, stream = code[k.dtype], _native.stream_handle(device)
+    workspace = _workspace(device, stream, _workspace_bytes(b, hq, hkv, d, groups, bt_width, block_size, kv_code, 0))
     rc = _native.fn("kvfp8_shared_prefix_decode")(
-        q.data_ptr(), _native.dtype_code(q.dtype), q.stride(0), q.stride(1), b, hq, hkv, d, k.data_ptr(), v.data_ptr(),
-        kv_code, _native.ptr(k_scales), _native.ptr(v_scales), num_blocks, block_size, table.data_ptr(), table.shape[0],
-        table.shape[1], slots.data_ptr(), _native.dtype_code(slots.dtype), lens.data_ptr(), _native.dtype_code(lens.dtype),
-        1.0 / math.sqrt(d), output.data_ptr(), workspace.data_ptr(), workspace.numel(), stream,
-        p_slots.data_ptr(), _native.dtype_code(p_slots.dtype), p_lens.data_ptr(), _native.dtype_code(p_lens.dtype),
-        p_starts.data_ptr(), _native.dtype_code(p_starts.dtype), len(p_slots))
+        q.data_ptr(), code[q.dtype], q.stride(0), q.stride(1), b, hq, hkv, d, k.data_ptr(), v.data_ptr(),
+        kv_code, _native.ptr(k_scales), _native.ptr(v_scales), num_blocks, block_size, table.data_ptr(), bt_rows,
+        bt_width, slots.data_ptr(), code[slots.dtype], lens.data_ptr(), code[lens.dtype], 1.0 / math.sqrt(d),
+        output.data_ptr(), workspace.data_ptr(), workspace.numel(), stream, p_slots.data_ptr(), code[p_slots.dtype],
+        p_lens.data_ptr(), code[p_lens.dtype], p_starts.data_ptr(), code[p_starts.dtype], groups)
     _native.check(rc, "kvfp8_shared_prefix_decode")
     return output
 
@@ -141,21 +147,22 @@ def shared_prefix_prefill_attention(q: t.Tensor, k: t.Tensor, v: t.Tensor, cum_s
         raise ValueError(f"{what}: k and v have the cache's heads")
     p_slots, p_lens, p_starts = _check_prefix(prefix, what)
     device = _native.require_gpu(q, k, v, cum_seq, pk, pv, k_scales, v_scales, table, p_slots, p_lens, p_starts, what=what)
-    cum_seq = cum_seq.contiguous()
+    if not cum_seq.is_contiguous():
+        cum_seq = cum_seq.contiguous()
     output, lse = flash_attention_forward(q, k, v, cum_seq, batch_max_seq_len, scale)
     batch, longest = cum_seq.shape[0] - 1, int(batch_max_seq_len)
-    if total == 0 or batch <= 0 or longest <= 0 or len(p_slots) == 0:
+    if total == 0 or batch <= 0 or longest <= 0 or p_slots.shape[0] == 0:
         return output, lse
     num_blocks, block_size, hkv, _ = pk.shape
-    kv_code, stream = _native.dtype_code(pk.dtype), _native.stream_handle(device)
-    nbytes = _workspace_bytes(total, hq, hkv, d, len(p_slots), table.shape[1], block_size, kv_code, 1)
-    workspace = _workspace(device, stream, nbytes)
-    rc = _native.lib().kvfp8_shared_prefix_prefill(
-        q.data_ptr(), _native.dtype_code(q.dtype), total, hq, hkv, d, pk.data_ptr(), pv.data_ptr(), kv_code,
-        _native.ptr(k_scales), _native.ptr(v_scales), num_blocks, block_size, table.data_ptr(), table.shape[0],
-        table.shape[1], p_slots.data_ptr(), _native.dtype_code(p_slots.dtype), p_lens.data_ptr(),
-        _native.dtype_code(p_lens.dtype), p_starts.data_ptr(), _native.dtype_code(p_starts.dtype), len(p_slots),
-        cum_seq.data_ptr(), _native.dtype_code(cum_seq.dtype), batch, longest, float(scale), output.data_ptr(),
-        lse.data_ptr(), workspace.data_ptr(), workspace.numel(), stream)
+    bt_rows, bt_width = table.shape
+    groups, code = p_slots.shape[0], _native.TORCH_TO_CODE
+    kv_code, stream = code[pk.dtype], _native.stream_handle(device)
+    workspace = _workspace(device, stream, _workspace_bytes(total, hq, hkv, d, groups, bt_width, block_size, kv_code, 1))
+    rc = _native.fn("kvfp8_shared_prefix_prefill")(
+        q.data_ptr(), code[q.dtype], total, hq, hkv, d, pk.data_ptr(), pv.data_ptr(), kv_code,
+        _native.ptr(k_scales), _native.ptr(v_scales), num_blocks, block_size, table.data_ptr(), bt_rows, bt_width,
+        p_slots.data_ptr(), code[p_slots.dtype], p_lens.data_ptr(), code[p_lens.dtype], p_starts.data_ptr(),
+        code[p_starts.dtype], groups, cum_seq.data_ptr(), code[cum_seq.dtype], batch, longest, float(scale),
+        output.data_ptr(), lse.data_ptr(), workspace.data_ptr(), workspace.numel(), stream)
     _native.check(rc, "kvfp8_shared_prefix_prefill")
     return output, lse

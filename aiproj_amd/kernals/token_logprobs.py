@@ -61,13 +61,15 @@ def _forward(logits: t.Tensor, tokens: t.Tensor, top: int):
     """(logprobs, entropy, top_logprobs, top_tokens, stats [T, 2])."""
     device = _check(logits, tokens, top)
     rows, vocab = logits.shape
-    tokens = tokens.contiguous()
-    logprobs, entropy = (t.empty(rows, dtype=t.float32, device=logits.device) for _ in range(2))
-    stats = t.empty((rows, 2), dtype=t.float32, device=logits.device)
-    top_logprobs = t.empty((rows, top), dtype=t.float32, device=logits.device)
-    top_tokens = t.empty((rows, top), dtype=t.int64, device=logits.device)
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    logprobs = t.empty(rows, dtype=t.float32, device=device)
+    entropy = t.empty_like(logprobs)
+    stats = t.empty((rows, 2), dtype=t.float32, device=device)
+    top_logprobs = t.empty((rows, top), dtype=t.float32, device=device)
+    top_tokens = t.empty((rows, top), dtype=t.int64, device=device)
     if rows:
-        rc = _native.lib().kvfp8_token_logprobs(
+        rc = _native.fn("kvfp8_token_logprobs")(
             logits.data_ptr(), _native.dtype_code(logits.dtype), logits.stride(0), rows, vocab,
             tokens.data_ptr(), _native.dtype_code(tokens.dtype), top, logprobs.data_ptr(), entropy.data_ptr(),
             stats.data_ptr(), top_logprobs.data_ptr(), top_tokens.data_ptr(), _native.stream_handle(device))
@@ -112,7 +114,7 @@ class TokenLogprobsFunction(t.autograd.Function):
         if grad.numel():
             tokens = tokens.contiguous()
             grad_logprobs, grad_entropy = (None if g is None else g.contiguous() for g in (grad_logprobs, grad_entropy))
-            rc = _native.lib().kvfp8_token_logprobs_backward(
+            rc = _native.fn("kvfp8_token_logprobs_backward")(
                 logits.data_ptr(), _native.dtype_code(logits.dtype), logits.stride(0), logits.shape[0], logits.shape[1],
                 tokens.data_ptr(), _native.dtype_code(tokens.dtype), entropy.data_ptr(), stats.data_ptr(),
                 _native.ptr(grad_logprobs), _native.ptr(grad_entropy), grad.data_ptr(), _native.stream_handle(logits.device))

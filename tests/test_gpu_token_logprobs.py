@@ -53,7 +53,8 @@ def _check_forward(logits, tokens, top):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("vocab", [1, 3, 7, 8, 9, 63, 257, 2049, 4100, 8192, 8193, 32000, 50001, 131077])
+@pytest.mark.parametrize("vocab", [1, 3, 7, 8, 9, 63, 257, 1027, 2049, 4100, 8192, 8193, 16390, 32000, 32771, 50001, 65540,
+                                   131077, 262145])
 def test_forward_against_float64(dtype, vocab):
     rows = 5
     logits = _logits(rows, vocab, dtype)
@@ -73,7 +74,7 @@ def test_rows_apart_and_off_alignment(dtype, rows):
     _check_forward(wide[:1].expand(rows, -1), t.zeros(2 * rows, dtype=t.int64, device="cuda")[::2], 2)
 
 
-@pytest.mark.parametrize("vocab", [500, 30000])
+@pytest.mark.parametrize("vocab", [500, 30000, 140000])
 def test_equal_logits_go_by_index(vocab):
     """Whole rows of one value (more than the list holds), few distinct values, and zeros of both signs."""
     rows = [t.zeros(vocab), t.full((vocab,), -7.5), t.arange(vocab) % 3 * 1.0, -(t.arange(vocab) // 100).float(),
@@ -84,7 +85,7 @@ def test_equal_logits_go_by_index(vocab):
             _check_forward(logits.to(dtype), t.arange(6, device="cuda"), top)
 
 
-@pytest.mark.parametrize("vocab", [300, 20000])
+@pytest.mark.parametrize("vocab", [300, 20000, 140001])
 def test_masked_entries(vocab):
     logits = _logits(4, vocab, t.float32)
     logits[0, 10:] = -t.inf                 # fewer left than alternatives asked for
@@ -103,7 +104,7 @@ def test_masked_entries(vocab):
     assert got.logprobs[3] == -t.inf and got.entropy[3] == 0 and bool((got.top_logprobs[3] == -t.inf).all())
 
 
-@pytest.mark.parametrize("vocab", [100, 9000])
+@pytest.mark.parametrize("vocab", [100, 9000, 140001])
 def test_nan_and_infinity(vocab):
     logits = _logits(3, vocab, t.float32)
     logits[0, 0] = logits[0, 77] = t.nan
@@ -253,6 +254,15 @@ def test_captured_and_replayed():
         graph.replay()
         t.cuda.synchronize()
         for a, b in zip(out, step()):
+            assert t.equal(a, b)
+
+
+@pytest.mark.parametrize("vocab", [3000, 20001, 140001])
+def test_equal_calls_give_equal_bits(vocab):
+    logits, tokens = _logits(100, vocab, t.bfloat16), t.randint(0, vocab, (100,), device="cuda")
+    first = token_logprobs(logits, tokens, 20)
+    for _ in range(20):
+        for a, b in zip(token_logprobs(logits, tokens, 20), first):
             assert t.equal(a, b)
 
 
