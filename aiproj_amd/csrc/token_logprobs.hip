@@ -18,10 +18,12 @@
 // issued at once, the maximum is known before the first exponential, and the row is read once. Longer rows
 // keep (m, S, sum e^d d) per thread online and are read again for the alternatives.
 //
-// Alternatives: each wave finds the `top`-th largest of its 64 thread maxima by a search over the bits of the
-// value (ballots); the largest such bound over the waves is one that at least `top` entries of the row
-// reach. The entries that reach it are collected in LDS and ranked by counting. Rows with more such entries
-// than the list holds (long runs of equal logits), and rows with NaN, are searched entry by entry instead.
+// Alternatives: with A waves that hold entries in all lanes, every wave finds the n-th largest of its 64 thread maxima,
+// n = ceil(top / A); the ceil(top / n)-th largest of these is a bound that at least `top` entries of the row reach,
+// and not many more. The entries that reach it are collected in LDS and ranked by counting. Where more reach it than the list holds (runs of equal logits, masked rows, sorted rows), the
+// bound is raised to the largest over the waves of the `top`-th thread maximum, only entries above it are
+// collected, and those equal to it follow by index. What still does not fit, and rows with NaN, are searched
+// entry by entry.
 #include "mfma_tiles.h"
 
 namespace kvfp8 {
@@ -223,14 +225,22 @@ token_logprobs_kernel(LogprobArgs a) {
         best = fmaxf(best, st.m);
         st = moved(st, wave_max(st.m));
     }
-    if (a.top > 0) {
-        // The wave's bound: the top-th largest thread maximum (0 where fewer threads hold entries).
-        const uint32_t key = tid < vectors || tid < rest ? ordered(best) : 0u;
+    // The n-th largest thread maximum of the wave, as an order of values (0 where fewer threads hold entries).
+    const uint32_t mine = tid < vectors || tid < rest ? ordered(best) : 0u;
+    auto nth_of_wave = [&](int n) __attribute__((always_inline)) {
         uint32_t bound = 0;
         for (int bit = 31; bit >= kLastBit<DT>; --bit) {
             const uint32_t trial = bound | (1u << bit);
-            if (__popcll(__ballot(key >= trial)) >= a.top) bound = trial;
+            if (__popcll(__ballot(mine >= trial)) >= n) bound = trial;
         }
+        return bound;
+    };
+    const int full = min(vectors / 64, kWaves);          // waves that hold entries in all lanes
+    if (a.top > 0) {
+        uint32_t bound = 0;
+        const int n = full > 0 ? (a.top + full - 1) / full : 0;
+        if (n == 1) bound = ordered(st.m);
+        else if (n > 1) bound = nth_of_wave(n);
         if (lane == 0) wave_bound[wave] = bound;
     }
     st.s = wave_sum(st.s);
@@ -253,9 +263,6 @@ token_logprobs_kernel(LogprobArgs a) {
     }
     if (a.top == 0) return;
 
-    uint32_t bound = holds ? wave_bound[lane & (kWaves - 1)] : 0u;
-#pragma unroll
-    for (int w = 1; w < 16; w <<= 1) bound = max(bound, (uint32_t)__shfl_xor((int)bound, w));
     auto emit = [&](int32_t rank, uint64_t key) {
         const float v = from_ordered((uint32_t)(key >> 32));
         a.top_logprobs[row * a.top + rank] = empty ? kNegInf : (v - st.m) - log_s;
@@ -288,48 +295,98 @@ token_logprobs_kernel(LogprobArgs a) {
             scan_memory(visit);
         }
     };
-    const bool clean = st.s == st.s;         // no NaN and no +inf
-    keep_packed();
-    // (Shortened to its upper bits, the order of -inf is that of no value.)
-    const float least = bound <= 0x007FFFFFu ? kNegInf : from_ordered(bound);
-    if (clean && best >= least)
-        scan([&](float v, int32_t index) {
-            if (v >= least) {
-                const int32_t at = atomicAdd(&listed, 1);
-                if (at < kList) list[at] = entry_key(ordered(v), index);
-            }
-        });
-    __syncthreads();
-    if (clean && listed <= kList) {
-        // The list's order is that of arrival; a rank counts keys, which are distinct.
-        const int32_t n = listed;
-        for (int32_t i = tid; i < n; i += NT) {
+    // The least value of an order bound. (Shortened to its upper bits, the order of -inf is that of no value.)
+    auto value_of = [&](uint32_t bound) __attribute__((always_inline)) { return bound <= 0x007FFFFFu ? kNegInf : from_ordered(bound); };
+    // Collects the entries above `least` (and those equal to it) and returns their number; all threads.
+    auto collect = [&](float least, bool equal) __attribute__((always_inline)) {
+        if (equal ? best >= least : best > least)
+            scan([&](float v, int32_t index) {
+                if (v > least || (equal && v == least)) {
+                    const int32_t at = atomicAdd(&listed, 1);
+                    if (at < kList) list[at] = entry_key(ordered(v), index);
+                }
+            });
+        __syncthreads();
+        return listed;
+    };
+    // The list's order is that of arrival; a rank counts keys, which are distinct. Sixteen lanes count for a key.
+    auto rank_list = [&](int32_t n) __attribute__((always_inline)) {
+        for (int32_t i = tid >> 4; i < n; i += NT / 16) {
             const uint64_t key = list[i];
-            int32_t rank = 0;
-            for (int32_t j = 0; j < n; ++j) rank += list[j] > key;
-            if (rank < a.top) emit(rank, key);
+            int32_t above = 0;
+            for (int32_t j = tid & 15; j < n; j += 16) above += list[j] > key;
+            const int32_t rank = (int32_t)row_sum((float)above);           // at most kList: exact
+            if (rank < a.top && (tid & 15) == 0) emit(rank, key);
         }
-        return;
+    };
+    const bool clean = st.s == st.s;                     // no NaN and no +inf
+    if (clean) {
+        keep_packed();
+        uint32_t bound = 0;
+        if (full > 0) {
+            const int each = (a.top + full - 1) / full, rank = (a.top + each - 1) / each - 1;
+            const int w = lane & (kWaves - 1);
+            const uint32_t b = w < full ? wave_bound[w] : 0u;
+            int above = 0;
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) {
+                const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)b, v);
+                above += v < full && (other > b || (other == b && v < w));
+            }
+            bound = (uint32_t)__builtin_amdgcn_readlane((int)b, (int)__builtin_ctzll(__ballot(w < full && above == rank)));
+        }
+        int32_t n = collect(value_of(bound), true);
+        if (n <= kList) {
+            rank_list(n);
+            return;
+        }
+        __syncthreads();                                 // all have read the bounds and the count
+        const uint32_t higher = nth_of_wave(a.top);
+        if (lane == 0) wave_bound[wave] = higher;
+        if (tid == 0) listed = 0;
+        __syncthreads();
+        for (int w = 0; w < kWaves; ++w) bound = max(bound, wave_bound[w]);
+        const float least = value_of(bound);
+        n = collect(least, false);
+        if (n <= kList) {
+            if (n < a.top) {
+                // The first entries equal to the bound, in the order of their index.
+                if (wave == 0) {
+                    for (int32_t i = lane; n < a.top && i - lane < a.vocab; i += 64) {
+                        const bool hit = i < a.vocab && Elem<DT>::load(x[i]) == least;
+                        const uint64_t hits = __ballot(hit);
+                        const int32_t at = n + __popcll(hits & (((uint64_t)1 << lane) - 1));
+                        if (hit && at < a.top) list[at] = entry_key(ordered(least), i);
+                        n += __popcll(hits);
+                    }
+                }
+                __syncthreads();
+                n = a.top;
+            }
+            rank_list(n);
+            return;
+        }
+        __syncthreads();                                 // all have read the count
     }
     // One alternative per round: the largest key below the last one.
     uint64_t last = 0;
     for (int32_t r = 0; r < a.top; ++r) {
-        uint64_t mine = 0;
+        uint64_t most = 0;
         scan_memory([&](float v, int32_t index) {
             const uint64_t key = entry_key(ordered(v), index);
-            if ((r == 0 || key < last) && key > mine) mine = key;
+            if ((r == 0 || key < last) && key > most) most = key;
         });
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
-            const uint64_t other = (uint64_t)__shfl_xor((long long)mine, off);
-            mine = other > mine ? other : mine;
+            const uint64_t other = (uint64_t)__shfl_xor((long long)most, off);
+            most = other > most ? other : most;
         }
         __syncthreads();
-        if (lane == 0) list[wave] = mine;
+        if (lane == 0) list[wave] = most;
         __syncthreads();
-        for (int w = 0; w < kWaves; ++w) mine = list[w] > mine ? list[w] : mine;
-        if (tid == 0) emit(r, mine);
-        last = mine;
+        for (int w = 0; w < kWaves; ++w) most = list[w] > most ? list[w] : most;
+        if (tid == 0) emit(r, most);
+        last = most;
     }
 }
 
@@ -413,13 +470,22 @@ void launch_rows(const LogprobArgs& a, int64_t rows, hipStream_t s) {
     hipLaunchKernelGGL((token_logprobs_kernel<DT, NT, R>), dim3((unsigned)rows), dim3(NT), 0, s, a);
 }
 
+// Threads and vectors a thread by the row's length. More rows than two per CU are bound by the loads that are in flight
+// between the workgroups' barriers, and take more, smaller workgroups. Measured, 4096 rows of 32000 bf16, no, 1, 5
+// and 20 alternatives: 1024 threads 49, 74, 71 and 81 us, 512 threads 43, 54, 57 and 63, 256 threads 42, 56, 63
+// and 63 (262 MB: 6.1 TB/s without alternatives). A few rows are bound by latency: one row, 1024 threads, 4.1, 6.9,
+// 7.0 and 7.9 us.
 template <int DT>
 hipError_t launch_logprobs(LogprobArgs a, int64_t rows, hipStream_t s) {
     const int64_t vectors = a.vocab / (DT == KVFP8_F32 ? 4 : 8);
     for (a.row0 = 0; a.row0 < rows; a.row0 += kMaxGroups) {
         const int64_t n = rows - a.row0 < kMaxGroups ? rows - a.row0 : kMaxGroups;
+        const bool many = n > 2 * device_cus();
         if (vectors <= 256) launch_rows<DT, 256, 1>(a, n, s);
         else if (vectors <= 1024) launch_rows<DT, 256, 4>(a, n, s);
+        else if (many && vectors <= 2048) launch_rows<DT, 512, 4>(a, n, s);
+        else if (many && vectors <= 4096) launch_rows<DT, 512, 8>(a, n, s);
+        else if (many && vectors <= 8192) launch_rows<DT, 512, 16>(a, n, s);
         else if (vectors <= 2048) launch_rows<DT, 1024, 2>(a, n, s);
         else if (vectors <= 4096) launch_rows<DT, 1024, 4>(a, n, s);
         else if (vectors <= 8192) launch_rows<DT, 1024, 8>(a, n, s);

@@ -85,6 +85,23 @@ def test_equal_logits_go_by_index(vocab):
             _check_forward(logits.to(dtype), t.arange(6, device="cuda"), top)
 
 
+@pytest.mark.parametrize("vocab", [1500, 9000, 32000, 140000])
+@pytest.mark.parametrize("dtype", [t.float32, t.bfloat16])
+def test_rows_with_structure(vocab, dtype):
+    """Sorted rows, all large entries in one thread's or wave's places, few entries left, one value with exceptions."""
+    up = t.arange(vocab).float()
+    block = t.where((t.arange(vocab) >= 512) & (t.arange(vocab) < 512 + 700), 5.0 + t.arange(vocab) / vocab, 0.0)
+    strided = t.where(t.arange(vocab) % 1024 < 8, 3.0, -1.0)
+    few = t.full((vocab,), -t.inf)
+    few[vocab // 2:vocab // 2 + 7] = t.arange(7).float()
+    flat = t.zeros(vocab)
+    flat[-3:] = 1.0
+    flat[::700] = -1.0
+    logits = t.stack([up / 100, -up / 100, block, strided, few, flat]).cuda().to(dtype)
+    for top in (1, 7, 20, 64):
+        _check_forward(logits, t.full((6,), vocab // 2, device="cuda"), top)
+
+
 @pytest.mark.parametrize("vocab", [300, 20000, 140001])
 def test_masked_entries(vocab):
     logits = _logits(4, vocab, t.float32)
