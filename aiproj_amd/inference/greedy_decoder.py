@@ -19,6 +19,12 @@ Unlike the reference runtime, the allocator's committed lengths are not advanced
 by every step (that would be host work inside the captured step): `generate()`
 commits the tokens it wrote when it returns, and a caller driving `step()` itself
 commits with `commit(steps)`.
+
+A prefix that all sequences share (a system prompt, or one prompt to be answered many times) is kept
+once: with `prefix_len`, `prefill(prompts, prefix)` runs it through the model as a request of its own
+and the prompts and every later step behind it (`kernals/shared_prefix_attention.py`). With
+`logprobs`, every step records the log probability of the token it chose, the entropy and that many
+alternatives (`kernals/token_logprobs.py`) in `scores`, rows in decode order like `history`.
 """
 
 from __future__ import annotations
@@ -27,19 +33,29 @@ import torch as t
 
 from aiproj_amd.inference.page_allocator import CacheContainer, PageAllocator
 from aiproj_amd.inference.paged_kv_cache import PagedKVCache
+from aiproj_amd.kernals.shared_prefix_attention import SharedPrefix
+from aiproj_amd.kernals.token_logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 from aiproj_amd.model.transformer import StepMeta, TransformerLM
 
 
 class GreedyDecoder:
     def __init__(self, model: TransformerLM, batch: int, max_len: int, cache_dtype=t.float8_e4m3fn,
-                 block_size: int = 16, device="cuda"):
+                 block_size: int = 16, device="cuda", prefix_len: int = 0, logprobs: int | None = None):
         cfg = model.cfg
+        if prefix_len < 0 or (prefix_len and prefix_len + max_len > cfg.max_seq_len):
+            raise ValueError("GreedyDecoder: prefix_len and max_len together are at most the model's max_seq_len")
+        if logprobs is not None and not 0 <= logprobs <= min(MAX_TOP, cfg.vocab_size):
+            raise ValueError(f"GreedyDecoder: logprobs is a number of alternatives up to {MAX_TOP}")
         self.model = model
         self.batch = batch
         self.block_size = block_size
         self.max_len = max_len
-        pages = batch * (-(-max_len // block_size))
-        self.allocator = PageAllocator(pages, block_size, batch, max_len, device)
+        pages = batch * (-(-max_len // block_size)) + -(-prefix_len // block_size)
+        self.allocator = PageAllocator(pages, block_size, batch + (prefix_len > 0), max(max_len, prefix_len), device)
+        self.prefix_len = prefix_len          # tokens reserved for the prefix; after prefill, those it has
+        self.prefix = None
+        self.logprobs = logprobs
+        self.scores = None
         self.caches = [PagedKVCache(pages, block_size, cfg.num_kv_heads, cfg.head_dim, device, cache_dtype)
                        for _ in range(cfg.num_layers)]
         self.device = t.device(device)
@@ -53,16 +69,34 @@ class GreedyDecoder:
         self.step_index = t.zeros(1, dtype=t.int64, device=device)
         self.graph = None
 
-    def prefill(self, prompts: t.Tensor) -> t.Tensor:
-        """prompts [B, P] int64 -> first sampled tokens [B] (also the next step's input)."""
+    def _prefill_prefix(self, prefix: t.Tensor | None):
+        """The shared prefix [P] int64 into the cache, as request `batch`."""
+        given = 0 if prefix is None else prefix.shape[0]
+        if given > self.prefix_len:
+            raise ValueError(f"GreedyDecoder: a prefix of {given} tokens, {self.prefix_len} are reserved")
+        self.prefix_len = given
+        if given == 0:
+            return
+        slot = self.allocator.allocate_request(self.batch, given)
+        positions = t.arange(given, device=self.device)
+        cu = t.tensor([0, given], dtype=t.int32, device=self.device)
+        ctx = self.allocator.create_container(t.tensor([slot], dtype=t.int64, device=self.device), cu, positions, validate=False)
+        self.model(prefix.to(self.device), StepMeta("prefill", positions, ctx, cu_seqlens=cu, max_seqlen=given), self.caches)
+        self.allocator.advance(self.batch, given)
+        self.prefix = SharedPrefix.one(slot, given, self.batch, self.device)
+
+    def prefill(self, prompts: t.Tensor, prefix: t.Tensor | None = None) -> t.Tensor:
+        """prompts [B, P] int64, behind `prefix` [N] int64 if given -> first sampled tokens [B] (also the next
+        step's input)."""
         batch, length = prompts.shape
         assert batch == self.batch and length < self.max_len
+        self._prefill_prefix(prefix)
         slots = [self.allocator.allocate_request(i, self.max_len) for i in range(batch)]
         self.slots = t.tensor(slots, dtype=t.int64, device=self.device)
         positions = t.arange(length, device=self.device).repeat(batch)
         cu = t.arange(batch + 1, device=self.device, dtype=t.int32) * length
         ctx = self.allocator.create_container(self.slots, cu, positions, validate=False)
-        meta = StepMeta("prefill", positions, ctx, cu_seqlens=cu, max_seqlen=length)
+        meta = StepMeta("prefill", positions + self.prefix_len, ctx, cu_seqlens=cu, max_seqlen=length, prefix=self.prefix)
         logits = self.model(prompts.reshape(-1).to(self.device), meta, self.caches)
         self.allocator.advance_batch(list(range(batch)), [length] * batch)
         self.tokens.copy_(logits.argmax(-1))
@@ -70,6 +104,11 @@ class GreedyDecoder:
         self.context_lengths.fill_(length + 1)
         # Every later token of every sequence, in decode order (fixed address).
         self.history = t.zeros(self.max_len - length, batch, dtype=t.int64, device=self.device)
+        if self.logprobs is not None:
+            shape = self.history.shape
+            self.scores = TokenLogprobs(t.zeros(shape, device=self.device), t.zeros(shape, device=self.device),
+                                        t.zeros((*shape, self.logprobs), device=self.device),
+                                        t.zeros((*shape, self.logprobs), dtype=t.int64, device=self.device))
         self.step_index.zero_()
         self.steps_left = self.max_len - length
         return self.tokens.clone()
@@ -82,10 +121,15 @@ class GreedyDecoder:
         offsets = self.positions % self.block_size
         # The new token of every sequence is written at its last attended position.
         ctx = CacheContainer(self.slots, blocks, offsets, self.context_lengths, table, appends_last_position=True)
-        meta = StepMeta("decode", self.positions, ctx)
+        # Positions count from the prefix's first token.
+        at = self.positions + self.prefix_len if self.prefix is not None else self.positions
+        meta = StepMeta("decode", at, ctx, prefix=self.prefix)
         logits = self.model(self.tokens, meta, self.caches)
         nxt = logits.argmax(-1)
         self.history.index_copy_(0, self.step_index, nxt.unsqueeze(0))
+        if self.scores is not None:
+            for kept, got in zip(self.scores, token_logprobs(logits, nxt, self.logprobs)):
+                kept.index_copy_(0, self.step_index, got.unsqueeze(0))
         self.step_index.add_(1)
         self.tokens.copy_(nxt)
         self.positions.add_(1)

@@ -25,7 +25,8 @@ kernel itself);
 the projections and the FFN are `RowLinear`: the HIP kernel `skinny_linear_kernel` for the
 few rows of a decode step, which then also does RoPE and the activation, plain GEMMs (hipBLASLt through torch) otherwise; prompt
 (prefill) attention is the varlen causal HIP kernel behind `flash_attention_forward`,
-as the reference calls its FlashAttentionFunction there (`attention.py:103-110`).
+as the reference calls its FlashAttentionFunction there (`attention.py:103-110`). Sequences that
+share a prefix in the cache (`StepMeta.prefix`) attend it through `shared_prefix_attention`.
 """
 
 from __future__ import annotations
@@ -40,6 +41,8 @@ from torch.nn import functional as F
 from aiproj_amd import _native
 from aiproj_amd.kernals.decode_attention import append_decode_attention
 from aiproj_amd.kernals.flash_attention import flash_attention_forward
+from aiproj_amd.kernals.shared_prefix_attention import (SharedPrefix, append_shared_prefix_decode_attention,
+                                                        shared_prefix_prefill_attention)
 from aiproj_amd.model.rmsnorm import add_rmsnorm, rmsnorm_forward
 
 
@@ -67,6 +70,8 @@ class StepMeta:
     cache_context: object              # CacheContainer: slots, physical_blocks, block_offsets, ...
     cu_seqlens: t.Tensor | None = None  # prefill only: [B + 1] offsets of the packed prompts (device)
     max_seqlen: int = 0                 # prefill only: longest prompt (host int)
+    prefix: SharedPrefix | None = None  # prefixes in the cache that the sequences continue
+    all_logits: bool = False            # prefill only: logits of every token, not of each prompt's last
 
 
 class RoPE(nn.Module):
@@ -218,12 +223,19 @@ class Attention(nn.Module):
             split = self.rope.split(qkv, meta.token_positions, cfg.num_q_heads, cfg.num_kv_heads)
             if split is not None:
                 q, k, v = split
-                out, _ = flash_attention_forward(q, k, v, meta.cu_seqlens, meta.max_seqlen, 1.0 / math.sqrt(cfg.head_dim))
+                out = self._attend_prompts(q, k, v, meta, cache)
                 cache.append_kv(ctx.physical_blocks, ctx.block_offsets, k, v)
                 return self.o_proj(out.reshape(-1, self.q_dim))
         # q and k heads are the first Hq + Hkv heads of every row: one in-place rotation.
         self.rope.apply_(qkv, meta.token_positions, cfg.num_q_heads + cfg.num_kv_heads)
         return self._attend(qkv, meta, cache)
+
+    def _attend_prompts(self, q: t.Tensor, k: t.Tensor, v: t.Tensor, meta: StepMeta, cache) -> t.Tensor:
+        scale = 1.0 / math.sqrt(self.cfg.head_dim)
+        if meta.prefix is not None:
+            return shared_prefix_prefill_attention(q, k, v, meta.cu_seqlens, meta.max_seqlen, scale, cache,
+                                                   meta.cache_context.block_table, meta.prefix)[0]
+        return flash_attention_forward(q, k, v, meta.cu_seqlens, meta.max_seqlen, scale)[0]
 
     def _attend(self, qkv: t.Tensor, meta: StepMeta, cache) -> t.Tensor:
         """The cache write, the attention and the output projection of rotated fused rows."""
@@ -234,9 +246,10 @@ class Attention(nn.Module):
         if meta.mode == "prefill":
             # The varlen causal HIP kernel (reference FlashAttentionFunction, `attention.py:103-110`).
             # q, k and v are views into the fused projection; the kernel takes packed rows.
-            out, _ = flash_attention_forward(q.contiguous(), k.contiguous(), v.contiguous(), meta.cu_seqlens,
-                                             meta.max_seqlen, 1.0 / math.sqrt(cfg.head_dim))
+            out = self._attend_prompts(q.contiguous(), k.contiguous(), v.contiguous(), meta, cache)
             cache.append_kv(ctx.physical_blocks, ctx.block_offsets, k, v)
+        elif meta.prefix is not None:
+            out = append_shared_prefix_decode_attention(q, k, v, cache, ctx, meta.prefix)
         else:
             # append_kv + decode_attention_wrapper (`attention.py:86-99`) as one call: on the
             # FP8 cache the decode kernel writes each sequence's new token itself.
@@ -304,7 +317,7 @@ class TransformerLM(nn.Module):
     @t.no_grad()
     def forward(self, tokens: t.Tensor, meta: StepMeta, caches) -> t.Tensor:
         """Logits [B, vocab]: of every token in decode mode (one per sequence), of each
-        prompt's last token in prefill mode."""
+        prompt's last token in prefill mode (of every token with `all_logits`)."""
         eps = self.cfg.rms_eps
         x = self.embed(tokens)
         h, _ = rmsnorm_forward(x, self.layers[0].mixer_norm, eps)
@@ -314,7 +327,7 @@ class TransformerLM(nn.Module):
             f = layer.ffn(h)
             nxt = self.layers[i + 1].mixer_norm if i + 1 < len(self.layers) else self.final_norm
             x, h = add_rmsnorm(x, f, nxt, eps)
-        if meta.mode == "prefill":
+        if meta.mode == "prefill" and not meta.all_logits:
             # Only the last prompt token of each sequence is sampled from.
             last = meta.cu_seqlens[1:].long() - 1
             h = h[last]

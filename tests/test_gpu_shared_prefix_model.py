@@ -1,0 +1,131 @@
+"""Shared prefixes and log probabilities in the decoder model: GreedyDecoder and score_continuations."""
+
+import pytest
+import torch as t
+
+from aiproj_amd.inference.greedy_decoder import GreedyDecoder
+from aiproj_amd.inference.page_allocator import PageAllocator
+from aiproj_amd.inference.paged_kv_cache import PagedKVCache
+from aiproj_amd.inference.scoring import score_continuations
+from aiproj_amd.kernals.token_logprobs import token_logprobs
+from aiproj_amd.model.transformer import ModelConfig, StepMeta, TransformerLM
+
+pytestmark = pytest.mark.gpu
+
+SMALL = ModelConfig(vocab_size=256, d_model=256, num_layers=2, num_q_heads=8, num_kv_heads=2, head_dim=64,
+                    d_ff=512, max_seq_len=256)
+# Logits of one model through two orders of its products, as for prefill and decode against one whole prefill.
+RTOL, ATOL = 3e-2, 1e-1
+
+
+@pytest.fixture(scope="module")
+def model():
+    g = t.Generator(device="cuda").manual_seed(3)
+    return TransformerLM(SMALL).to(device="cuda", dtype=t.bfloat16).init_weights(g).eval()
+
+
+def _tokens(*shape, seed=0):
+    g = t.Generator(device="cuda").manual_seed(seed)
+    return t.randint(0, SMALL.vocab_size, shape, generator=g, device="cuda")
+
+
+def _whole_logits(model, rows):
+    """Logits of every token of whole sequences, packed, without a prefix."""
+    lengths = [len(r) for r in rows]
+    alloc = PageAllocator(sum(-(-n // 16) for n in lengths), 16, len(rows), max(lengths), "cuda")
+    caches = [PagedKVCache(alloc.num_blocks, 16, SMALL.num_kv_heads, SMALL.head_dim, "cuda", t.bfloat16)
+              for _ in range(SMALL.num_layers)]
+    slots = t.tensor([alloc.allocate_request(i, n) for i, n in enumerate(lengths)], device="cuda")
+    cu = t.tensor([0, *lengths], device="cuda").cumsum(0).to(t.int32)
+    pos = t.cat([t.arange(n, device="cuda") for n in lengths])
+    ctx = alloc.create_container(slots, cu, pos, validate=False)
+    meta = StepMeta("prefill", pos, ctx, cu_seqlens=cu, max_seqlen=max(lengths), all_logits=True)
+    return model(t.cat(rows), meta, caches).split(lengths)
+
+
+@pytest.mark.parametrize("prefix_len", [1, 37, 100])
+def test_shared_prefix_decodes_like_whole_prompts(model, prefix_len):
+    """Prefill and eight forced decode steps behind a shared prefix against whole sequences, unquantized cache."""
+    batch, length, steps = 5, 9, 8
+    prefix, rows = _tokens(prefix_len), _tokens(batch, length + steps, seed=1)
+    decoder = GreedyDecoder(model, batch, length + steps, cache_dtype=t.bfloat16, prefix_len=prefix_len + 3)
+    decoder.prefill(rows[:, :length], prefix)
+    want = [x.float() for x in _whole_logits(model, [t.cat([prefix, r]) for r in rows])]
+    for i in range(steps):
+        decoder.tokens.copy_(rows[:, length + i])
+        got = decoder.step().float()
+        for b in range(batch):
+            t.testing.assert_close(got[b], want[b][prefix_len + length + i], rtol=RTOL, atol=ATOL)
+
+
+@pytest.mark.parametrize("cache_dtype", [t.bfloat16, t.float8_e4m3fn])
+def test_graph_replays_equal_eager_steps(model, cache_dtype):
+    """Tokens, and the scores that every step records, of replayed and eager decoding."""
+    prefix, prompts = _tokens(70), _tokens(6, 5, seed=2)
+    runs = []
+    for use_graph in (False, True):
+        decoder = GreedyDecoder(model, 6, 40, cache_dtype=cache_dtype, prefix_len=70, logprobs=4)
+        decoder.prefill(prompts, prefix)
+        tokens = decoder.generate(20, use_graph=use_graph)
+        runs.append((tokens, *(x[:20] for x in decoder.scores)))
+    for a, b in zip(*runs):
+        assert t.equal(a, b)
+    tokens, logprobs, entropy, top_logprobs, top_tokens = runs[0]
+    # The chosen token is the most probable one.
+    assert t.equal(top_tokens[..., 0], tokens) and t.equal(top_logprobs[..., 0], logprobs)
+    assert bool((logprobs < 0).all()) and bool((entropy > 0).all())
+
+
+def test_scores_are_those_of_the_logits(model):
+    decoder = GreedyDecoder(model, 3, 30, logprobs=2)
+    decoder.prefill(_tokens(3, 7, seed=4))
+    for i in range(5):
+        logits = decoder.step()
+        want = token_logprobs(logits, decoder.tokens, 2)
+        for kept, got in zip(decoder.scores, want):
+            assert t.equal(kept[i], got)
+
+
+def test_decoder_without_prefix_or_scores_is_as_before(model):
+    prompts = _tokens(4, 6, seed=5)
+    plain, with_room = GreedyDecoder(model, 4, 30), GreedyDecoder(model, 4, 30, prefix_len=20)
+    assert plain.scores is None
+    assert t.equal(plain.prefill(prompts), with_room.prefill(prompts))
+    assert t.equal(plain.generate(10), with_room.generate(10))
+
+
+def test_refused_prefixes(model):
+    with pytest.raises(ValueError):
+        GreedyDecoder(model, 2, 200, prefix_len=57)                    # past the model's positions
+    with pytest.raises(ValueError):
+        GreedyDecoder(model, 2, 20, logprobs=65)
+    decoder = GreedyDecoder(model, 2, 20, prefix_len=8)
+    with pytest.raises(ValueError):
+        decoder.prefill(_tokens(2, 3), _tokens(9))
+
+
+@pytest.mark.parametrize("lengths", [[1], [1, 1, 1], [5, 1, 17, 2], [40, 33]])
+def test_continuations_score_like_whole_sequences(model, lengths):
+    """Log probabilities of continuations against those of whole sequences' logits in float64."""
+    prompt, continuations = _tokens(50, seed=6), [_tokens(n, seed=7 + i) for i, n in enumerate(lengths)]
+    got = score_continuations(model, prompt, continuations, top=3, cache_dtype=t.bfloat16)
+    whole = _whole_logits(model, [t.cat([prompt, c]) for c in continuations])
+    assert [len(g.logprobs) for g in got] == lengths
+    for g, c, logits in zip(got, continuations, whole):
+        rows = logits[len(prompt) - 1:-1].double()
+        logp = t.log_softmax(rows, -1)
+        want = logp.gather(1, c[:, None])[:, 0]
+        # A log probability is off by at most the largest error of its row's logits and that of their log sum.
+        slack = 2 * (ATOL + RTOL * rows.abs().amax(-1))
+        assert bool(((g.logprobs.double() - want).abs() <= slack).all())
+        assert bool(((g.top_logprobs.double() - logp.gather(1, g.top_tokens)).abs() <= slack[:, None]).all())
+        assert g.top_tokens.shape == (len(c), 3) and bool((g.entropy > 0).all())
+
+
+def test_refused_continuations(model):
+    prompt = _tokens(250)
+    for bad in ([], [_tokens(0)], [_tokens(7)], [_tokens(2, 3)]):
+        with pytest.raises(ValueError):
+            score_continuations(model, prompt, bad)
+    with pytest.raises(ValueError):
+        score_continuations(model, prompt[:0], [_tokens(2)])
