@@ -37,6 +37,27 @@ typedef __attribute__((address_space(3))) const u32x2_t lds_u32x2;
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+// c += a b of 32 x 16 and 16 x 32 (lane l: A[l % 32][8 (l / 32) + i], B likewise, c[8 (i / 4) + 4 (l / 32) + i % 4][l % 32]).
+template <bool kF16>
+__device__ __forceinline__ f32x16_t mma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+    if constexpr (kF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// Over the two lanes of a row.
+__device__ __forceinline__ float max_across_halves(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    return fmaxf(as_float(a[0]), as_float(a[1]));
+}
+__device__ __forceinline__ float sum_across_halves(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    return as_float(a[0]) + as_float(a[1]);
+}
+
 // Two codes -> two 16-bit values in a dword.
 template <bool kF16, bool kHi>
 __device__ __forceinline__ uint32_t widen2(uint32_t x) {
@@ -51,11 +72,12 @@ struct WideLds {
     uint8_t v[2][kKeys * kRow];
     float scale[4][2][kKeys];
     int32_t count[4][4];                                 // tokens of each tile that count
+    uint8_t spare[16 + 256];                             // what lanes without a value write
 };
 
 // NW waves, 32 rows each.
 template <int kD, int QT, int ES, int NW>
-__global__ void __launch_bounds__(64 * NW)
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
     static_assert(kD % 16 == 0 && kD >= 64 && kD <= 128 && (ES == 1 || kD % 64 == 0), "head sizes of this kernel");
     using T = typename Elem<QT>::T;
@@ -65,8 +87,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
     constexpr int kThreads = 64 * NW;
     constexpr int ROW = WideLds<kD>::kRow;
     constexpr int CPR = ROW / 16;                        // 16-byte chunks of an LDS row
-    constexpr int NB = kD / 16, KS = kD / 32;
-    constexpr bool kHalf = kD % 32 != 0;                 // and one step of 16 dims
+    constexpr int NB = (kD + 31) / 32, KS = kD / 16;     // blocks of 32 dims of O, steps of 16 dims of Q K^T
     // Staging: a row of K or V is `SLOTS` runs of 16 bytes of cache; slot x of the block's 2 x 64 x SLOTS goes to
     // thread x % kThreads. A wave's rows of one load lie in one 16-token tile, so its page is wave-uniform.
     constexpr int SLOTS = ES == 1 ? CPR / 2 : CPR;
@@ -93,13 +114,17 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
     PrefixItem it;
     if (!prefix_item(a, grid, 32 * NW, it)) return;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int m16 = lane & 15, j = lane >> 4;
+    const int col = lane & 31, hi = lane >> 5;           // the lane's row of a wave's, and half
     const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
     const int h = it.h;
     const int32_t blocks = (it.hi - it.lo + kKeys - 1) / kKeys;
     const int32_t r0 = it.r0 + 32 * wave;                // first pair of the wave
     const bool active = r0 < it.pairs;
 
+    // Where chunk c of an LDS row stands.
+    auto swizzle = [](int row, int c) __attribute__((always_inline)) {
+        return 16 * (c ^ (CPR == 16 ? ((row & 3) << 2) | ((row >> 2) & 3) : (row >> 1) & 7));
+    };
     // Row and tensor of load i of this thread; the tile of its wave's rows.
     auto row_of = [&](int i) __attribute__((always_inline)) { return ((int)threadIdx.x + kThreads * i) % PER / SLOTS; };
     auto wave_row = [&](int i) __attribute__((always_inline)) { return (64 * wave + kThreads * i) % PER / SLOTS; };
@@ -122,6 +147,10 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
 #pragma unroll
         for (int u = 0; u < TILES; ++u) page[u] = fetch_page(g, u);
     };
+    const uint32_t pages = (uint32_t)min(a.d.num_blocks, (int64_t)INT32_MAX);
+    // A thread's rows have one place in their tiles, and so one offset behind a tile's first row.
+    const uint32_t row_off = (uint32_t)((row_of(0) & 15) * (int32_t)row_bytes + 16 * (run < RUNS ? run : 0));
+    const uint32_t scale_off = (uint32_t)(((wave_row(0) & 15) + s_row) * a.d.num_kv_heads);
     u32x4_t raw[LOADS];
     float scale[TILES];
     int64_t base[TILES];                                 // first cache row of the wave's tiles: of the K block in flight
@@ -130,9 +159,9 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
 #pragma unroll
         for (int u = 0; u < TILES; ++u) {
             const int32_t tok = it.lo + g * kKeys + (wave_row(u) & ~15);
-            const bool ok = page[u] >= 0 && page[u] < a.d.num_blocks && tok < it.hi;
+            const bool ok = (uint32_t)page[u] < pages && tok < it.hi;
             count_k[u] = ok ? min(16, it.hi - tok) : 0;
-            base[u] = ok ? (int64_t)page[u] * a.d.block_size + (tok & (a.d.block_size - 1)) : 0;
+            base[u] = (int64_t)(ok ? page[u] : 0) * a.d.block_size + (ok ? tok & (a.d.block_size - 1) : 0);
         }
     };
     auto is_v = [&](int i) __attribute__((always_inline)) { return kByWave ? loads_v : kThreads * i >= PER; };
@@ -140,9 +169,8 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             if (is_v(i) != v) continue;
-            const uint8_t* src = reinterpret_cast<const uint8_t*>(v ? a.d.v_cache : a.d.k_cache) +
-                                 (base[i % TILES] + (row_of(i) & 15)) * row_bytes + h * kD * ES + 16 * (run < RUNS ? run : 0);
-            raw[i] = *reinterpret_cast<const u32x4_t*>(src);
+            const uint8_t* src = reinterpret_cast<const uint8_t*>(v ? a.d.v_cache : a.d.k_cache) + base[i % TILES] * row_bytes + h * kD * ES;
+            raw[i] = *reinterpret_cast<const u32x4_t*>(src + row_off);
         }
         if (v) {
 #pragma unroll
@@ -150,7 +178,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
         } else if constexpr (ES == 1) {
 #pragma unroll
             for (int u = 0; u < TILES; ++u)
-                scale[u] = (s_tensor ? a.d.v_scales : a.d.k_scales)[(base[u] + (wave_row(u) & 15) + s_row) * a.d.num_kv_heads + h];
+                scale[u] = ((s_tensor ? a.d.v_scales : a.d.k_scales) + base[u] * a.d.num_kv_heads + h)[scale_off];
         }
     };
     // Rows that do not count become zeros (their bytes may be anything).
@@ -161,7 +189,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
             const int row = row_of(i);
             const bool live = (row & 15) < (v ? count_v : count_k)[i % TILES];
             uint8_t* dst = (v ? lds_v[buf] : lds_k[buf]) + row * ROW;
-            if (run >= RUNS) continue;
+            const bool held = run < RUNS;                // else to where nobody reads
             if constexpr (ES == 1) {
                 u32x4_t x[2];
 #pragma unroll
@@ -177,184 +205,192 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
                 }
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    *reinterpret_cast<u32x4_t*>(dst + 16 * ((2 * run + e) ^ (row % CPR))) = x[e];
+                    *reinterpret_cast<u32x4_t*>(held ? dst + swizzle(row, 2 * run + e) : lds.wide.spare) = x[e];
             } else {
-                *reinterpret_cast<u32x4_t*>(dst + 16 * (run ^ (row % CPR))) = live ? raw[i] : u32x4_t{0u, 0u, 0u, 0u};
+                *reinterpret_cast<u32x4_t*>(held ? dst + swizzle(row, run) : lds.wide.spare) = live ? raw[i] : u32x4_t{0u, 0u, 0u, 0u};
             }
         }
         if (v) return;
         if constexpr (ES == 1) {
 #pragma unroll
             for (int u = 0; u < TILES; ++u) {
-                const float x = (wave_row(u) & 15) + s_row < count_k[u] ? scale[u] : 0.0f;
-                if (s_mine) lds_scale[g & 3][s_tensor][wave_row(u) + s_row] = s_tensor ? x : x * a.d.score_scale;
+                const int row = wave_row(u) + s_row;
+                const float x = (row & 15) < count_k[u] ? scale[u] : 0.0f;
+                *(s_mine ? &lds_scale[g & 3][s_tensor][row] : reinterpret_cast<float*>(lds.wide.spare) + 4 + lane) = s_tensor ? x : x * a.d.score_scale;
             }
         }
 #pragma unroll
         for (int u = 0; u < TILES; ++u)
-            if (lane == 0 && !loads_v && wave_row(u) % 16 == 0) lds_count[g & 3][wave_row(u) / 16] = count_k[u];
+            *(lane == 0 && !loads_v && wave_row(u) % 16 == 0 ? &lds_count[g & 3][wave_row(u) / 16]
+                                                             : reinterpret_cast<int32_t*>(lds.wide.spare) + 4 + lane) = count_k[u];
     };
 
-    // Q^T operands: lane (row 16 qt + l % 16, l / 16) holds dims 32 s + 8 (l / 16) .. + 7 (pairs past the last
-    // repeat it: their rows are never stored).
-    u32x4_t qop[2][KS];
-    uint2 qhalf[2];
+    // Q^T operands: lane (row l % 32, l / 32) holds dims 16 s + 8 (l / 32) .. + 7 (pairs past the last repeat it: their
+    // rows are never stored).
+    u32x4_t qop[KS];
     auto load_q = [&]() __attribute__((always_inline)) {
+        const int32_t pair = min(r0 + col, it.pairs - 1);
+        const int32_t t = (uint32_t)pair / (uint32_t)G;
+        const T* src = reinterpret_cast<const T*>(a.d.q) + (int64_t)(it.rs + t) * a.d.q_stride_b + (h * G + (pair - t * G)) * a.d.q_stride_h;
+        auto element2 = [&](int d) __attribute__((always_inline)) { return (uint32_t)src[d] | ((uint32_t)src[d + 1] << 16); };
 #pragma unroll
-        for (int qt = 0; qt < 2; ++qt) {
-            const int32_t pair = min(r0 + 16 * qt + m16, it.pairs - 1);
-            const int32_t t = (uint32_t)pair / (uint32_t)G;
-            const T* src = reinterpret_cast<const T*>(a.d.q) + (int64_t)(it.rs + t) * a.d.q_stride_b + (h * G + (pair - t * G)) * a.d.q_stride_h;
-            auto element2 = [&](int d) __attribute__((always_inline)) { return (uint32_t)src[d] | ((uint32_t)src[d + 1] << 16); };
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const int d = 32 * s + 8 * j;
-                if (grid.q_vec) qop[qt][s] = *reinterpret_cast<const u32x4_t*>(src + d);
-                else qop[qt][s] = u32x4_t{element2(d), element2(d + 2), element2(d + 4), element2(d + 6)};
-            }
-            if constexpr (kHalf) {
-                const int d = 32 * KS + 4 * j;
-                if (grid.q_vec) qhalf[qt] = *reinterpret_cast<const uint2*>(src + d);
-                else qhalf[qt] = make_uint2(element2(d), element2(d + 2));
-            }
+        for (int s = 0; s < KS; ++s) {
+            const int d = 16 * s + 8 * hi;
+            if (grid.q_vec) qop[s] = *reinterpret_cast<const u32x4_t*>(src + d);
+            else qop[s] = u32x4_t{element2(d), element2(d + 2), element2(d + 4), element2(d + 6)};
         }
     };
 
-    // Per-lane byte offsets of the operand reads: K row m16, chunk 4 s + j; V^T as in the transposing read
-    // ds_read_b64_tr_b16: lane (j, m16) reads dims 16 nb + 4 (m16 % 4) .. + 3 of key 4 j + m16 / 4 of a 16-key
-    // tile and receives V[4 j + r][16 nb + m16], r = 0..3.
-    int k_off[KS], k_half = 0, v_off[NB];
+    // Per-lane byte offsets of the operand reads: K row l % 32, chunk 2 s + l / 32. V^T by the transposing read
+    // ds_read_b64_tr_b16: of 16 lanes lane i reads dims 4 (i % 4) .. + 3 of key i / 4 of a block of 4 keys x 16 dims and
+    // receives dim i of the four keys. Lanes 0..15 and 16..31 (32..47, 48..63) take the two halves of 32 dims, lanes
+    // below 32 keys 0..3 and 8..11 (two reads) of 16, the others 4..7 and 12..15: what their scores belong to. Dims
+    // past the head size are read from chunks that nobody writes and end in rows of O that nobody stores.
+    int k_off[KS], v_off[NB][2];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) k_off[s] = m16 * ROW + 16 * ((4 * s + j) ^ (m16 % CPR));
-    if constexpr (kHalf) k_half = m16 * ROW + 16 * ((4 * KS + (j >> 1)) ^ (m16 % CPR)) + 8 * (j & 1);
-    {
-        const int vrow = 4 * j + (m16 >> 2);
+    for (int s = 0; s < KS; ++s) k_off[s] = col * ROW + swizzle(col, 2 * s + hi);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-            v_off[nb] = vrow * ROW + 16 * ((2 * nb + ((m16 >> 1) & 1)) ^ (vrow % CPR)) + 8 * (m16 & 1);
-    }
-
-    f32x4_t o[2][NB];
-    float m[2], l[2];
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int qt = 0; qt < 2; ++qt) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) o[qt][nb] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        m[qt] = kNegInf;
-        l[qt] = 0.0f;
-    }
-
-    f32x4_t sacc[4][2];
-    auto qk = [&](auto buf_c) __attribute__((always_inline)) {
-        constexpr int buf = decltype(buf_c)::value;
-        lds_u8* const kl = (lds_u8*)&lds_k[buf][0];
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
-                const u32x4_t kop = *(lds_u32x4*)(kl + k_off[s] + 16 * kt * ROW);
-#pragma unroll
-                for (int qt = 0; qt < 2; ++qt)
-                    sacc[kt][qt] = mma16<kF16>(kop, qop[qt][s], s == 0 ? f32x4_t{0.0f, 0.0f, 0.0f, 0.0f} : sacc[kt][qt]);
-            }
-        if constexpr (kHalf) {
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
-                const uint2 kop = __builtin_bit_cast(uint2, *(lds_u32x2*)(kl + k_half + 16 * kt * ROW));
-#pragma unroll
-                for (int qt = 0; qt < 2; ++qt) sacc[kt][qt] = mma16_half<kF16>(kop, qhalf[qt], sacc[kt][qt]);
-            }
+        for (int e = 0; e < 2; ++e) {
+            const int vrow = 8 * e + 4 * hi + ((lane & 15) >> 2), chunk = 4 * nb + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+            v_off[nb][e] = vrow * ROW + swizzle(vrow, chunk) + 8 * (lane & 1);
         }
-    };
-    // P'^T operands; pp holds tokens 16 (2 pp + i / 4) + 4 j + i % 4.
+
+    f32x16_t o[NB];
+    float ref = 0.0f, lim = kNegInf, l = 0.0f;           // a row's reference (0 before its first score), how far scores may pass it
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[nb][i] = 0.0f;
+
+    // Scores and P'^T operands of a block's halves of 32 tokens. Score i of a row: token 8 (i / 4) + 4 (l / 32) + i % 4.
+    f32x16_t sacc[2];
     u32x4_t pop[2][kParts][2];
-    auto softmax = [&](int32_t g) __attribute__((always_inline)) {
-        const float(*scales)[kKeys] = lds_scale[g & 3];
-        // Scaled scores (score i of a row: token 16 (i / 4) + 4 j + i % 4).
+    // Steps of K operands that are read before the products of a half, the others among them.
+    constexpr int kPre = KS / 2;
+    u32x4_t kop[KS];
+    auto read_k = [&](auto buf_c, auto half_c, int first, int last) __attribute__((always_inline)) {
+        constexpr int buf = decltype(buf_c)::value, half = decltype(half_c)::value;
+        lds_u8* const kl = (lds_u8*)&lds_k[buf][32 * half * ROW];
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-            float4 ks = make_float4(a.d.score_scale, a.d.score_scale, a.d.score_scale, a.d.score_scale);
-            if constexpr (ES == 1) {
-                ks = *reinterpret_cast<const float4*>(&scales[0][16 * kt + 4 * j]);
-            }
-#pragma unroll
-            for (int qt = 0; qt < 2; ++qt) {
-                sacc[kt][qt][0] *= ks.x;
-                sacc[kt][qt][1] *= ks.y;
-                sacc[kt][qt][2] *= ks.z;
-                sacc[kt][qt][3] *= ks.w;
-            }
-        }
-        const int4 counts = *reinterpret_cast<const int4*>(&lds_count[g & 3][0]);
-        const int n[4] = {uniform(counts.x), uniform(counts.y), uniform(counts.z), uniform(counts.w)};
-        if (n[0] + n[1] + n[2] + n[3] < kKeys) {         // wave-uniform
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                for (int jj = 0; jj < 4; ++jj)
-                    if (4 * j + jj >= n[kt]) sacc[kt][0][jj] = sacc[kt][1][jj] = kNegInf;
-        }
-        float neg_m[2];
-#pragma unroll
-        for (int qt = 0; qt < 2; ++qt) {
-            float mx = sacc[0][qt][0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sacc[i / 4][qt][i % 4]);
-            // The reference moves where some row's maximum passes it by 2^8; each lane tests its 16 tokens.
-            if (__ballot(mx > m[qt] + kLag)) {
-                const float m_new = fmaxf(m[qt], max_across_rows(mx));
-                const float alpha = __builtin_amdgcn_exp2f(m[qt] - (m_new == kNegInf ? 0.0f : m_new));
-                l[qt] *= alpha;
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) o[qt][nb] *= alpha;
-                m[qt] = m_new;
-            }
-            neg_m[qt] = m[qt] == kNegInf ? 0.0f : -m[qt];
-        }
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-            f32x4_t vs = {1.0f, 1.0f, 1.0f, 1.0f};
-            if constexpr (ES == 1) vs = *reinterpret_cast<const f32x4_t*>(&scales[1][16 * kt + 4 * j]);
-#pragma unroll
-            for (int qt = 0; qt < 2; ++qt) {
-                float x[4];
-#pragma unroll
-                for (int jj = 0; jj < 4; ++jj) {
-                    const float p = __builtin_amdgcn_exp2f(sacc[kt][qt][jj] + neg_m[qt]);
-                    l[qt] += p;
-                    x[jj] = ES == 1 ? p * vs[jj] : p;
-                }
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const uint32_t top = pack2<kF16V>(x[2 * w], x[2 * w + 1]);
-                    pop[qt][0][kt >> 1][2 * (kt & 1) + w] = top;
-                    if constexpr (kParts == 2)
-                        pop[qt][1][kt >> 1][2 * (kt & 1) + w] =
-                            pack2<false>(x[2 * w] - bits_f32(top << 16), x[2 * w + 1] - bits_f32(top & 0xFFFF0000u));
-                }
-            }
-        }
+        for (int s = first; s < last; ++s) kop[s] = *(lds_u32x4*)(kl + k_off[s]);
     };
-    auto pv = [&](auto buf_c) __attribute__((always_inline)) {
-        constexpr int buf = decltype(buf_c)::value;
-        lds_u8* const vl = (lds_u8*)&lds_v[buf][0];
+    auto qk = [&](auto half_c) __attribute__((always_inline)) {
+        constexpr int half = decltype(half_c)::value;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) sacc[half] = mma32<kF16>(kop[s], qop[s], s == 0 ? f32x16_t{} : sacc[half]);
+    };
+    auto pv = [&](auto buf_c, auto half_c) __attribute__((always_inline)) {
+        constexpr int buf = decltype(buf_c)::value, half = decltype(half_c)::value;
+        lds_u8* const vl = (lds_u8*)&lds_v[buf][32 * half * ROW];
 #pragma unroll
         for (int pp = 0; pp < 2; ++pp)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 u32x4_t av;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vl + v_off[nb] + 16 * (2 * pp + half) * ROW));
+                for (int e = 0; e < 2; ++e) {
+                    const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vl + v_off[nb][e] + 16 * pp * ROW));
                     const uint2 w = __builtin_bit_cast(uint2, x);
-                    av[2 * half] = w.x;
-                    av[2 * half + 1] = w.y;
+                    av[2 * e] = w.x;
+                    av[2 * e + 1] = w.y;
                 }
 #pragma unroll
-                for (int qt = 0; qt < 2; ++qt)
-#pragma unroll
-                    for (int part = 0; part < kParts; ++part) o[qt][nb] = mma16<kF16V>(av, pop[qt][part][pp], o[qt][nb]);
+                for (int part = 0; part < kParts; ++part) o[nb] = mma32<kF16V>(av, pop[half][part][pp], o[nb]);
             }
+    };
+    // Scores of a half relative to the rows' references.
+    float mx;
+    int2 counts;                                         // tokens of the half's tiles that count
+    auto relate = [&](int32_t g, auto half_c) __attribute__((always_inline)) {
+        constexpr int half = decltype(half_c)::value;
+        counts = *reinterpret_cast<const int2*>(&lds_count[g & 3][2 * half]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            f32x4_t ks = {a.d.score_scale, a.d.score_scale, a.d.score_scale, a.d.score_scale};
+            if constexpr (ES == 1) ks = *reinterpret_cast<const f32x4_t*>(&lds_scale[g & 3][0][32 * half + 8 * q + 4 * hi]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sacc[half][4 * q + i] = __builtin_fmaf(sacc[half][4 * q + i], ks[i], -ref);
+        }
+    };
+    auto largest = [&](auto half_c) __attribute__((always_inline)) {
+        constexpr int half = decltype(half_c)::value;
+        mx = sacc[half][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sacc[half][i]);
+    };
+    // Tokens of the half that do not count, and references that have to move: where some row's maximum passes its
+    // own by 2^8 (each lane tests its 16 tokens). `alpha` is then the factor of what has been summed relative to the
+    // old reference: l at once, O one half later, when the last products of such weights have been added.
+    float alpha = 1.0f;
+    auto settle = [&](auto half_c) __attribute__((always_inline)) -> bool {
+        constexpr int half = decltype(half_c)::value;
+        const int n0 = uniform(counts.x), n1 = uniform(counts.y);
+        if (n0 + n1 < 32) {                              // wave-uniform
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (8 * (i / 4 % 2) + 4 * hi + i % 4 >= (i < 8 ? n0 : n1)) sacc[half][i] = kNegInf;
+            largest(half_c);
+        }
+        if (!__ballot(mx > lim)) return false;
+        const float top = max_across_halves(mx);         // relative to ref
+        const bool fresh = lim == kNegInf;
+        const float step = fresh ? (top == kNegInf ? 0.0f : top) : fmaxf(top, 0.0f);
+        alpha = fresh ? 0.0f : __builtin_amdgcn_exp2f(-step);
+        lim = fresh && top == kNegInf ? kNegInf : kLag;
+        ref += step;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sacc[half][i] -= step;
+        return true;
+    };
+    auto weigh = [&](int32_t g, auto half_c) __attribute__((always_inline)) {
+        constexpr int half = decltype(half_c)::value;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            f32x4_t vs = {1.0f, 1.0f, 1.0f, 1.0f};
+            if constexpr (ES == 1) vs = *reinterpret_cast<const f32x4_t*>(&lds_scale[g & 3][1][32 * half + 8 * q + 4 * hi]);
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(sacc[half][4 * q + i]);
+                l += p;
+                x[i] = ES == 1 ? p * vs[i] : p;
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const uint32_t top = pack2<kF16V>(x[2 * w], x[2 * w + 1]);
+                pop[half][0][q / 2][2 * (q % 2) + w] = top;
+                if constexpr (kParts == 2)
+                    pop[half][1][q / 2][2 * (q % 2) + w] =
+                        pack2<false>(x[2 * w] - bits_f32(top << 16), x[2 * w + 1] - bits_f32(top & 0xFFFF0000u));
+            }
+        }
+    };
+    // The products are spread over the softmax's operations, V's operand reads run ahead of them. What the region
+    // leaves is kept in its place: the compiler would sink it to its use behind the next branch, away from the products.
+    constexpr int kReads = 4 * NB + KS - kPre, kProducts = 2 * NB * kParts + KS, kAhead = (ES == 1 ? 8 : 0) + 1;
+    auto interleave = [&](auto half_c) __attribute__((always_inline)) {
+        constexpr int half = decltype(half_c)::value;
+        constexpr bool stages = half == 0;
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);                      // LDS reads of scales and counts
+#pragma unroll
+        for (int i = 0; i < kProducts; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                       // matrix products
+            __builtin_amdgcn_sched_group_barrier(0x402, stages ? 9 : 6, 0);          // softmax, widening
+            if (2 * i < kReads) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            else if (stages) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+        }
+#pragma unroll
+        for (int pp = 0; pp < 2; ++pp)
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+                u32x4_t& weights = pop[half][part][pp];
+                __asm__ volatile("" : "+v"(weights));
+            }
+        float &sum = l, &most = mx;
+        __asm__ volatile("" : "+v"(sum), "+v"(most));
     };
 
     // A barrier that waits for this wave's LDS operations and leaves its loads in flight.
@@ -364,6 +400,8 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
         __builtin_amdgcn_s_barrier();
         __asm__ volatile("" ::: "memory");
     };
+    constexpr std::integral_constant<int, 0> c0{};
+    constexpr std::integral_constant<int, 1> c1{};
     fetch(0);
     locate(0);
     issue(false);
@@ -375,122 +413,113 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
     issue(false);
     fetch(2);
     barrier();
-    constexpr std::integral_constant<int, 0> b0{};
-    constexpr std::integral_constant<int, 1> b1{};
-    // The matrix phase of step g (buffer of K(g), V(g): g % 2). Past the last block the staging moves rows that count
-    // nothing, so that there is no branch around it.
-    // Operand reads run ahead of the products by up to 16 (an LDS read under this load takes some 200 cycles, a
-    // product 16); left alone, the compiler reads each operand right before its use.
-    constexpr int kReads = 4 * NB + 4 * KS + (kHalf ? 4 : 0), kProducts = 4 * NB * kParts + 8 * KS + (kHalf ? 8 : 0);
-    constexpr int kAhead = 16, kPace = (kProducts - kAhead) / ((kReads - kAhead) / 2);
-    auto matrix = [&](int32_t g, auto buf_c, bool first) __attribute__((always_inline)) {
+    bool moved = false;
+    if (active) {
+        read_k(c0, c0, 0, KS);
+        qk(c0);
+        relate(0, c0);
+        largest(c0);
+        read_k(c0, c1, 0, kPre);
+        settle(c0);                                      // O and l are zeros yet
+    }
+    // Half `half` of block g, whose scores are there: its weights; the scores of the next half (of block gn,
+    // buffer kbuf); the products with V of the half before (buffer vbuf). All three are independent of each other.
+    auto part = [&](int32_t g, auto half_c, int32_t gn, auto kbuf_c, auto vbuf_c, bool first) __attribute__((always_inline)) {
+        constexpr std::integral_constant<int, 1 - decltype(half_c)::value> next{};
+        read_k(kbuf_c, next, kPre, KS);
+        qk(next);
+        weigh(g, half_c);
+        if (!first) pv(vbuf_c, next);
+        relate(gn, next);
+        largest(next);
+    };
+    auto rest = [&](auto half_c) __attribute__((always_inline)) {
+        if (moved) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) o[nb] *= alpha;
+        }
+        constexpr std::integral_constant<int, 1 - decltype(half_c)::value> next{};
+        moved = settle(next);
+    };
+    // Step g (buffer of K(g), V(g): g % 2). Past the last block the staging moves rows that count nothing, so that
+    // there is no branch around it.
+    auto step = [&](int32_t g, auto buf_c, bool first) __attribute__((always_inline)) {
         constexpr std::integral_constant<int, 1 - decltype(buf_c)::value> other{};
-        publish(true, decltype(buf_c)::value, g);
-        publish(false, other.value, g + 1);
-        issue(true);
-        locate(g + 2);
-        issue(false);
-        fetch(g + 3);
-        if (!active) return;
-        if (first) {
-            qk(buf_c);
+        auto stage = [&]() __attribute__((always_inline)) {
+            publish(true, decltype(buf_c)::value, g);
+            publish(false, other.value, g + 1);
+            issue(true);
+            locate(g + 2);
+            issue(false);
+            fetch(g + 3);
+        };
+        if (!active) {
+            stage();
+            barrier();
             return;
         }
-        pv(other);
-        qk(buf_c);
-        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);              // LDS reads
-#pragma unroll
-        for (int i = 0; i < (kReads - kAhead) / 2; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, kPace, 0);           // matrix products
-            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
+        part(g, c0, g, buf_c, other, first);
+        stage();
+        interleave(c0);
+        barrier();
+        read_k(other, c0, 0, kPre);
+        rest(c0);
+        part(g, c1, g + 1, other, buf_c, false);
+        interleave(c1);
+        read_k(other, c1, 0, kPre);
+        rest(c1);
     };
-    // Both halves run the same 2 * blocks barriers.
-    if (wave < NW / 2) {
-        matrix(0, b0, true);
-        barrier();
-        if (active) softmax(0);
-        barrier();
-        for (int32_t g = 1; g < blocks; g += 2) {
-            matrix(g, b1, false);
-            barrier();
-            if (active) softmax(g);
-            barrier();
-            if (g + 1 < blocks) {
-                matrix(g + 1, b0, false);
-                barrier();
-                if (active) softmax(g + 1);
-                barrier();
-            }
-        }
-    } else {
-        barrier();
-        matrix(0, b0, true);
-        barrier();
-        for (int32_t g = 1; g < blocks; g += 2) {
-            if (active) softmax(g - 1);
-            barrier();
-            matrix(g, b1, false);
-            barrier();
-            if (g + 1 < blocks) {
-                if (active) softmax(g);
-                barrier();
-                matrix(g + 1, b0, false);
-                barrier();
-            }
-        }
-        if (active) softmax(blocks - 1);
-    }
-    if (active) {
-        if ((blocks & 1) != 0) pv(b0);
-        else pv(b1);
+    step(0, c0, true);
+    for (int32_t g = 1; g < blocks; g += 2) {
+        step(g, c1, false);
+        if (g + 1 < blocks) step(g + 1, c0, false);
     }
     if (!active) return;
-
-    // Lane (row, j) holds dims 16 nb + 4 j + jj of its row.
+    if ((blocks & 1) != 0) pv(c0, c1);
+    else pv(c1, c1);
+    // Nothing moves behind the last block: its scores do not count.
+    const float m = lim == kNegInf ? kNegInf : ref;
+    const float lt = sum_across_halves(l);
+    const int32_t pair = r0 + col;
+    if (pair >= it.pairs) return;
+    const int32_t t = (uint32_t)pair / (uint32_t)G;
+    const int64_t row = it.rs + t;
+    const int hq = h * G + (pair - t * G);
+    // Element 4 q + i of block nb: dim 32 nb + 8 q + 4 hi + i of the row.
+    if (a.cu != nullptr && a.splits == 1) {
+        // The prompt form's only state of the row: joined with out and lse at once.
+        if (seq_of_row(a, row) < 0) return;
+        const int64_t at = row * a.d.num_q_heads + hq;
+        const float mo = a.lse[at] * kLog2e;
+        const float mn = fmaxf(m, mo), mu = mn == kNegInf ? 0.0f : mn;
+        const float wp = fast_exp2(m - mu), wo = fast_exp2(mo - mu);
+        const float den = lt * wp + wo;
+        const float inv = den > 0.0f || den != den ? 1.0f / den : 0.0f;
+        T* out = reinterpret_cast<T*>(a.d.out) + at * kD + 4 * hi;
 #pragma unroll
-    for (int qt = 0; qt < 2; ++qt) {
-        const float lt = sum_across_rows(l[qt]);
-        const int32_t pair = r0 + 16 * qt + m16;
-        if (pair >= it.pairs) continue;
-        const int32_t t = (uint32_t)pair / (uint32_t)G;
-        const int64_t row = it.rs + t;
-        const int hq = h * G + (pair - t * G);
-        if (a.cu != nullptr && a.splits == 1) {
-            // The prompt form's only state of the row: joined with out and lse at once.
-            if (seq_of_row(a, row) < 0) continue;
-            const int64_t at = row * a.d.num_q_heads + hq;
-            const float mo = a.lse[at] * kLog2e;
-            const float mn = fmaxf(m[qt], mo), mu = mn == kNegInf ? 0.0f : mn;
-            const float wp = fast_exp2(m[qt] - mu), wo = fast_exp2(mo - mu);
-            const float den = lt * wp + wo;
-            const float inv = den > 0.0f || den != den ? 1.0f / den : 0.0f;
-            T* out = reinterpret_cast<T*>(a.d.out) + at * kD + 4 * j;
+        for (int d = 0; d < kD; d += 8) {
+            uint2* dst = reinterpret_cast<uint2*>(out + d);
+            const uint2 x = *dst;
+            const float y[4] = {Elem<QT>::load((T)(x.x & 0xFFFFu)), Elem<QT>::load((T)(x.x >> 16)),
+                                Elem<QT>::load((T)(x.y & 0xFFFFu)), Elem<QT>::load((T)(x.y >> 16))};
+            float z[4];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                uint2* dst = reinterpret_cast<uint2*>(out + 16 * nb);
-                const uint2 x = *dst;
-                const float y[4] = {Elem<QT>::load((T)(x.x & 0xFFFFu)), Elem<QT>::load((T)(x.x >> 16)),
-                                    Elem<QT>::load((T)(x.y & 0xFFFFu)), Elem<QT>::load((T)(x.y >> 16))};
-                float z[4];
-#pragma unroll
-                for (int jj = 0; jj < 4; ++jj) z[jj] = (o[qt][nb][jj] * wp + y[jj] * wo) * inv;
-                *dst = make_uint2(pack2<kF16>(z[0], z[1]), pack2<kF16>(z[2], z[3]));
-            }
-            // The row's four lanes run in step: all have read lse.
-            if (j == 0) a.lse[at] = (mu + __builtin_log2f(den)) * kLn2;
-            continue;
+            for (int i = 0; i < 4; ++i) z[i] = (o[d / 32][d % 32 / 2 + i] * wp + y[i] * wo) * inv;
+            *dst = make_uint2(pack2<kF16>(z[0], z[1]), pack2<kF16>(z[2], z[3]));
         }
-        const int64_t pi = prefix_part(a, row, it.part, hq);
-        if (j == 0) {
-            a.d.part_m[pi] = m[qt];
-            a.d.part_l[pi] = lt;
-        }
+        // The row's two lanes run in step: both have read lse.
+        if (hi == 0) a.lse[at] = (mu + __builtin_log2f(den)) * kLn2;
+        return;
+    }
+    const int64_t pi = prefix_part(a, row, it.part, hq);
+    if (hi == 0) {
+        a.d.part_m[pi] = m;
+        a.d.part_l[pi] = lt;
+    }
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-            *reinterpret_cast<float4*>(a.d.part_acc + pi * kD + 16 * nb + 4 * j) =
-                make_float4(o[qt][nb][0], o[qt][nb][1], o[qt][nb][2], o[qt][nb][3]);
+    for (int d = 0; d < kD; d += 8) {
+        const int i = d % 32 / 2;
+        *reinterpret_cast<float4*>(a.d.part_acc + pi * kD + d + 4 * hi) = make_float4(o[d / 32][i], o[d / 32][i + 1], o[d / 32][i + 2], o[d / 32][i + 3]);
     }
 }
 
