@@ -84,6 +84,7 @@ struct PrefixMfmaPlan {
     int32_t blocks;                   // row blocks, at most
     int32_t splits, step_shift;       // of a prefix
     int32_t own_groups, own_heads, own_blocks, own_splits;        // decode form, as in PrefixGrid
+    int32_t per_xcd, tail_from, tail_splits;                      // as in PrefixGrid
     int64_t states;                   // float32 states: m at 0, l and acc at these byte offsets
     int64_t part_l, part_acc, bytes;
 };
@@ -95,7 +96,8 @@ struct PrefixGrid {
     int32_t blocks;                   // row blocks, at most
     int32_t total;                    // items of the prefixes: blocks x KV heads x splits
     int32_t per_xcd;                  // total / 8, rounded up
-    int32_t prefix_groups;            // workgroups of the prefixes, 8 per_xcd
+    int32_t tail_from, tail_splits;   // an XCD's items from this one on are split (prompt form, else none: per_xcd, 1)
+    int32_t prefix_groups;            // workgroups of the prefixes: 8 (tail_from + (per_xcd - tail_from) tail_splits)
     int32_t own_groups;               // workgroups of the own tokens
     int32_t own_heads;                // KV heads of one of them
     int32_t own_blocks;               // blocks of 16 q heads of a KV head

@@ -15,6 +15,7 @@ constexpr int kXcds = 8;              // workgroups are dispatched round-robin o
 struct PrefixItem {
     int32_t h;                        // (first) KV head
     int32_t part;                     // where the states go
+    int32_t tail;                     // number of the row block among those split at the end, else -1
     int32_t rs;                       // first q row of the group
     int32_t pairs;                    // its pairs
     int32_t r0;                       // first pair of the block
@@ -32,16 +33,16 @@ __device__ __forceinline__ int32_t group_row(const PrefixArgs& a, int i) {
     return (int32_t)(row < 0 ? 0 : (row > a.rows ? a.rows : row));
 }
 
-// The item of this workgroup, false without one (rows, pairs and tokens are int32, checked on the host).
-// Each XCD takes one run of (split, KV head, row block), so that the blocks of one head and split meet their
-// tokens in the same L2. A wave looks through 64 groups at once, every value of a group in its lane.
-__device__ __forceinline__ bool prefix_item(const PrefixArgs& a, const PrefixGrid& grid, int rows_per_block, PrefixItem& it) {
-    const int32_t local = (int32_t)(blockIdx.x / kXcds);
-    const int32_t index = (int32_t)(blockIdx.x % kXcds) * grid.per_xcd + local;
-    if (index >= grid.total || local >= grid.per_xcd) return false;
+// Item `index` of the prefixes with the tokens of one of its `parts` (part -1: of none); false without one (rows,
+// pairs and tokens are int32, checked on the host). A wave looks through 64 groups at once, every value of a group in
+// its lane.
+__device__ __forceinline__ bool find_item(const PrefixArgs& a, const PrefixGrid& grid, int rows_per_block, int32_t index,
+                                          int32_t tail_part, PrefixItem& it, int32_t* tokens_out) {
     const int32_t unit = (uint32_t)index / (uint32_t)grid.blocks;
-    it.part = (uint32_t)unit / (uint32_t)a.d.num_kv_heads;
-    it.h = unit - it.part * a.d.num_kv_heads;
+    const int32_t split = (uint32_t)unit / (uint32_t)a.d.num_kv_heads;
+    const int32_t splits = it.tail < 0 ? a.splits : grid.tail_splits;
+    it.part = it.tail < 0 ? split : tail_part;
+    it.h = unit - split * a.d.num_kv_heads;
     const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
     int32_t left = index - unit * grid.blocks;
     const int lane = threadIdx.x & 63;
@@ -67,7 +68,8 @@ __device__ __forceinline__ bool prefix_item(const PrefixArgs& a, const PrefixGri
             it.pairs = __builtin_amdgcn_readlane(pairs, at);
             it.r0 = (left - __builtin_amdgcn_readlane(incl - blocks, at)) * rows_per_block;
             const int32_t n = __builtin_amdgcn_readlane(tokens, at);
-            const int64_t per = split_tokens(n, a.step_shift, a.splits);
+            if (tokens_out != nullptr) *tokens_out = n;
+            const int64_t per = split_tokens(n, a.step_shift, splits);
             const int64_t lo = it.part * per;
             if (lo >= n) return false;
             it.lo = uniform((int32_t)lo);
@@ -79,6 +81,23 @@ __device__ __forceinline__ bool prefix_item(const PrefixArgs& a, const PrefixGri
         left -= __builtin_amdgcn_readlane(incl, 63);
     }
     return false;
+}
+
+// The item of this workgroup. Each XCD takes one run of (split, KV head, row block), so that the blocks of one head
+// and split meet their tokens in the same L2; those of a run that would leave CUs idle at its end are split.
+__device__ __forceinline__ bool prefix_item(const PrefixArgs& a, const PrefixGrid& grid, int rows_per_block, PrefixItem& it) {
+    const int32_t xcd = (int32_t)(blockIdx.x % kXcds);
+    int32_t local = (int32_t)(blockIdx.x / kXcds), part = 0;
+    it.tail = -1;
+    if (local >= grid.tail_from) {
+        const int32_t x = local - grid.tail_from, at = (uint32_t)x / (uint32_t)grid.tail_splits;
+        part = x - at * grid.tail_splits;
+        local = grid.tail_from + at;
+        it.tail = xcd * (grid.per_xcd - grid.tail_from) + at;
+    }
+    const int32_t index = xcd * grid.per_xcd + local;
+    if (index >= grid.total || local >= grid.per_xcd) return false;
+    return find_item(a, grid, rows_per_block, index, part, it, nullptr);
 }
 
 // Own tokens: block of 16 q heads, KV heads and split of a sequence. Neighbouring workgroups take the heads of the

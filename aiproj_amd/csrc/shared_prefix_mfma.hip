@@ -40,6 +40,46 @@ __device__ __forceinline__ void store_run(typename Elem<QT>::T* dst, const float
     }
 }
 
+// Four columns of a softmax state in the making.
+struct JoinedState {
+    float mr = kNegInf, den = 0.0f;
+    float4 num = {0.0f, 0.0f, 0.0f, 0.0f};
+
+    __device__ __forceinline__ void add(float mi, float li, float4 x) {
+        const float mn = fmaxf(mr, mi);
+        const float mu = mn == kNegInf ? 0.0f : mn;
+        const float wa = fast_exp2(mr - mu), wb = fast_exp2(mi - mu);
+        num.x = num.x * wa + x.x * wb;
+        num.y = num.y * wa + x.y * wb;
+        num.z = num.z * wa + x.z * wb;
+        num.w = num.w * wa + x.w * wb;
+        den = den * wa + li * wb;
+        mr = mn;
+    }
+    // The states of the lanes kLanes apart.
+    template <int kLanes>
+    __device__ __forceinline__ void across() {
+#pragma unroll
+        for (int off = kLanes; off < 64; off <<= 1)
+            add(__shfl_xor(mr, off), __shfl_xor(den, off),
+                make_float4(__shfl_xor(num.x, off), __shfl_xor(num.y, off), __shfl_xor(num.z, off), __shfl_xor(num.w, off)));
+    }
+    // The row's attention over its prompt, out and *lse; *lse becomes that of both.
+    template <int QT>
+    __device__ __forceinline__ void with_prompt(const typename Elem<QT>::T* out, float* lse, int lane) {
+        add(*lse * kLog2e, 1.0f,
+            make_float4(Elem<QT>::load(out[0]), Elem<QT>::load(out[1]), Elem<QT>::load(out[2]), Elem<QT>::load(out[3])));
+        __builtin_amdgcn_wave_barrier();                 // every lane has read lse before lane 0 writes it
+        if (lane == 0) *lse = ((mr == kNegInf ? 0.0f : mr) + __builtin_log2f(den)) * kLn2;
+    }
+    template <int QT>
+    __device__ __forceinline__ void store(typename Elem<QT>::T* out) const {
+        const bool ok = den > 0.0f || den != den;
+        const float y[4] = {ok ? num.x / den : 0.0f, ok ? num.y / den : 0.0f, ok ? num.z / den : 0.0f, ok ? num.w / den : 0.0f};
+        store_run<QT, 4>(out, y);
+    }
+};
+
 // One wave per (row, q head) joins the states of its prefix and own tokens, in the prompt form with out and lse
 // in place of the latter. Lanes take 16 C float4 columns; 4 / C states are read side by side.
 template <int C, int QT, bool kOwn>
@@ -65,40 +105,62 @@ prefix_join_kernel(PrefixArgs a) {
     const int held_own = kOwn ? split_count(mine, split_tokens(mine, 5, a.own_splits)) : 0;
     const int d4 = min(lane % kLanes, D / 4 - 1), po = lane / kLanes;
 
-    float mr = kNegInf, den = 0.0f;
-    float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    auto add = [&](float mi, float li, float4 x) __attribute__((always_inline)) {
-        const float mn = fmaxf(mr, mi);
-        const float mu = mn == kNegInf ? 0.0f : mn;
-        const float wa = fast_exp2(mr - mu), wb = fast_exp2(mi - mu);
-        num.x = num.x * wa + x.x * wb;
-        num.y = num.y * wa + x.y * wb;
-        num.z = num.z * wa + x.z * wb;
-        num.w = num.w * wa + x.w * wb;
-        den = den * wa + li * wb;
-        mr = mn;
-    };
+    JoinedState st;
 #pragma unroll 4
     for (int i = po; i < held + held_own; i += kPass) {
         const int64_t pi = prefix_part(a, row, i < held ? i : a.splits + i - held, hq);
-        add(a.d.part_m[pi], a.d.part_l[pi], reinterpret_cast<const float4*>(a.d.part_acc + pi * D)[d4]);
+        st.add(a.d.part_m[pi], a.d.part_l[pi], reinterpret_cast<const float4*>(a.d.part_acc + pi * D)[d4]);
     }
-#pragma unroll
-    for (int off = kLanes; off < 64; off <<= 1)
-        add(__shfl_xor(mr, off), __shfl_xor(den, off),
-            make_float4(__shfl_xor(num.x, off), __shfl_xor(num.y, off), __shfl_xor(num.z, off), __shfl_xor(num.w, off)));
+    st.across<kLanes>();
     if (po != 0 || 4 * (lane % kLanes) >= D) return;
     const int64_t at = unit;
     T* out = reinterpret_cast<T*>(a.d.out) + at * D + 4 * d4;
-    if constexpr (!kOwn) {
-        add(a.lse[at] * kLog2e, 1.0f,
-            make_float4(Elem<QT>::load(out[0]), Elem<QT>::load(out[1]), Elem<QT>::load(out[2]), Elem<QT>::load(out[3])));
-        __builtin_amdgcn_wave_barrier();                 // every lane has read lse before lane 0 writes it
-        if (lane == 0) a.lse[at] = ((mr == kNegInf ? 0.0f : mr) + __builtin_log2f(den)) * kLn2;
+    if constexpr (!kOwn) st.with_prompt<QT>(out, a.lse + at, lane);
+    st.store<QT>(out);
+}
+
+// Prompt form: the states of the row blocks that were split at the end, with out and lse. One wave per four
+// pairs (often of one row: one search for its sequence).
+template <int C, int QT>
+__global__ void __launch_bounds__(256)
+prefix_tail_kernel(PrefixArgs a, PrefixGrid grid, int rows_per_block) {
+    constexpr int kLanes = 16 * C, kPass = 64 / kLanes;
+    using T = typename Elem<QT>::T;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int D = a.d.head_dim;
+    const uint32_t per_block = (uint32_t)rows_per_block / 16;
+    const int32_t tails = grid.per_xcd - grid.tail_from;
+    PrefixItem it;
+    it.tail = blockIdx.x / per_block;
+    const int32_t first_pair = 16 * (int32_t)(blockIdx.x - it.tail * per_block) + 4 * wave;
+    const int32_t xcd = (uint32_t)it.tail / (uint32_t)tails, index = xcd * grid.per_xcd + grid.tail_from + (it.tail - xcd * tails);
+    int32_t tokens;
+    if (index >= grid.total || !find_item(a, grid, rows_per_block, index, 0, it, &tokens)) return;
+    const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
+    const int held = split_count(tokens, split_tokens(tokens, a.step_shift, grid.tail_splits));
+    const int d4 = min(lane % kLanes, D / 4 - 1), po = lane / kLanes;
+    int32_t last = -1;
+    bool inside = false;
+    for (int p = 0; p < 4; ++p) {
+        const int32_t pair = it.r0 + first_pair + p;
+        if (pair >= it.pairs) return;
+        const int32_t t = (uint32_t)pair / (uint32_t)G;
+        const int64_t row = it.rs + t;
+        if (t != last) inside = seq_of_row(a, row) >= 0;
+        last = t;
+        if (!inside) continue;
+        JoinedState st;
+        const int64_t first = ((int64_t)it.tail * rows_per_block + first_pair + p) * grid.tail_splits;
+#pragma unroll 4
+        for (int i = po; i < held; i += kPass)
+            st.add(a.d.part_m[first + i], a.d.part_l[first + i], reinterpret_cast<const float4*>(a.d.part_acc + (first + i) * D)[d4]);
+        st.across<kLanes>();
+        if (po != 0 || 4 * (lane % kLanes) >= D) continue;
+        const int64_t at = row * a.d.num_q_heads + it.h * G + (pair - t * G);
+        T* out = reinterpret_cast<T*>(a.d.out) + at * D + 4 * d4;
+        st.with_prompt<QT>(out, a.lse + at, lane);
+        st.store<QT>(out);
     }
-    const bool ok = den > 0.0f || den != den;
-    const float y[4] = {ok ? num.x / den : 0.0f, ok ? num.y / den : 0.0f, ok ? num.z / den : 0.0f, ok ? num.w / den : 0.0f};
-    store_run<QT, 4>(out, y);
 }
 
 // ------------------------------------------------------------------ host
@@ -171,7 +233,26 @@ PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_k
     int64_t splits = columns > 0 ? (left + columns / 2) / columns : 1;
     splits = splits < most ? splits : most;
     p.splits = (int32_t)(splits < 1 ? 1 : splits);
-    p.states = prompt && p.splits == 1 && p.rows > 16 ? 0 : rows * num_q_heads * (p.splits + (prompt ? 0 : p.own_splits));
+    // Prompt form, more row blocks than run at once: an XCD's last ones, which would leave CUs idle, are split into as
+    // many parts as end soonest (a part costs its states, about 1/50 of a round).
+    p.per_xcd = (int32_t)((columns * p.splits + kXcds - 1) / kXcds);
+    p.tail_from = p.per_xcd;
+    p.tail_splits = 1;
+    const bool in_place = prompt && p.splits == 1 && p.rows > 16;
+    const int64_t at_once = slots / kXcds;
+    if (in_place && at_once > 0 && p.per_xcd > at_once) {
+        const int64_t tail = p.per_xcd % at_once;
+        float best = 1.0f;
+        for (int parts = 2; tail > 0 && parts <= 8 && parts <= most; ++parts) {
+            const float cost = (float)((tail * parts + at_once - 1) / at_once) / parts + 0.02f * parts;
+            if (cost < best) {
+                best = cost;
+                p.tail_from = (int32_t)(p.per_xcd - tail);
+                p.tail_splits = parts;
+            }
+        }
+    }
+    p.states = in_place ? (int64_t)kXcds * (p.per_xcd - p.tail_from) * p.rows * p.tail_splits : rows * num_q_heads * (p.splits + (prompt ? 0 : p.own_splits));
     p.part_l = (int64_t)align256((size_t)p.states * 4);
     p.part_acc = 2 * p.part_l;
     p.bytes = p.part_acc + (int64_t)align256((size_t)p.states * head_dim * 4);
@@ -191,8 +272,10 @@ hipError_t launch_prefix_mfma(PrefixArgs a, int kv_dtype, const PrefixMfmaPlan& 
     const int64_t total = (int64_t)p.blocks * a.d.num_kv_heads * p.splits;
     g.blocks = p.blocks;
     g.total = (int32_t)total;
-    g.per_xcd = (int32_t)((total + kXcds - 1) / kXcds);
-    g.prefix_groups = kXcds * g.per_xcd;
+    g.per_xcd = p.per_xcd;
+    g.tail_from = p.tail_from;
+    g.tail_splits = p.tail_splits;
+    g.prefix_groups = kXcds * (p.tail_from + (p.per_xcd - p.tail_from) * p.tail_splits);
     g.own_groups = p.own_groups;
     g.own_heads = p.own_heads;
     g.own_blocks = p.own_blocks;
@@ -205,7 +288,14 @@ hipError_t launch_prefix_mfma(PrefixArgs a, int kv_dtype, const PrefixMfmaPlan& 
         if (err != hipSuccess) return err;
     }
     if (a.cu == nullptr) return launch_join<QT, true>(a, s);
-    return p.states == 0 ? hipSuccess : launch_join<QT, false>(a, s);
+    if (p.states == 0) return hipSuccess;
+    if (p.tail_splits > 1) {
+        const dim3 grid((unsigned)(kXcds * (p.per_xcd - p.tail_from)) * (unsigned)(p.rows / 16));
+        if (a.d.head_dim == 64) hipLaunchKernelGGL((prefix_tail_kernel<1, QT>), grid, dim3(256), 0, s, a, g, p.rows);
+        else hipLaunchKernelGGL((prefix_tail_kernel<2, QT>), grid, dim3(256), 0, s, a, g, p.rows);
+        return hipGetLastError();
+    }
+    return launch_join<QT, false>(a, s);
 }
 
 template hipError_t launch_prefix_mfma<KVFP8_F32>(PrefixArgs, int, const PrefixMfmaPlan&, void*, hipStream_t);

@@ -486,7 +486,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
     const int64_t row = it.rs + t;
     const int hq = h * G + (pair - t * G);
     // Element 4 q + i of block nb: dim 32 nb + 8 q + 4 hi + i of the row.
-    if (a.cu != nullptr && a.splits == 1) {
+    if (a.cu != nullptr && a.splits == 1 && it.tail < 0) {
         // The prompt form's only state of the row: joined with out and lse at once.
         if (seq_of_row(a, row) < 0) return;
         const int64_t at = row * a.d.num_q_heads + hq;
@@ -511,7 +511,8 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
         if (hi == 0) a.lse[at] = (mu + __builtin_log2f(den)) * kLn2;
         return;
     }
-    const int64_t pi = prefix_part(a, row, it.part, hq);
+    const int64_t pi = it.tail < 0 ? prefix_part(a, row, it.part, hq)
+                                   : ((int64_t)it.tail * (32 * NW) + (pair - it.r0)) * grid.tail_splits + it.part;
     if (hi == 0) {
         a.d.part_m[pi] = m;
         a.d.part_l[pi] = lt;

@@ -275,6 +275,32 @@ def test_prompts_against_float64(form, name):
     _check_prompt(c, *_run_prompt(c))
 
 
+# More row blocks than the card runs at once (KV heads x rows above 512 workgroups, for blocks of 256 and of 128 rows), so
+# that the last ones are split: one group, uneven groups with an empty and a short prefix, blocks of 128.
+SPLIT_ENDS = {
+    "one": ([300, 1, 250, 549], [700], [4], 0),
+    "uneven": ([100, 400, 7, 300, 0, 290], [530, 0, 20, 300], [2, 1, 1, 1], 1),
+    "halves": ([100 - (i % 3) for i in range(8)], [64 * (i + 1) + i for i in range(8)], [1] * 8, 0),
+}
+
+
+@pytest.mark.parametrize("q_dtype", [BF16, F16])
+@pytest.mark.parametrize("name", SPLIT_ENDS)
+def test_prompts_whose_last_blocks_are_split(name, q_dtype, monkeypatch):
+    monkeypatch.setitem(PROMPTS, name, SPLIT_ENDS[name])
+    c = _prompt((64, 64, 64, q_dtype, FP8, 16), name)
+    out, lse = _run_prompt(c)
+    _check_prompt(c, out, lse)
+    again, lse_again = _run_prompt(c)
+    assert t.equal(out, again) and t.equal(lse, lse_again)
+    longest = 120
+    out, lse = _run_prompt(c, longest)
+    inside = t.zeros(len(c.q), dtype=t.bool)
+    for a, b in zip(c.bounds, c.bounds[1:]):
+        inside[a:min(b, a + longest)] = True
+    _check_prompt(c, out, lse, inside.to("cuda"))
+
+
 def test_rows_of_no_sequence_and_past_the_longest():
     """Rows behind the last sequence and rows past batch_max_seq_len of theirs hold what flash attention leaves there."""
     c = _prompt(FORMS[1], "groups")
