@@ -274,7 +274,8 @@ int shared_args(PrefixArgs& a, const void* q, int q_dtype, int64_t q_stride_t, i
     if (rows < 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || d <= 0 || num_blocks <= 0 || bt_rows <= 0 || bt_width <= 0 ||
         block_size <= 0 || (block_size & (block_size - 1)) != 0 || groups < 0)
         return KVFP8_ESHAPE;
-    if (d > kGenMaxD || rows > INT32_MAX || rows * hq > INT32_MAX || bt_width * block_size > INT32_MAX) return KVFP8_ELIMIT;
+    // The kernels' token numbers are int32 and run up to three blocks past the last.
+    if (d > kGenMaxD || rows > INT32_MAX || rows * hq > INT32_MAX || bt_width * block_size > INT32_MAX - 8192) return KVFP8_ELIMIT;
     if (rows == 0) return KVFP8_OK;
     if (!q || !k_cache || !v_cache || !block_table || !out || (groups > 0 && (!p_slots || !p_lens || !p_starts)))
         return KVFP8_ENULL;

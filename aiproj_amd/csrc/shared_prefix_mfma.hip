@@ -208,7 +208,10 @@ PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_k
                                 int64_t bt_width, int32_t block_size, int q_dtype, bool prompt) {
     PrefixMfmaPlan p = {};
     const int64_t cus = device_cus(), heads = num_q_heads / num_kv_heads;
-    const int64_t most = bt_width * block_size / 256 > 0 ? bt_width * block_size / 256 : 1;    // splits of 256 tokens or more
+    // Splits of 256 tokens or more, in the prompt form 128 (540 rows x 1000 tokens of head size 80: 17.9 us against 21.7;
+    // 32 x 4096 in the decode form, beside own tokens: 24.0 us against 19.8).
+    const int64_t least = prompt ? 128 : 256;
+    const int64_t most = bt_width * block_size / least > 0 ? bt_width * block_size / least : 1;
     const int64_t pairs = rows * heads, mean = groups > 0 ? pairs / groups : 0;
     p.rows = q_dtype == KVFP8_F32 || mean < kWidePairs[0] ? 16 : (mean < kWidePairs[1] ? 128 : 256);
     p.step_shift = p.rows == 16 ? 5 : 6;
