@@ -45,7 +45,7 @@ struct LogprobArgs {
     int32_t tokens64;
     float* logprobs;
     float* entropy;
-    float2* stats;                    // (m, ln S) of every row
+    float2* stats;                    // (m, ln S) of every row, or null
     float* top_logprobs;              // [rows, top]
     int64_t* top_tokens;
 };
@@ -259,7 +259,7 @@ token_logprobs_kernel(LogprobArgs a) {
     if (tid == 0) {
         a.logprobs[row] = !given ? 0.0f : (empty ? kNegInf : (chosen - st.m) - log_s);
         a.entropy[row] = empty ? 0.0f : log_s - st.t / st.s;
-        a.stats[row] = make_float2(st.m, log_s);
+        if (a.stats != nullptr) a.stats[row] = make_float2(st.m, log_s);
     }
     if (a.top == 0) return;
 
@@ -526,7 +526,7 @@ extern "C" int kvfp8_token_logprobs(const void* logits, int dtype, int64_t row_s
     if (top < 0 || top > vocab) return KVFP8_ESHAPE;
     if (top > kMaxTop) return KVFP8_ELIMIT;
     if (rows == 0) return KVFP8_OK;
-    if (!logits || !tokens || !logprobs || !entropy || !stats || (top > 0 && (!top_logprobs || !top_tokens)))
+    if (!logits || !tokens || !logprobs || !entropy || (top > 0 && (!top_logprobs || !top_tokens)))
         return KVFP8_ENULL;
     if (!aligned(logits, dtype) || (uintptr_t)stats % 8 != 0) return KVFP8_ESTRIDE;
     const LogprobArgs a = {logits, row_stride, 0, (int32_t)vocab, top, tokens, tok_dtype == KVFP8_I64,

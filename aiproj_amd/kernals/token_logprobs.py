@@ -57,22 +57,22 @@ def _check(logits: t.Tensor, tokens: t.Tensor, top: int) -> t.device:
     return _native.require_gpu(logits, tokens, what="token_logprobs")
 
 
-def _forward(logits: t.Tensor, tokens: t.Tensor, top: int):
-    """(logprobs, entropy, top_logprobs, top_tokens, stats [T, 2])."""
+def _forward(logits: t.Tensor, tokens: t.Tensor, top: int, for_backward: bool = False):
+    """(logprobs, entropy, top_logprobs, top_tokens, stats [T, 2] for the backward or None)."""
     device = _check(logits, tokens, top)
     rows, vocab = logits.shape
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     logprobs = t.empty(rows, dtype=t.float32, device=device)
     entropy = t.empty_like(logprobs)
-    stats = t.empty((rows, 2), dtype=t.float32, device=device)
+    stats = t.empty((rows, 2), dtype=t.float32, device=device) if for_backward else None
     top_logprobs = t.empty((rows, top), dtype=t.float32, device=device)
     top_tokens = t.empty((rows, top), dtype=t.int64, device=device)
     if rows:
         rc = _native.fn("kvfp8_token_logprobs")(
             logits.data_ptr(), _native.dtype_code(logits.dtype), logits.stride(0), rows, vocab,
             tokens.data_ptr(), _native.dtype_code(tokens.dtype), top, logprobs.data_ptr(), entropy.data_ptr(),
-            stats.data_ptr(), top_logprobs.data_ptr(), top_tokens.data_ptr(), _native.stream_handle(device))
+            _native.ptr(stats), top_logprobs.data_ptr(), top_tokens.data_ptr(), _native.stream_handle(device))
         _native.check(rc, "kvfp8_token_logprobs")
     return logprobs, entropy, top_logprobs, top_tokens, stats
 
@@ -95,7 +95,7 @@ def _plain_backward(logits, tokens, entropy, stats, grad_logprobs, grad_entropy)
 class TokenLogprobsFunction(t.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top):
-        logprobs, entropy, top_logprobs, top_tokens, stats = _forward(logits, tokens, top)
+        logprobs, entropy, top_logprobs, top_tokens, stats = _forward(logits, tokens, top, True)
         ctx.mark_non_differentiable(top_logprobs, top_tokens)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, tokens, entropy, stats)

@@ -454,7 +454,7 @@ int kvfp8_shared_prefix_prefill(const void* q_dev, int q_dtype, int64_t rows, in
  *   top_logprobs, top_tokens [rows, top]: the largest logits, ties to the lowest index.
  * A row of -inf alone: log probabilities -inf, entropy 0. NaN or +inf in a row: NaN.
  * top 0..64, at most vocab (its outputs may be NULL when 0); vocab below 2^30.
- * stats: [rows, 2], 8-byte aligned. No reference counterpart (it samples the argmax,
+ * stats: [rows, 2], 8-byte aligned, or NULL. No reference counterpart (it samples the argmax,
  * reference src/torch_llm/inference/sampling.py).
  */
 int kvfp8_token_logprobs(const void* logits_dev, int dtype, int64_t row_stride, int64_t rows, int64_t vocab,
