@@ -80,7 +80,7 @@ __device__ __forceinline__ int64_t prefix_part(const PrefixArgs& a, int64_t row,
 bool prefix_mfma_supported(int32_t head_dim, int32_t block_size, int q_dtype, int kv_dtype);
 
 struct PrefixMfmaPlan {
-    int32_t rows;                     // pairs per row block: 16, 128 or 256
+    int32_t rows;                     // pairs per row block: 16 or 256
     int32_t blocks;                   // row blocks, at most
     int32_t splits, step_shift;       // of a prefix
     int32_t own_groups, own_heads, own_blocks, own_splits;        // decode form, as in PrefixGrid
@@ -105,7 +105,7 @@ struct PrefixGrid {
 };
 
 template <int QT>
-hipError_t launch_prefix_wide(const PrefixArgs& a, int kv_dtype, int rows, const PrefixGrid& g, hipStream_t s);
+hipError_t launch_prefix_wide(const PrefixArgs& a, int kv_dtype, const PrefixGrid& g, hipStream_t s);
 
 template <int QT>
 hipError_t launch_prefix_mfma(PrefixArgs a, int kv_dtype, const PrefixMfmaPlan& p, void* workspace, hipStream_t s);

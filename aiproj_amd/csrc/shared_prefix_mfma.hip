@@ -2,7 +2,7 @@
 //
 // A call is two launches. The first leaves softmax states: its first workgroups take the prefixes, (row block,
 // KV head, split of the prefix) each, the others the sequences' own tokens, (sequence, block of 16 q heads, KV
-// heads, split) each. Groups of many rows take blocks of 128 or 256 rows (shared_prefix_wide.hip), others
+// heads, split) each. Groups of many rows take blocks of 256 rows (shared_prefix_wide.hip), others
 // blocks of 16 (shared_prefix_narrow.h). The second launch joins a row's states.
 #include "shared_prefix_narrow.h"
 
@@ -191,8 +191,13 @@ hipError_t launch_join(const PrefixArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Pairs of an average group from which blocks of 128 and 256 rows are taken.
-constexpr int64_t kWidePairs[2] = {64, 192};
+// Pairs of an average group from which blocks of 256 rows are taken, and in block tables that address no more than
+// kShortTable tokens. Whole calls of 32 q and 8 KV heads x 128, blocks of 16 against 256 rows, us:
+//   pairs x tokens    48 x 1024  14.5  16.4    128 x 1024  16.6  19.7    256 x 1024  19.8  25.0    512 x 1024  29.2  29.1
+//                     48 x 4096  16.8  18.3     64 x 4096  20.1  19.0    128 x 4096  26.9  23.6    256 x 4096  39.1  32.2
+//                     48 x 16384 30.5  32.0     64 x 16384 42.3  35.0    128 x 16384 68.1  37.9    256 x 16384  117  51.5
+// Blocks of 128 rows lay between the two or behind both (64 x 4096 21.3, 128 x 4096 26.1, 128 x 16384 40.5).
+constexpr int64_t kWidePairs = 64, kWidePairsShort = 512, kShortTable = 2048;
 
 bool narrow_size(int32_t d) { return d == 80 || d == 96 || d == 112; }
 
@@ -213,7 +218,7 @@ PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_k
     const int64_t least = prompt ? 128 : 256;
     const int64_t most = bt_width * block_size / least > 0 ? bt_width * block_size / least : 1;
     const int64_t pairs = rows * heads, mean = groups > 0 ? pairs / groups : 0;
-    p.rows = q_dtype == KVFP8_F32 || mean < kWidePairs[0] ? 16 : (mean < kWidePairs[1] ? 128 : 256);
+    p.rows = q_dtype == KVFP8_F32 || mean < (bt_width * block_size <= kShortTable ? kWidePairsShort : kWidePairs) ? 16 : 256;
     p.step_shift = p.rows == 16 ? 5 : 6;
     // Own tokens: 16 q heads of `own_heads` KV heads a workgroup, one wave or more a head; about half as many
     // workgroups as CUs, up to which the waves of a workgroup serve one head and long contexts are split.
@@ -222,8 +227,7 @@ PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_k
     if (!prompt) {
         p.own_blocks = (int32_t)((heads + 15) / 16);
         const int64_t items = rows * p.own_blocks * num_kv_heads;
-        const int waves = p.rows == 128 ? 4 : 8;
-        while (p.own_heads < waves && num_kv_heads % (2 * p.own_heads) == 0 && items / (2 * p.own_heads) >= cus / 2) p.own_heads *= 2;
+        while (p.own_heads < kWaves && num_kv_heads % (2 * p.own_heads) == 0 && items / (2 * p.own_heads) >= cus / 2) p.own_heads *= 2;
         const int64_t wanted = cus / 2 / (items / p.own_heads);
         p.own_splits = (int32_t)(wanted < 1 ? 1 : (wanted < most ? wanted : most));
         p.own_groups = (int32_t)(items / p.own_heads * p.own_splits);
@@ -231,8 +235,7 @@ PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_k
     // Prefixes: the workgroups that are left of one per CU; with more own tokens than fit beside them, all.
     p.blocks = (int32_t)((pairs + (int64_t)groups * (p.rows - 1)) / p.rows);                    // every group's last block may be unfilled
     const int64_t columns = (int64_t)p.blocks * num_kv_heads;
-    const int64_t slots = (p.rows == 128 ? 2 : 1) * cus;
-    const int64_t left = p.own_groups <= slots / 2 ? slots - p.own_groups : slots;
+    const int64_t left = p.own_groups <= cus / 2 ? cus - p.own_groups : cus;
     int64_t splits = columns > 0 ? (left + columns / 2) / columns : 1;
     splits = splits < most ? splits : most;
     p.splits = (int32_t)(splits < 1 ? 1 : splits);
@@ -242,7 +245,7 @@ PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_k
     p.tail_from = p.per_xcd;
     p.tail_splits = 1;
     const bool in_place = prompt && p.splits == 1 && p.rows > 16;
-    const int64_t at_once = slots / kXcds;
+    const int64_t at_once = cus / kXcds;
     if (in_place && at_once > 0 && p.per_xcd > at_once) {
         const int64_t tail = p.per_xcd % at_once;
         float best = 1.0f;
@@ -287,7 +290,7 @@ hipError_t launch_prefix_mfma(PrefixArgs a, int kv_dtype, const PrefixMfmaPlan& 
     if (g.prefix_groups + g.own_groups > 0) {
         hipError_t err;
         if constexpr (QT == KVFP8_F32) err = launch_narrow_kv<QT>(a, kv_dtype, g, s);
-        else err = p.rows > 16 ? launch_prefix_wide<QT>(a, kv_dtype, p.rows, g, s) : launch_narrow_kv<QT>(a, kv_dtype, g, s);
+        else err = p.rows > 16 ? launch_prefix_wide<QT>(a, kv_dtype, g, s) : launch_narrow_kv<QT>(a, kv_dtype, g, s);
         if (err != hipSuccess) return err;
     }
     if (a.cu == nullptr) return launch_join<QT, true>(a, s);

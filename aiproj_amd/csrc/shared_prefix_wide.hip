@@ -1,26 +1,33 @@
-// Shared prefixes for many rows: blocks of 256 or 128 (row, q head) pairs against a prefix, gfx950.
+// Shared prefixes for many rows: blocks of 256 (row, q head) pairs against a prefix, gfx950.
 //
-// A workgroup takes one (row block, KV head, split of the prefix). Its eight or four waves hold 32 rows each and
-// share the prefix's tokens through LDS in blocks of 64: the codes are widened to 16 bits once per
-// workgroup on their way there (exact), instead of once per wave, and the tokens' bytes cross L2 once per
-// 256 rows. Per block and wave (MFMA 16x16x32, layouts in mfma_tiles.h):
+// A workgroup takes one (row block, KV head, split of the prefix). Its eight waves hold 32 rows each and share the
+// prefix's tokens through LDS in blocks of 64: the codes are widened to 16 bits once per workgroup on their way
+// there (exact), instead of once per wave, and the tokens' bytes cross L2 once per 256 rows. A wave takes a block in
+// two halves of 32 tokens (MFMA 32x32x16: A[row = l % 32][k = 8 (l / 32) + i], B likewise, D[row = 8 (i / 4) + 4 (l / 32)
+// + i % 4][col = l % 32]):
 //   S^T[token, row] = K Q^T     A = K rows from LDS, B = Q^T from registers
-//   softmax                     scores x k_scale[token] x sm_scale x log2(e) in float32, online, base 2; the
-//                               reference follows a row's maximum only where that exceeds it by 2^8
-//   O^T[d, row] += V^T P'^T     P' = p v_scale[token] from the score registers; A = V^T by transposing LDS reads
-// The vector ALU bounds it: nine operations a score, one of them the exponential at a quarter rate.
+//   softmax                     t = fma(score, k_scale[token] x sm_scale x log2(e), -reference), float32, online, base 2;
+//                               the reference follows a row's maximum only where that exceeds it by 2^8
+//   O^T[d, row] += V^T P'^T     P' = e2(t) v_scale[token] from the score registers; A = V^T by transposing LDS reads
 //
-// LDS rows are 16-byte chunks at position chunk ^ (row % chunks per row), so that the 16 rows of an operand
-// read lie in different bank groups.
+// One stretch of code without a branch holds, for half s, the products of the scores of half s + 1, the weights of half
+// s and the products with V of half s - 1, which are independent of each other; scheduling groups spread the products
+// over the vector operations and start the LDS reads ahead. The staging of later blocks lies in the stretch of a block's
+// first half, a barrier behind it:
+//   first half of g     scores K(g) second half, V(g - 1) second half;  V(g) and K(g + 1) to LDS, loads of V(g + 1), K(g + 2)
+//   second half of g    scores K(g + 1) first half, V(g) first half
+// so two buffers of each do: K(g + 1) replaces K(g - 1) and V(g) replaces V(g - 2), both last read before the barrier of
+// block g - 1. Scales and counts, of which a wave that lags may still read those of g - 1, have four buffers.
 //
-// The two halves of the waves alternate between a phase on the matrix cores (PV of block g - 1, QK of
-// block g) and one on the vector ALU (softmax of block g), half a step apart, with a barrier after each phase:
-//   phase 2 g       waves 0..3: PV(g - 1), QK(g)    waves 4..7: softmax(g - 1)
-//   phase 2 g + 1   waves 0..3: softmax(g)          waves 4..7: PV(g - 1), QK(g)
-// so K(g) and V(g - 1) are read in phases 2 g and 2 g + 1. In its matrix phase of step g a wave moves its part of
-// K(g + 1) and V(g) from registers to the buffers that K(g - 1) and V(g - 2) have left, and issues the loads of
-// K(g + 2) and V(g + 1). Scales and counts (softmax(g) of waves 4..7 reads them in phase 2 g + 2, when waves 0..3
-// write those of g + 2) have four buffers.
+// What bounds it (256 x 64 heads, 16384 tokens of 8 KV heads x 128, bf16 on e4m3fn: 157-175 us without the own tokens, 800-870
+// TFLOP/s): a block takes 5200 cycles of which the matrix cores work 2050 and the vector ALU 2300 (nine operations a score,
+// the exponential counts two), and one hides little of the other: next to 16x16x32 products vector operations of
+// another wave took 70% of their time on top, next to 32x32x16 ones 37% (both alone in a loop). LDS reads fill 1600 cycles
+// (256 bytes each), the widened writes 500. Measured on 9216 rows x 16 heads x 4096 tokens: two half-workgroups in turn on
+// products and softmax 480 us, this order with 16x16x32 products 463, with 32x32x16 445.
+//
+// LDS rows are 16-byte chunks in an order by row in which neither the 32 rows of a K read nor the 4 x 4 chunks of a
+// transposing read meet in a bank (4.4 and 3.7 cycles an instruction; chunk ^ (row % 16) 4.4 and, for these blocks, 7.9).
 #include "shared_prefix_narrow.h"
 
 namespace kvfp8 {
@@ -29,6 +36,7 @@ namespace {
 
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr int kKeys = 64;             // tokens per block
+constexpr int kWideWaves = 8;
 constexpr float kLag = 8.0f;          // log2 of how far a row's maximum may exceed its reference
 
 typedef __attribute__((address_space(3))) const uint8_t lds_u8;
@@ -75,16 +83,15 @@ struct WideLds {
     uint8_t spare[16 + 256];                             // what lanes without a value write
 };
 
-// NW waves, 32 rows each.
-template <int kD, int QT, int ES, int NW>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <int kD, int QT, int ES>
+__global__ void __launch_bounds__(64 * kWideWaves)
 prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
     static_assert(kD % 16 == 0 && kD >= 64 && kD <= 128 && (ES == 1 || kD % 64 == 0), "head sizes of this kernel");
     using T = typename Elem<QT>::T;
     constexpr bool kF16 = QT == KVFP8_F16;               // K and Q^T operands
     constexpr bool kF16V = kF16 && ES == 2;              // V^T and P operands; f16 q over codes: two bf16 parts of P
     constexpr int kParts = kF16 && ES == 1 ? 2 : 1;
-    constexpr int kThreads = 64 * NW;
+    constexpr int NW = kWideWaves, kThreads = 64 * NW;
     constexpr int ROW = WideLds<kD>::kRow;
     constexpr int CPR = ROW / 16;                        // 16-byte chunks of an LDS row
     constexpr int NB = (kD + 31) / 32, KS = kD / 16;     // blocks of 32 dims of O, steps of 16 dims of Q K^T
@@ -267,8 +274,9 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
     // Scores and P'^T operands of a block's halves of 32 tokens. Score i of a row: token 8 (i / 4) + 4 (l / 32) + i % 4.
     f32x16_t sacc[2];
     u32x4_t pop[2][kParts][2];
-    // Steps of K operands that are read before the products of a half, the others among them.
-    constexpr int kPre = KS / 2;
+    // Steps of K operands that are read before the products of a half, the others among them (weights of two parts leave
+    // no registers for that).
+    constexpr int kPre = kParts == 2 ? 0 : KS / 2;
     u32x4_t kop[KS];
     auto read_k = [&](auto buf_c, auto half_c, int first, int last) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value, half = decltype(half_c)::value;
@@ -525,28 +533,27 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
 }
 
 template <int kD, int QT, int ES>
-hipError_t launch_wide(const PrefixArgs& a, int rows, const PrefixGrid& g, hipStream_t s) {
+hipError_t launch_wide(const PrefixArgs& a, const PrefixGrid& g, hipStream_t s) {
     const dim3 grid((unsigned)(g.prefix_groups + g.own_groups));
-    if (rows == 256) hipLaunchKernelGGL((prefix_wide_kernel<kD, QT, ES, 8>), grid, dim3(512), 0, s, a, g);
-    else hipLaunchKernelGGL((prefix_wide_kernel<kD, QT, ES, 4>), grid, dim3(256), 0, s, a, g);
+    hipLaunchKernelGGL((prefix_wide_kernel<kD, QT, ES>), grid, dim3(64 * kWideWaves), 0, s, a, g);
     return hipGetLastError();
 }
 
 }  // namespace
 
 template <int QT>
-hipError_t launch_prefix_wide(const PrefixArgs& a, int kv_dtype, int rows, const PrefixGrid& g, hipStream_t s) {
-    if (kv_dtype != KVFP8_E4M3FN) return a.d.head_dim == 64 ? launch_wide<64, QT, 2>(a, rows, g, s) : launch_wide<128, QT, 2>(a, rows, g, s);
+hipError_t launch_prefix_wide(const PrefixArgs& a, int kv_dtype, const PrefixGrid& g, hipStream_t s) {
+    if (kv_dtype != KVFP8_E4M3FN) return a.d.head_dim == 64 ? launch_wide<64, QT, 2>(a, g, s) : launch_wide<128, QT, 2>(a, g, s);
     switch (a.d.head_dim) {
-        case 64: return launch_wide<64, QT, 1>(a, rows, g, s);
-        case 80: return launch_wide<80, QT, 1>(a, rows, g, s);
-        case 96: return launch_wide<96, QT, 1>(a, rows, g, s);
-        case 112: return launch_wide<112, QT, 1>(a, rows, g, s);
-        default: return launch_wide<128, QT, 1>(a, rows, g, s);
+        case 64: return launch_wide<64, QT, 1>(a, g, s);
+        case 80: return launch_wide<80, QT, 1>(a, g, s);
+        case 96: return launch_wide<96, QT, 1>(a, g, s);
+        case 112: return launch_wide<112, QT, 1>(a, g, s);
+        default: return launch_wide<128, QT, 1>(a, g, s);
     }
 }
 
-template hipError_t launch_prefix_wide<KVFP8_F16>(const PrefixArgs&, int, int, const PrefixGrid&, hipStream_t);
-template hipError_t launch_prefix_wide<KVFP8_BF16>(const PrefixArgs&, int, int, const PrefixGrid&, hipStream_t);
+template hipError_t launch_prefix_wide<KVFP8_F16>(const PrefixArgs&, int, const PrefixGrid&, hipStream_t);
+template hipError_t launch_prefix_wide<KVFP8_BF16>(const PrefixArgs&, int, const PrefixGrid&, hipStream_t);
 
 }  // namespace kvfp8
