@@ -7,8 +7,8 @@
 // and states of disjoint sets join exactly: M = max(m1, m2), l = l1 e^(m1 - M) + l2 e^(m2 - M), acc
 // likewise; the output is acc / l, 0 for a row without tokens. States are float32, scores base 2.
 //
-// The matrix-core kernels are in shared_prefix_mfma.hip. prefix_generic_kernel takes every cache, head size (up to 512) and page size: one wave per (row, q
-// head, split of the row's tokens), on the vector ALU.
+// The matrix-core kernels are in shared_prefix_mfma.hip. prefix_generic_kernel takes every cache, head size (up to 512)
+// and page size: one wave per (row, q head, split of the row's tokens), on the vector ALU.
 #include "shared_prefix.h"
 
 namespace kvfp8 {

@@ -81,7 +81,9 @@ struct JoinedState {
 };
 
 // One wave per (row, q head) joins the states of its prefix and own tokens, in the prompt form with out and lse
-// in place of the latter. Lanes take 16 C float4 columns; 4 / C states are read side by side.
+// in place of the latter. Lanes take 16 C float4 columns; 4 / C states are read side by side. Bound by the search for
+// the row's group and a chain of three loads where there are few rows (32 x 32 heads: 5.6 us, 16 + 1 states), by the
+// states' bytes where there are many (256 x 64 heads, 5 states: 16 us, 2.7 TB/s).
 template <int C, int QT, bool kOwn>
 __global__ void __launch_bounds__(256)
 prefix_join_kernel(PrefixArgs a) {
@@ -120,7 +122,8 @@ prefix_join_kernel(PrefixArgs a) {
 }
 
 // Prompt form: the states of the row blocks that were split at the end, with out and lse. One wave per four
-// pairs (often of one row: one search for its sequence).
+// pairs (often of one row: one search for its sequence). 64 blocks of 256 pairs in four parts, D 128: 16 us (20 with a
+// search for every pair).
 template <int C, int QT>
 __global__ void __launch_bounds__(256)
 prefix_tail_kernel(PrefixArgs a, PrefixGrid grid, int rows_per_block) {

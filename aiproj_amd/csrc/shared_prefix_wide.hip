@@ -80,7 +80,7 @@ struct WideLds {
     uint8_t v[2][kKeys * kRow];
     float scale[4][2][kKeys];
     int32_t count[4][4];                                 // tokens of each tile that count
-    uint8_t spare[16 + 256];                             // what lanes without a value write
+    __attribute__((aligned(16))) uint8_t spare[16 + 256];  // what lanes without a value write
 };
 
 template <int kD, int QT, int ES>

@@ -20,10 +20,10 @@
 //
 // Alternatives: with A waves that hold entries in all lanes, every wave finds the n-th largest of its 64 thread maxima,
 // n = ceil(top / A); the ceil(top / n)-th largest of these is a bound that at least `top` entries of the row reach,
-// and not many more. The entries that reach it are collected in LDS and ranked by counting. Where more reach it than the list holds (runs of equal logits, masked rows, sorted rows), the
-// bound is raised to the largest over the waves of the `top`-th thread maximum, only entries above it are
-// collected, and those equal to it follow by index. What still does not fit, and rows with NaN, are searched
-// entry by entry.
+// and not many more. The entries that reach it are collected in LDS and ranked by counting. Where more reach it than
+// the list holds (runs of equal logits, masked rows, sorted rows), the bound is raised to the largest over the waves of
+// the `top`-th thread maximum, only entries above it are collected, and those equal to it follow by index. What still
+// does not fit, and rows with NaN, are searched entry by entry.
 #include "mfma_tiles.h"
 
 namespace kvfp8 {
@@ -404,6 +404,9 @@ struct LogprobGradArgs {
     void* dx;                         // [rows, vocab] contiguous
 };
 
+// Bound by HBM: a piece of a row per workgroup, its logits read and the gradient written 16 bytes a lane, nothing
+// exchanged (the row's m, ln S and entropy come from the forward). 4096 x 32000 bf16: 84-90 us, 5.8-6.2 TB/s; 333 x 32000
+// float32: 15 us.
 constexpr int kGradThreads = 256;
 
 template <int DT>

@@ -71,6 +71,8 @@ class GreedyDecoder:
 
     def _prefill_prefix(self, prefix: t.Tensor | None):
         """The shared prefix [P] int64 into the cache, as request `batch`."""
+        if prefix is not None and prefix.ndim != 1:
+            raise ValueError("GreedyDecoder: a prefix is a vector of tokens")
         given = 0 if prefix is None else prefix.shape[0]
         if given > self.prefix_len:
             raise ValueError(f"GreedyDecoder: a prefix of {given} tokens, {self.prefix_len} are reserved")

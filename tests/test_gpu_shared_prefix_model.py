@@ -102,6 +102,8 @@ def test_refused_prefixes(model):
     decoder = GreedyDecoder(model, 2, 20, prefix_len=8)
     with pytest.raises(ValueError):
         decoder.prefill(_tokens(2, 3), _tokens(9))
+    with pytest.raises(ValueError):
+        decoder.prefill(_tokens(2, 3), _tokens(1, 4))
 
 
 @pytest.mark.parametrize("lengths", [[1], [1, 1, 1], [5, 1, 17, 2], [40, 33]])
