@@ -330,6 +330,8 @@ int run_generic(PrefixArgs& a, const PrefixPlan& p, int q_dtype, int kv_dtype, v
 // Whether a call runs on the matrix cores.
 bool mfma_shape(int64_t rows, int32_t hq, int32_t hkv, int32_t d, int32_t groups, int32_t bs, int q_dtype, int kv_dtype) {
     if (!prefix_mfma_supported(d, bs, q_dtype, kv_dtype)) return false;
+    // Byte offsets within 16 tokens are int32 (elements of 2 bytes at most).
+    if ((int64_t)hkv * d > (int64_t)1 << 25) return false;
     // Workgroups (at most a row block of 16 pairs and one of own tokens each, or some hundreds) are counted in int32,
     // and a launch has fewer than 2^32 threads.
     return rows * hq < ((int64_t)1 << 22) && (int64_t)groups * hkv < ((int64_t)1 << 21);

@@ -123,3 +123,24 @@ def test_workspace_size_depends_on_shapes_only():
         # A batch without groups, down to fewer pairs than a row block holds.
         assert fn(1, 2, 2, 64, 0, 64, 16, _native.E4M3FN, prompt) >= 0
     assert fn(0, 8, 2, 64, 1, 64, 16, _native.E4M3FN, 0) == 0
+
+
+def test_rows_past_int32_offsets_take_the_generic_kernel():
+    """2^19 KV heads of 128: a row of 16 tokens passes int32 offsets. The generic kernel keeps no states for so many
+    rows; the matrix-core kernels would."""
+    fn = _native.lib().kvfp8_shared_prefix_workspace_bytes
+    assert fn(1, 2 ** 19, 2 ** 19, 128, 1, 4, 16, _native.E4M3FN, 0) == 0
+    assert fn(1, 2 ** 18, 2 ** 18, 128, 1, 4, 16, _native.E4M3FN, 0) > 0
+
+
+def test_tables_up_to_the_end_of_int32_are_refused():
+    """The kernels look up to three blocks of tokens past the last one."""
+    lib, some = _native.lib(), 4096
+
+    def decode(width):
+        return lib.kvfp8_shared_prefix_decode(some, _native.BF16, 256, 64, 1, 4, 2, 64, some, some, _native.BF16, None, None, 8, 16,
+                                              some, 4, width, some, _native.I64, some, _native.I32, 0.1, some, None, 0, None,
+                                              some, _native.I64, some, _native.I64, some, _native.I64, 1)
+
+    assert decode(2 ** 27 - 512) == -6
+    assert decode(2 ** 27 - 513) == -5          # taken, but for its workspace
