@@ -223,14 +223,16 @@ PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_k
     const int64_t pairs = rows * heads, mean = groups > 0 ? pairs / groups : 0;
     p.rows = q_dtype == KVFP8_F32 || mean < (bt_width * block_size <= kShortTable ? kWidePairsShort : kWidePairs) ? 16 : 256;
     p.step_shift = p.rows == 16 ? 5 : 6;
-    // Own tokens: 16 q heads of `own_heads` KV heads a workgroup, one wave or more a head; about half as many
-    // workgroups as CUs, up to which the waves of a workgroup serve one head and long contexts are split.
+    // Own tokens: 16 q heads of `own_heads` KV heads a workgroup, one wave or more a head, so that no more than half of the
+    // CUs are taken where the heads allow it and the prefixes run beside them (24 x 8 KV heads behind 1024 tokens: 14.5 us
+    // a call with 96 workgroups, 19.6 with 192); below that the waves of a workgroup serve one head and long contexts
+    // are split.
     p.own_heads = 1;
     p.own_splits = 1;
     if (!prompt) {
         p.own_blocks = (int32_t)((heads + 15) / 16);
         const int64_t items = rows * p.own_blocks * num_kv_heads;
-        while (p.own_heads < kWaves && num_kv_heads % (2 * p.own_heads) == 0 && items / (2 * p.own_heads) >= cus / 2) p.own_heads *= 2;
+        while (p.own_heads < kWaves && num_kv_heads % (2 * p.own_heads) == 0 && items / p.own_heads > cus / 2) p.own_heads *= 2;
         const int64_t wanted = cus / 2 / (items / p.own_heads);
         p.own_splits = (int32_t)(wanted < 1 ? 1 : (wanted < most ? wanted : most));
         p.own_groups = (int32_t)(items / p.own_heads * p.own_splits);
