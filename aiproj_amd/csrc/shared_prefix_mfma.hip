@@ -216,13 +216,14 @@ PrefixMfmaPlan prefix_mfma_plan(int64_t rows, int32_t num_q_heads, int32_t num_k
                                 int64_t bt_width, int32_t block_size, int q_dtype, bool prompt) {
     PrefixMfmaPlan p = {};
     const int64_t cus = device_cus(), heads = num_q_heads / num_kv_heads;
-    // Splits of 256 tokens or more, in the prompt form 128 (540 rows x 1000 tokens of head size 80: 17.9 us against 21.7;
-    // 32 x 4096 in the decode form, beside own tokens: 24.0 us against 19.8).
-    const int64_t least = prompt ? 128 : 256;
-    const int64_t most = bt_width * block_size / least > 0 ? bt_width * block_size / least : 1;
     const int64_t pairs = rows * heads, mean = groups > 0 ? pairs / groups : 0;
     p.rows = q_dtype == KVFP8_F32 || mean < (bt_width * block_size <= kShortTable ? kWidePairsShort : kWidePairs) ? 16 : 256;
     p.step_shift = p.rows == 16 ? 5 : 6;
+    // Splits of 128 tokens or more: 540 rows x 1000 tokens of head size 80 in the prompt form 17.9 us against 21.7 with 256,
+    // blocks of 16 on 1024 tokens 12.4 against 14.1 (whole call). Blocks of 256 rows beside own tokens of 256: 128 pairs x
+    // 4096 tokens 19.8 us, with 128 24.0.
+    const int64_t least = prompt || p.rows == 16 ? 128 : 256;
+    const int64_t most = bt_width * block_size / least > 0 ? bt_width * block_size / least : 1;
     // Own tokens: 16 q heads of `own_heads` KV heads a workgroup, one wave or more a head, so that no more than half of the
     // CUs are taken where the heads allow it and the prefixes run beside them (24 x 8 KV heads behind 1024 tokens: 14.5 us
     // a call with 96 workgroups, 19.6 with 192); below that the waves of a workgroup serve one head and long contexts

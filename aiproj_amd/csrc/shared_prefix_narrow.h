@@ -12,7 +12,7 @@
 // its P' enters as two bf16 parts (an f16 P' would lose scales outside f16's range); float32 q and its P'
 // as three bf16 parts; bf16 and f16 caches with q of their type are operands as they are.
 // Bound by latency where there are few tokens (a step's loads wait for its pages, the first ones for the group's search:
-// 4 x 8 heads, 500 tokens: 6.7 us), by the widening and transposing of V's codes and the loads' latency where there are
+// 4 x 8 heads, 500 tokens: 6.1 us), by the widening and transposing of V's codes and the loads' latency where there are
 // many: own tokens of 256 sequences, 520 on average, 8 KV heads x 128: 82 us, 3.4 TB/s (decode without prefixes takes
 // 76 us for the same tokens). Page numbers read a step ahead and loads without a branch around them did not change that.
 #pragma once
