@@ -100,6 +100,53 @@ def test_pages_outside_the_pool_and_slots_outside_the_table(form):
     assert full
 
 
+# Groups of so many rows that blocks of 256 take them (tables of more than 2048 tokens).
+LARGE = [(8, 2, 64, BF16, FP8, 16), (32, 8, 128, BF16, FP8, 16), (16, 2, 128, F16, FP8, 32), (16, 2, 80, BF16, FP8, 16),
+         (16, 2, 112, F16, FP8, 16), (16, 4, 128, BF16, BF16, 16), (8, 2, 64, F16, F16, 64)]
+
+
+@pytest.mark.parametrize("form", LARGE)
+def test_large_groups_with_pages_outside_the_pool(form):
+    """Pages missing at the start, in the middle and at the end of a prefix, and a prefix of missing pages alone."""
+    hq, hkv, d, q_dtype, cache_dtype, page = form
+    c = cases.case([(3 * i) % 20 for i in range(90)], [2600, 700, 400], [40, 20, 30], hq, hkv, d, q_dtype, cache_dtype, page)
+    for at in (0, 7, 8, 20, 2600 // page - 1, 2600 // page):
+        c.table[c.prefix.slots[0], at] = -1 if at % 2 else c.cache.k.shape[0] + at
+    c.table[c.prefix.slots[2], :] = -1
+    _check_decode(c, shared_prefix_decode_attention(c.q, c.cache, c.ctx, c.prefix))
+    c.prefix.lengths[1] = 0
+    c.prefixes[1] = 0
+    _check_decode(c, shared_prefix_decode_attention(c.q, c.cache, c.ctx, c.prefix))
+
+
+@pytest.mark.parametrize("turn", ["rising", "falling", "waves"])
+@pytest.mark.parametrize("form", LARGE)
+def test_large_groups_whose_maxima_move(form, turn):
+    """Scores from -60 to 60 along the prefix, for half of the rows in the other direction, so that references move in many
+    blocks, in some rows of a wave at a time."""
+    hq, hkv, d, q_dtype, cache_dtype, page = form
+    n = 2600
+    c = cases.case([(3 * i) % 20 for i in range(50)], [n], [50], hq, hkv, d, q_dtype, cache_dtype, page)
+    gen = t.Generator(device="cpu").manual_seed(d)
+    u = t.nn.functional.normalize(t.randn(d, generator=gen), dim=0)
+    at = t.arange(n) / n
+    along = {"rising": 2 * at - 1, "falling": 1 - 2 * at, "waves": t.sin(40 * at)}[turn]
+    k = 8 * along[:, None, None] * u + 0.1 * t.randn(n, hkv, d, generator=gen)
+    v = t.randn(n, hkv, d, generator=gen)
+    pages = c.table[c.prefix.slots[0].long(), :-(-n // page)].long().cpu()
+    token = t.arange(n)
+    c.cache.append_kv(pages[token // page].cuda(), (token % page).cuda(), k.cuda(), v.cuda())
+    sign = t.where(t.rand(len(c.own), hq, 1, generator=gen) < 0.5, -1.0, 1.0)
+    c.q = (sign * u * 60 * math.sqrt(d) / 8 + 0.1 * t.randn(len(c.own), hq, d, generator=gen)).to(q_dtype).cuda()
+    got = shared_prefix_decode_attention(c.q, c.cache, c.ctx, c.prefix)
+    want, weight = cases.decode_64(c)
+    # A score is off by (D + 6) 2^-24 of sum |q k| scale, below 72 here (60 along u, under 6 from each noise; own tokens
+    # have about 54): the sum's D steps, the two scales, their product and the difference to a reference. Weights and
+    # their sum move by as much relatively.
+    bound = HALF[q_dtype] * want.abs() + (_weights_half(q_dtype, cache_dtype) + 2.0 ** -12 + 2 * (d + 6) * 2.0 ** -24 * 72) * weight
+    assert bool(((got.double() - want).abs() <= bound).all()), float(((got.double() - want).abs() - bound).max())
+
+
 @pytest.mark.parametrize("form", [FORMS[1], FORMS[9], FORMS[2], FORMS[7]])
 def test_lengths_past_the_table_are_clipped(form):
     hq, hkv, d, q_dtype, cache_dtype, page = form
