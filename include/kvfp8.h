@@ -408,7 +408,7 @@ int kvfp8_skinny_linear_rope(const void* x_dev, int dtype, int64_t x_stride, int
  * prefix_slots[g], read once for the whole group. Sequences of no group attend their own tokens
  * only. Own tokens, cache, block table and errors as kvfp8_paged_decode (slots and context_lengths
  * count own tokens). All index arrays int32/int64 on the device. head_dim 1..512, any batch with
- * batch * num_q_heads below 2^31.
+ * batch * num_q_heads below 2^31; bt_width * block_size below 2^31 - 8192.
  *   workspace: kvfp8_shared_prefix_workspace_bytes(batch, ..., prompt = 0) bytes, 256-byte aligned, any
  *   contents.
  * No reference counterpart: there every sequence reads its own pages
