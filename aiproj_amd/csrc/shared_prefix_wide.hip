@@ -20,7 +20,7 @@
 // block g - 1. Scales and counts, of which a wave that lags may still read those of g - 1, have four buffers.
 //
 // What bounds it (256 x 64 heads, 16384 tokens of 8 KV heads x 128, bf16 on e4m3fn: 157-175 us without the own tokens, 800-870
-// TFLOP/s): a block takes 5200 cycles of which the matrix cores work 2050 and the vector ALU 2300 (nine operations a score,
+// TFLOP/s): a block takes 5200 cycles of which the matrix cores work 2050 and the vector ALU 2300 (six operations a score,
 // the exponential counts two), and one hides little of the other: next to 16x16x32 products vector operations of
 // another wave took 70% of their time on top, next to 32x32x16 ones 37% (both alone in a loop). LDS reads fill 1600 cycles
 // (256 bytes each), the widened writes 500. Measured on 9216 rows x 16 heads x 4096 tokens: two half-workgroups in turn on
