@@ -116,11 +116,13 @@ struct Sums {
     float m, s, t;      // max, sum e^(x - m), sum e^(x - m) (x - m)
 };
 
-// The state with its maximum moved up to m (finite or -inf, at least a.m).
+// The state with its maximum moved up to m (finite or -inf, at least a.m). Below -200 f is 0, and d is kept finite for
+// the product: entries of a type's lowest value are some 1e38 below the others, which the number of them takes past
+// float32's range.
 __device__ __forceinline__ Sums moved(Sums a, float m) {
     const float d = a.m == kNegInf ? 0.0f : a.m - m;     // an empty state has s = t = 0
     const float f = __builtin_amdgcn_exp2f(d * kLog2e);
-    return Sums{m, a.s * f, (a.t + d * a.s) * f};
+    return Sums{m, a.s * f, (a.t + fmaxf(d, -200.0f) * a.s) * f};
 }
 
 // Adds e^d and e^d d of d = x - m. Below -200 e^d is 0, and d is kept finite for the product.
