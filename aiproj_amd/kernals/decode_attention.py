@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import functools
 import math
+import threading
 from dataclasses import dataclass
 
 import torch as t
@@ -98,24 +99,32 @@ def _workspace_bytes(b, hq, hkv, d, bt_width, block_size, kv_code) -> int:
     return _native.lib().kvfp8_decode_workspace_bytes(b, hq, hkv, d, bt_width, block_size, kv_code)
 
 
-# Decode workspaces of the calls that launch at once (decode_attention_wrapper and the
-# fused step), one per (device, stream): such calls run in stream order, so each can
-# reuse the previous call's block (the workspace needs no initialization; every call
-# rewrites what it reads). A call that needs more gets a larger block. Prepared calls
-# (prepare_decode), which may be launched later and in halves, and every call under
-# graph capture take a block of their own, so no two of them share one.
-_WORKSPACES: dict = {}
+class _Workspaces(threading.local):
+    """Workspaces of the calls that launch at once (decode_attention_wrapper, the fused step and the
+    shared-prefix calls), one per (device, stream) of a thread: a thread's calls run in stream order,
+    so each can reuse the previous call's block (the workspace needs no initialization; every call
+    rewrites what it reads). A call that needs more gets a larger block. Threads have blocks of their own
+    because a call is several launches, made without the interpreter's lock: two threads on one stream may
+    enqueue theirs in turn, and one's second launch reads what its first one left. Prepared calls
+    (prepare_decode), which may be launched later and in halves, and every call under
+    graph capture take a block of their own, so no two of them share one."""
+
+    def __init__(self):
+        self.held = {}
+
+
+_WORKSPACES = _Workspaces()
 
 
 def _workspace(device: t.device, stream: int, nbytes: int) -> t.Tensor:
     nbytes = max(nbytes, 1)
     if t.cuda.is_current_stream_capturing():
         return t.empty(nbytes, dtype=t.uint8, device=device)
-    key = (device.index, stream)
-    ws = _WORKSPACES.get(key)
+    held, key = _WORKSPACES.held, (device.index, stream)
+    ws = held.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = t.empty(nbytes, dtype=t.uint8, device=device)
-        _WORKSPACES[key] = ws
+        held[key] = ws
     return ws
 
 
@@ -123,8 +132,8 @@ def prepare_decode(q, paged_kv_cache, cache_batch_context=None, _launch_now=Fals
     """Validate the arguments of `decode_attention_wrapper` (same forms, same
     asserts and errors), allocate its output and workspace, and return the
     prepared call without launching anything. (`_launch_now`: the caller launches the
-    call right away on the current stream, so it may take the stream's shared
-    workspace.)"""
+    call right away on the current stream, so it may take the workspace that its thread
+    keeps for the stream.)"""
     if cache_batch_context is None:
         kv = paged_kv_cache                       # PagedKVRead form
         k_cache, v_cache = kv.k, kv.v

@@ -111,7 +111,9 @@ int64_t kvfp8_decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t
  * k/v scales: [num_blocks, block_size, Hkv] float32, NULL unless e4m3fn.
  * block_table: [bt_rows, bt_width] int32, entries outside [0, num_blocks) skipped.
  * slots: [B] int32/int64 rows of block_table; context_lengths: [B] int32/int64.
- * workspace: at least kvfp8_decode_workspace_bytes(...) bytes, any contents.
+ * workspace: at least kvfp8_decode_workspace_bytes(...) bytes, any contents. A call is several
+ *   launches, and threads that call on one stream at once enqueue theirs in turn: they
+ *   need a workspace each. So do calls on different streams.
  */
 int kvfp8_paged_decode(const void* q_dev, int q_dtype, int64_t q_stride_b, int64_t q_stride_h,
                        int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
@@ -410,7 +412,7 @@ int kvfp8_skinny_linear_rope(const void* x_dev, int dtype, int64_t x_stride, int
  * count own tokens). All index arrays int32/int64 on the device. head_dim 1..512, any batch with
  * batch * num_q_heads below 2^31; bt_width * block_size below 2^31 - 8192.
  *   workspace: kvfp8_shared_prefix_workspace_bytes(batch, ..., prompt = 0) bytes, 256-byte aligned, any
- *   contents.
+ *   contents; one for each thread and stream, as for kvfp8_paged_decode.
  * No reference counterpart: there every sequence reads its own pages
  * (reference src/torch_llm/kernals/decode_attention.py:39-550).
  */
