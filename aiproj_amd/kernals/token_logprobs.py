@@ -16,8 +16,10 @@ Sums are float32, one launch of the HIP kernel `token_logprobs_kernel` (C ABI
 `kvfp8_token_logprobs`), nothing is synchronized with the host and no [T, V] copy is made. Where
 gradients are wanted, `logprobs` and `entropy` are differentiable in the logits: one launch of
 `token_logprobs_grad_kernel` (`kvfp8_token_logprobs_backward`) reads the logits again and writes the
-gradient in their type. Gradients that a transform looks at (`is_grads_batched`, vmap) take
-PyTorch operations in float32.
+gradient in their type. Calls that a transform, mode or trace looks at (forward-mode derivatives, vmap,
+`torch.func`, `torch.jit.trace`, `torch.compile`), and gradients that one looks at (`is_grads_batched`), take
+PyTorch operations in float32, which have derivatives of every kind and order. The kernels' backward is
+differentiable once.
 
 The reference has no counterpart: its sampler takes the argmax of the logits.
 """
@@ -77,6 +79,25 @@ def _forward(logits: t.Tensor, tokens: t.Tensor, top: int, for_backward: bool = 
     return logprobs, entropy, top_logprobs, top_tokens, stats
 
 
+def _plain_forward(logits, tokens, top):
+    """(logprobs, entropy, top_logprobs, top_tokens) as PyTorch operations in float32."""
+    x = logits.float()
+    m = x.detach().amax(-1, keepdim=True)
+    empty = m == -t.inf                                  # every entry is -inf
+    d = x - t.where(empty, 0.0, m)
+    e = t.exp(d)
+    total = t.where(empty, 1.0, e.sum(-1, keepdim=True))
+    log_s = t.log(total)
+    # Below -200 e^d is 0, and d is kept finite for the product.
+    entropy = t.where(empty, 0.0, log_s - (e * d.clamp(min=-200.0)).sum(-1, keepdim=True) / total)[:, 0]
+    inside = (tokens >= 0) & (tokens < x.shape[1])
+    given = d.gather(1, t.where(inside, tokens, 0).long()[:, None]) - log_s
+    logprobs = t.where(inside, t.where(empty, -t.inf, given)[:, 0], 0.0)
+    values, order = t.sort(x.detach() + 0.0, dim=-1, descending=True, stable=True)
+    top_logprobs = t.where(empty, -t.inf, values[:, :top] - m - log_s.detach())
+    return logprobs, entropy, top_logprobs, order[:, :top]
+
+
 def _plain_backward(logits, tokens, entropy, stats, grad_logprobs, grad_entropy):
     """The gradient as PyTorch operations in float32."""
     vocab = logits.shape[1]
@@ -123,6 +144,9 @@ class TokenLogprobsFunction(t.autograd.Function):
 
 
 def token_logprobs(logits: t.Tensor, tokens: t.Tensor, top: int = 0) -> TokenLogprobs:
+    if not _native.is_plain(logits, tokens):
+        _check(logits, tokens, top)
+        return TokenLogprobs(*_plain_forward(logits, tokens, top))
     if t.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*TokenLogprobsFunction.apply(logits, tokens, top))
     return TokenLogprobs(*_forward(logits, tokens, top)[:4])
