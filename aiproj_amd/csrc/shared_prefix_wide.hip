@@ -6,9 +6,12 @@
 // two halves of 32 tokens (MFMA 32x32x16: A[row = l % 32][k = 8 (l / 32) + i], B likewise, D[row = 8 (i / 4) + 4 (l / 32)
 // + i % 4][col = l % 32]):
 //   S^T[token, row] = K Q^T     A = K rows from LDS, B = Q^T from registers
-//   softmax                     t = fma(score, k_scale[token] x sm_scale x log2(e), -reference), float32, online, base 2;
-//                               the reference follows a row's maximum only where that exceeds it by 2^8
-//   O^T[d, row] += V^T P'^T     P' = e2(t) v_scale[token] from the score registers; A = V^T by transposing LDS reads
+//   softmax                     t = score x (k_scale[token] x sm_scale x log2(e)), e2(t - reference), float32, online, base
+//                               2; the reference follows a row's maximum only where that exceeds it by 2^8. The product
+//                               is rounded before the reference is taken off: fused, an equal key in a later block would
+//                               differ by up to half a step of the reference, which at scores of 1e8 is a factor of 16
+//                               (the operation more costs 1.1% to 1.6% of a call)
+//   O^T[d, row] += V^T P'^T     P' = e2() v_scale[token] from the score registers; A = V^T by transposing LDS reads
 //
 // One stretch of code without a branch holds, for half s, the products of the scores of half s + 1, the weights of half
 // s and the products with V of half s - 1, which are independent of each other; scheduling groups spread the products
@@ -20,7 +23,7 @@
 // block g - 1. Scales and counts, of which a wave that lags may still read those of g - 1, have four buffers.
 //
 // What bounds it (256 x 64 heads, 16384 tokens of 8 KV heads x 128, bf16 on e4m3fn: 157-175 us without the own tokens, 800-870
-// TFLOP/s): a block takes 5200 cycles of which the matrix cores work 2050 and the vector ALU 2300 (six operations a score,
+// TFLOP/s): a block takes 5200 cycles of which the matrix cores work 2050 and the vector ALU 2300 (seven operations a score,
 // the exponential counts two), and one hides little of the other: next to 16x16x32 products vector operations of
 // another wave took 70% of their time on top, next to 32x32x16 ones 37% (both alone in a loop). LDS reads fill 1600 cycles
 // (256 bytes each), the widened writes 500. Measured on 9216 rows x 16 heads x 4096 tokens: two half-workgroups in turn on
@@ -265,7 +268,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
         }
 
     f32x16_t o[NB];
-    float ref = 0.0f, lim = kNegInf, l = 0.0f;           // a row's reference (0 before its first score), how far scores may pass it
+    float ref = 0.0f, lim = kNegInf, l = 0.0f;           // a row's reference (0 before its first score), what scores may reach
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -308,10 +311,11 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
                 for (int part = 0; part < kParts; ++part) o[nb] = mma32<kF16V>(av, pop[half][part][pp], o[nb]);
             }
     };
-    // Scores of a half relative to the rows' references.
+    // Scores of a half with their scales.
     float mx;
     int2 counts;                                         // tokens of the half's tiles that count
-    auto relate = [&](int32_t g, auto half_c) __attribute__((always_inline)) {
+    auto scale_scores = [&](int32_t g, auto half_c) __attribute__((always_inline)) {
+#pragma clang fp contract(off)
         constexpr int half = decltype(half_c)::value;
         counts = *reinterpret_cast<const int2*>(&lds_count[g & 3][2 * half]);
 #pragma unroll
@@ -319,7 +323,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
             f32x4_t ks = {a.d.score_scale, a.d.score_scale, a.d.score_scale, a.d.score_scale};
             if constexpr (ES == 1) ks = *reinterpret_cast<const f32x4_t*>(&lds_scale[g & 3][0][32 * half + 8 * q + 4 * hi]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sacc[half][4 * q + i] = __builtin_fmaf(sacc[half][4 * q + i], ks[i], -ref);
+            for (int i = 0; i < 4; ++i) sacc[half][4 * q + i] *= ks[i];
         }
     };
     auto largest = [&](auto half_c) __attribute__((always_inline)) {
@@ -342,18 +346,17 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
             largest(half_c);
         }
         if (!__ballot(mx > lim)) return false;
-        const float top = max_across_halves(mx);         // relative to ref
+        const float top = max_across_halves(mx);
         const bool fresh = lim == kNegInf;
-        const float step = fresh ? (top == kNegInf ? 0.0f : top) : fmaxf(top, 0.0f);
-        alpha = fresh ? 0.0f : __builtin_amdgcn_exp2f(-step);
-        lim = fresh && top == kNegInf ? kNegInf : kLag;
-        ref += step;
+        const float to = fresh ? (top == kNegInf ? 0.0f : top) : fmaxf(top, ref);
+        alpha = fresh ? 0.0f : __builtin_amdgcn_exp2f(ref - to);
+        lim = fresh && top == kNegInf ? kNegInf : to + kLag;
+        ref = to;
         l *= alpha;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sacc[half][i] -= step;
         return true;
     };
     auto weigh = [&](int32_t g, auto half_c) __attribute__((always_inline)) {
+#pragma clang fp contract(off)
         constexpr int half = decltype(half_c)::value;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -362,7 +365,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(sacc[half][4 * q + i]);
+                const float p = __builtin_amdgcn_exp2f(sacc[half][4 * q + i] - ref);
                 l += p;
                 x[i] = ES == 1 ? p * vs[i] : p;
             }
@@ -386,7 +389,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
 #pragma unroll
         for (int i = 0; i < kProducts; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                       // matrix products
-            __builtin_amdgcn_sched_group_barrier(0x402, stages ? 9 : 6, 0);          // softmax, widening
+            __builtin_amdgcn_sched_group_barrier(0x402, stages ? 10 : 7, 0);          // softmax, widening
             if (2 * i < kReads) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
             else if (stages) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
         }
@@ -425,7 +428,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
     if (active) {
         read_k(c0, c0, 0, KS);
         qk(c0);
-        relate(0, c0);
+        scale_scores(0, c0);
         largest(c0);
         read_k(c0, c1, 0, kPre);
         settle(c0);                                      // O and l are zeros yet
@@ -438,7 +441,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
         qk(next);
         weigh(g, half_c);
         if (!first) pv(vbuf_c, next);
-        relate(gn, next);
+        scale_scores(gn, next);
         largest(next);
     };
     auto rest = [&](auto half_c) __attribute__((always_inline)) {
