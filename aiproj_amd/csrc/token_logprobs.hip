@@ -136,8 +136,9 @@ __device__ __forceinline__ void add_entry(Sums& a, float x, float m) {
 // Two entries of -inf (one of float32).
 template <int DT>
 constexpr uint32_t kNegInfBits = DT == KVFP8_F32 ? 0xFF800000u : (DT == KVFP8_BF16 ? 0xFF80FF80u : 0xFC00FC00u);
-// Lowest bit of the wave's search for a bound: the values' own last bit, or 20 bits of float32 (a bound that is
-// a little low only lets more entries into the list).
+// Lowest bit of the wave's first search for a bound: the values' own last bit, or 20 bits of float32 (a bound that is
+// a little low only lets more entries into the list; in the order of negative values the bits left out are ones, so it
+// lies below the value itself). The second bound has all bits: it has to be a value of the row, which entries equal.
 template <int DT>
 constexpr int kLastBit = DT == KVFP8_BF16 ? 16 : (DT == KVFP8_F16 ? 13 : 12);
 
@@ -229,9 +230,9 @@ token_logprobs_kernel(LogprobArgs a) {
     }
     // The n-th largest thread maximum of the wave, as an order of values (0 where fewer threads hold entries).
     const uint32_t mine = tid < vectors || tid < rest ? ordered(best) : 0u;
-    auto nth_of_wave = [&](int n) __attribute__((always_inline)) {
+    auto nth_of_wave = [&](int n, int last_bit) __attribute__((always_inline)) {
         uint32_t bound = 0;
-        for (int bit = 31; bit >= kLastBit<DT>; --bit) {
+        for (int bit = 31; bit >= last_bit; --bit) {
             const uint32_t trial = bound | (1u << bit);
             if (__popcll(__ballot(mine >= trial)) >= n) bound = trial;
         }
@@ -242,7 +243,7 @@ token_logprobs_kernel(LogprobArgs a) {
         uint32_t bound = 0;
         const int n = full > 0 ? (a.top + full - 1) / full : 0;
         if (n == 1) bound = ordered(st.m);
-        else if (n > 1) bound = nth_of_wave(n);
+        else if (n > 1) bound = nth_of_wave(n, kLastBit<DT>);
         if (lane == 0) wave_bound[wave] = bound;
     }
     st.s = wave_sum(st.s);
@@ -343,7 +344,7 @@ token_logprobs_kernel(LogprobArgs a) {
             return;
         }
         __syncthreads();                                 // all have read the bounds and the count
-        const uint32_t higher = nth_of_wave(a.top);
+        const uint32_t higher = nth_of_wave(a.top, 0);
         if (lane == 0) wave_bound[wave] = higher;
         if (tid == 0) listed = 0;
         __syncthreads();

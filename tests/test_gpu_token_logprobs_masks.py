@@ -69,3 +69,18 @@ def test_gradients_behind_masks_of_large_finite_values(dtype, vocab, trains):
         slack = size * (_slack(logits, logp)[:, None] * 4 + 2.0 ** -22 * (1 + far))
         tiny = t.finfo(dtype).tiny * t.finfo(dtype).eps / 2
         assert bool(((grad.double() - want).abs() <= HALF[dtype] * 1.01 * want.abs() + slack + tiny).all())
+
+
+@pytest.mark.parametrize("left", [0, 1, 10, 63])
+@pytest.mark.parametrize("value", [-1e4, -7.5, -0.3, 0.0, 1.7])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_alternatives_of_rows_with_fewer_entries_than_asked_for(dtype, value, left):
+    """More entries of one value than the list holds, which follow those above it by index; some of the rest lie below it."""
+    for vocab in (2000, 9000, 32000, 140000):
+        logits = t.full((3, vocab), value, device="cuda", dtype=dtype)
+        gen = t.Generator(device="cuda").manual_seed(left)
+        for row, at in enumerate((0, vocab // 2, vocab - left - 7)):
+            logits[row, at:at + left] = value + 1 + t.rand(left, generator=gen, device="cuda").to(dtype)
+            logits[row, at + left:at + left + 5] = value - 1
+        for top in (20, 64):
+            _check_forward(logits, t.tensor([0, 1, vocab - 1], device="cuda"), top)
