@@ -261,6 +261,12 @@ hipError_t launch_generic_kv(const PrefixArgs& a, int kv_dtype, hipStream_t s) {
 bool index_dtype(int t) { return t == KVFP8_I32 || t == KVFP8_I64; }
 bool float_dtype(int t) { return t == KVFP8_F32 || t == KVFP8_F16 || t == KVFP8_BF16; }
 
+// Sizes (none negative) that the kernels take, from which nothing on the host overflows. Their token numbers are int32
+// and run up to three blocks past the last.
+bool within_limits(int64_t rows, int32_t hq, int32_t d, int64_t bt_width, int32_t block_size) {
+    return d <= kGenMaxD && rows <= INT32_MAX && rows * hq <= INT32_MAX && bt_width <= (INT32_MAX - 8192) / block_size;
+}
+
 // What the two forms check alike; fills the shared arguments.
 int shared_args(PrefixArgs& a, const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h, int64_t rows,
                 int32_t hq, int32_t hkv, int32_t d, const void* k_cache, const void* v_cache, int kv_dtype,
@@ -274,8 +280,7 @@ int shared_args(PrefixArgs& a, const void* q, int q_dtype, int64_t q_stride_t, i
     if (rows < 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || d <= 0 || num_blocks <= 0 || bt_rows <= 0 || bt_width <= 0 ||
         block_size <= 0 || (block_size & (block_size - 1)) != 0 || groups < 0)
         return KVFP8_ESHAPE;
-    // The kernels' token numbers are int32 and run up to three blocks past the last.
-    if (d > kGenMaxD || rows > INT32_MAX || rows * hq > INT32_MAX || bt_width * block_size > INT32_MAX - 8192) return KVFP8_ELIMIT;
+    if (!within_limits(rows, hq, d, bt_width, block_size)) return KVFP8_ELIMIT;
     if (rows == 0) return KVFP8_OK;
     if (!q || !k_cache || !v_cache || !block_table || !out || (groups > 0 && (!p_slots || !p_lens || !p_starts)))
         return KVFP8_ENULL;
@@ -372,8 +377,8 @@ extern "C" int64_t kvfp8_shared_prefix_workspace_bytes(int64_t rows, int32_t num
                                                        int32_t head_dim, int32_t groups, int64_t bt_width,
                                                        int32_t block_size, int kv_dtype, int prompt) {
     if (rows <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || groups < 0 || bt_width <= 0 ||
-        block_size <= 0)
-        return 0;
+        block_size <= 0 || !within_limits(rows, num_q_heads, head_dim, bt_width, block_size))
+        return 0;                                        // the calls refuse these
     // The larger of what the paths need that a call of these shapes may take (its pointers decide).
     int64_t bytes = make_plan(rows, num_q_heads, head_dim, bt_width, block_size, prompt != 0).bytes;
     if (num_q_heads % num_kv_heads == 0)

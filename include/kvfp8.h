@@ -412,7 +412,7 @@ int kvfp8_skinny_linear_rope(const void* x_dev, int dtype, int64_t x_stride, int
  * count own tokens). All index arrays int32/int64 on the device. head_dim 1..512, any batch with
  * batch * num_q_heads below 2^31; bt_width * block_size below 2^31 - 8192.
  *   workspace: kvfp8_shared_prefix_workspace_bytes(batch, ..., prompt = 0) bytes, 256-byte aligned, any
- *   contents; one for each thread and stream, as for kvfp8_paged_decode.
+ *   contents; one for each thread and stream, as for kvfp8_paged_decode. Sizes that the calls refuse need 0.
  * No reference counterpart: there every sequence reads its own pages
  * (reference src/torch_llm/kernals/decode_attention.py:39-550).
  */
