@@ -10,7 +10,9 @@
 //   O^T[d, row] += V^T P'^T     P' = p v_scale[token]; V^T by byte transposes of eight token rows
 // Operand types: bf16 q over e4m3fn codes bf16 throughout; f16 q multiplies codes widened to f16 (exact),
 // its P' enters as two bf16 parts (an f16 P' would lose scales outside f16's range); float32 q and its P'
-// as three bf16 parts; bf16 and f16 caches with q of their type are operands as they are.
+// as three bf16 parts; bf16 and f16 caches with q of their type are operands as they are. A P' of one part is off by up to
+// half a step of its type and the sum of weights is not: for bf16 an error of 2.3e-3 of the output's norm against the 1.7e-3
+// that its own rounding makes. A second part would cost a product more for each.
 // Bound by latency where there are few tokens (a step's loads wait for its pages, the first ones for the group's search:
 // 4 x 8 heads, 500 tokens: 6.1 us), by the widening and transposing of V's codes and the loads' latency where there are
 // many: own tokens of 256 sequences, 520 on average, 8 KV heads x 128: 82 us, 3.4 TB/s (decode without prefixes takes

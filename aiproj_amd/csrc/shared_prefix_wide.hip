@@ -23,7 +23,7 @@
 // block g - 1. Scales and counts, of which a wave that lags may still read those of g - 1, have four buffers.
 //
 // What bounds it (256 x 64 heads, 16384 tokens of 8 KV heads x 128, bf16 on e4m3fn: 157-175 us without the own tokens, 800-870
-// TFLOP/s): a block takes 5200 cycles of which the matrix cores work 2050 and the vector ALU 2300 (seven operations a score,
+// TFLOP/s): a block takes 5300 cycles of which the matrix cores work 2050 and the vector ALU 2500 (seven operations a score,
 // the exponential counts two), and one hides little of the other: next to 16x16x32 products vector operations of
 // another wave took 70% of their time on top, next to 32x32x16 ones 37% (both alone in a loop). LDS reads fill 1600 cycles
 // (256 bytes each), the widened writes 500. Measured on 9216 rows x 16 heads x 4096 tokens: two half-workgroups in turn on
@@ -40,7 +40,9 @@ namespace {
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr int kKeys = 64;             // tokens per block
 constexpr int kWideWaves = 8;
-constexpr float kLag = 8.0f;          // log2 of how far a row's maximum may exceed its reference
+// log2 of how far a row's maximum may exceed its reference. Weights reach 2^8 so, and the largest is not 1 in general: it
+// is rounded to the products' type like the others, by at most half a step relatively, while their sum is not.
+constexpr float kLag = 8.0f;
 
 typedef __attribute__((address_space(3))) const uint8_t lds_u8;
 typedef __attribute__((address_space(3))) const u32x4_t lds_u32x4;
@@ -498,7 +500,7 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
     const int hq = h * G + (pair - t * G);
     // Element 4 q + i of block nb: dim 32 nb + 8 q + 4 hi + i of the row.
     if (a.cu != nullptr && a.splits == 1 && it.tail < 0) {
-        // The prompt form's only state of the row: joined with out and lse at once.
+        // The prompt form's only state of the row: joined with out and lse at once (out has been rounded once before).
         if (seq_of_row(a, row) < 0) return;
         const int64_t at = row * a.d.num_q_heads + hq;
         const float mo = a.lse[at] * kLog2e;
