@@ -41,6 +41,7 @@ _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _DECODE_ARGS = [_P, _INT, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _INT, _P, _P, _I64, _I32, _P, _I64, _I64,
                 _P, _INT, _P, _INT, ctypes.c_float, _P, _P, _I64, _P]
+_NORM_ROPE_ARGS = [_P, _INT, _I64, _I32, _I32, _I32, _I64, _P, _INT, _P, _P, _INT, _I64, _P, _P, _INT, ctypes.c_float]
 _PREFIX_ARGS = [_P, _INT, _P, _INT, _P, _INT, _I32]
 SIGNATURES = {
     "kvfp8_quantize_append": (_INT, [_P, _P, _INT, _I64, _I64, _I64, _I64, _P, _INT, _P, _INT,
@@ -78,6 +79,9 @@ SIGNATURES = {
                                                                    _I64, _P]),
     "kvfp8_token_logprobs": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _INT, _I32, _P, _P, _P, _P, _P, _P]),
     "kvfp8_token_logprobs_backward": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _INT, _P, _P, _P, _P, _P, _P]),
+    "kvfp8_norm_rope": (_INT, _NORM_ROPE_ARGS + [_P, _P, _P, _P, _INT, _P, _INT, _I64, _I32, _P, _P, _INT, _P, _P, _P]),
+    "kvfp8_norm_rope_backward_workspace_bytes": (_I64, [_I64, _I32, _I32, _I32]),
+    "kvfp8_norm_rope_backward": (_INT, _NORM_ROPE_ARGS + [_P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "kvfp8_timing_enable": (_INT, [_I32]),
     "kvfp8_timing_read": (_INT, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_I64)]),
     "kvfp8_strerror": (ctypes.c_char_p, [_INT]),
@@ -184,6 +188,17 @@ def stream_handle(device: torch.device) -> int:
         index = device.index if device.index is not None else torch.cuda.current_device()
         return _raw_stream(index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(name: str, device: torch.device, *args) -> None:
+    """Entry point `name` with these arguments and the current stream of `device` behind them, on that device: a kernel
+    is launched on the device that is current, which need not be its tensors'."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(name)(*args, stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(name)(*args, stream_handle(device))
+    check(rc, name)
 
 
 # Looked up once: is_plain is asked on every call of some entry points (0.7 µs; a little more than half of the time that

@@ -174,6 +174,37 @@ static PyObject* py_kvfp8_token_logprobs_backward(PyObject* self, PyObject* cons
     return PyLong_FromLong(rc);
 }
 
+/* kvfp8_norm_rope: 32 arguments, eps at 16. */
+static PyObject* py_kvfp8_norm_rope(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+    (void)self;
+    int64_t iv[32];
+    float eps = 0.0f;
+    if (!parse(args, nargs, 32, 16, iv, &eps, "kvfp8_norm_rope")) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = kvfp8_norm_rope(PTR(0), (int)iv[1], iv[2], (int32_t)iv[3], (int32_t)iv[4], (int32_t)iv[5], iv[6], PTR(7), (int)iv[8],
+                         PTR(9), PTR(10), (int)iv[11], iv[12], PTR(13), PTR(14), (int)iv[15], eps, PTR(17), PTR(18), PTR(19),
+                         PTR(20), (int)iv[21], PTR(22), (int)iv[23], iv[24], (int32_t)iv[25], PTR(26), PTR(27), (int)iv[28],
+                         (float*)PTR(29), (float*)PTR(30), PTR(31));
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+/* kvfp8_norm_rope_backward: 26 arguments, eps at 16. */
+static PyObject* py_kvfp8_norm_rope_backward(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+    (void)self;
+    int64_t iv[26];
+    float eps = 0.0f;
+    if (!parse(args, nargs, 26, 16, iv, &eps, "kvfp8_norm_rope_backward")) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = kvfp8_norm_rope_backward(PTR(0), (int)iv[1], iv[2], (int32_t)iv[3], (int32_t)iv[4], (int32_t)iv[5], iv[6], PTR(7),
+                                  (int)iv[8], PTR(9), PTR(10), (int)iv[11], iv[12], PTR(13), PTR(14), (int)iv[15], eps,
+                                  PTR(17), PTR(18), PTR(19), PTR(20), PTR(21), PTR(22), PTR(23), iv[24], PTR(25));
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
 static PyMethodDef methods[] = {
     {"kvfp8_paged_decode", (PyCFunction)(void (*)(void))py_kvfp8_paged_decode, METH_FASTCALL, NULL},
     {"kvfp8_paged_decode_split", (PyCFunction)(void (*)(void))py_kvfp8_paged_decode_split, METH_FASTCALL, NULL},
@@ -185,6 +216,8 @@ static PyMethodDef methods[] = {
     {"kvfp8_shared_prefix_prefill", (PyCFunction)(void (*)(void))py_kvfp8_shared_prefix_prefill, METH_FASTCALL, NULL},
     {"kvfp8_token_logprobs", (PyCFunction)(void (*)(void))py_kvfp8_token_logprobs, METH_FASTCALL, NULL},
     {"kvfp8_token_logprobs_backward", (PyCFunction)(void (*)(void))py_kvfp8_token_logprobs_backward, METH_FASTCALL, NULL},
+    {"kvfp8_norm_rope", (PyCFunction)(void (*)(void))py_kvfp8_norm_rope, METH_FASTCALL, NULL},
+    {"kvfp8_norm_rope_backward", (PyCFunction)(void (*)(void))py_kvfp8_norm_rope_backward, METH_FASTCALL, NULL},
     {NULL, NULL, 0, NULL},
 };
 

@@ -1,0 +1,208 @@
+"""Norms of the query and key heads with the position rotation, in one pass over fused projection rows.
+
+Models that norm their queries and keys per head apply, to every head row x of q and k of a token,
+
+    y = x / sqrt(mean(x^2) + eps) * weight          (one weight [D] for the q heads, one for the k heads)
+
+and then the interleaved-pair rotation of the token's position (`model/transformer.py` `RoPE`, whose tables these
+functions take). Both happen in float32 with one rounding to the rows' type, one launch of `norm_rope_kernel` (C ABI
+`kvfp8_norm_rope`); values are copied.
+
+* `norm_rope(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, q_weight, k_weight, eps) -> (q, k, v)`:
+  packed q [T, Hq, D], k and v [T, Hkv, D] of rows [T, (Hq + 2 Hkv) D] (float32, float16 or bfloat16, unit element
+  stride, any row stride). Differentiable once in qkv and both weights: one launch of `norm_rope_backward_kernel` and
+  one for the weights (`kvfp8_norm_rope_backward`), sums in a fixed order. Calls and gradients that a transform, mode or
+  trace looks at take PyTorch operations in float32, which have derivatives of every kind and order.
+* `norm_rope_append(..., eps, paged_kv_cache, physical_blocks, block_offsets, packed=False)`: the same, and k and v
+  written to the paged cache on the way: what `append_kv` writes of them, where k is quantized (or stored) from its
+  float32 values, without the rounding to the rows' type before. Returns q, or (q, k, v) with `packed`, for the attention
+  of prompts. No gradients. Token locations as in `append_kv`: those outside the pool are skipped (padded rows), and no
+  two rows share one.
+
+`q_weight` and `k_weight` may both be None: rotation alone, in float32 with one rounding (`RoPE.split` rounds after
+every operation, as the reference does). Positions outside the tables leave the normed rows unrotated. D is even and at
+most 512. The reference has neither (its rotation: `model/rope.py:46-55`).
+"""
+
+from __future__ import annotations
+
+import torch as t
+
+from aiproj_amd import _native
+
+_DTYPES = (t.float32, t.float16, t.bfloat16)
+
+
+def _check(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, q_weight, k_weight, what: str):
+    """Head size of the rows."""
+    if qkv.ndim != 2 or positions.shape != qkv.shape[:1]:
+        raise ValueError(f"{what}: rows [T, (Hq + 2 Hkv) D] and positions [T]")
+    heads = num_q_heads + 2 * num_kv_heads
+    if num_q_heads <= 0 or num_kv_heads <= 0 or qkv.shape[1] % heads or qkv.shape[1] == 0:
+        raise ValueError(f"{what}: rows hold num_q_heads + 2 num_kv_heads heads")
+    d = qkv.shape[1] // heads
+    if qkv.dtype not in _DTYPES:
+        raise ValueError(f"{what}: unsupported dtype {qkv.dtype}")
+    if positions.dtype not in (t.int32, t.int64):
+        raise ValueError(f"{what}: positions must be int32 or int64")
+    if d % 2 or d > 512:
+        raise ValueError(f"{what}: head size {d} is odd or above 512")
+    if (cos_table.ndim != 2 or cos_table.shape[1] != d // 2 or cos_table.shape[0] == 0 or sin_table.shape != cos_table.shape
+            or cos_table.dtype not in _DTYPES or sin_table.dtype != cos_table.dtype):
+        raise ValueError(f"{what}: tables [positions, D / 2] of one floating dtype")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError(f"{what}: weights for both q and k, or for neither")
+    if q_weight is not None and (q_weight.shape != (d,) or k_weight.shape != (d,) or q_weight.dtype not in _DTYPES
+                                 or k_weight.dtype != q_weight.dtype):
+        raise ValueError(f"{what}: weights [D] of one floating dtype")
+    return d
+
+
+def _c(x):
+    return x if x is None or x.is_contiguous() else x.contiguous()
+
+
+def _operands(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, q_weight, k_weight, eps):
+    """The arguments that both C entries begin with, and the tensors whose addresses they hold."""
+    if qkv.stride(1) != 1:
+        qkv = qkv.contiguous()
+    positions, cos_table, sin_table, q_weight, k_weight = map(_c, (positions, cos_table, sin_table, q_weight, k_weight))
+    code, ptr = _native.TORCH_TO_CODE, _native.ptr
+    args = (qkv.data_ptr(), code[qkv.dtype], qkv.shape[0], num_q_heads, num_kv_heads, d, qkv.stride(0), positions.data_ptr(),
+            code[positions.dtype], cos_table.data_ptr(), sin_table.data_ptr(), code[cos_table.dtype], cos_table.shape[0],
+            ptr(q_weight), ptr(k_weight), code[t.float32 if q_weight is None else q_weight.dtype], float(eps))
+    return args, (qkv, positions, cos_table, sin_table, q_weight, k_weight)
+
+
+_NO_CACHE = (None, _native.I64, None, _native.I64, 0, 0, None, None, _native.E4M3FN, None, None)
+
+
+def _empty(rows, heads, d, like):
+    return t.empty((rows, heads, d), dtype=like.dtype, device=like.device)
+
+
+def _forward(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, q_weight, k_weight, eps, what):
+    device = _native.require_gpu(qkv, positions, cos_table, sin_table, q_weight, k_weight, what=what)
+    rows = qkv.shape[0]
+    q, k, v = (_empty(rows, h, d, qkv) for h in (num_q_heads, num_kv_heads, num_kv_heads))
+    if rows:
+        args, keep = _operands(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, q_weight, k_weight, eps)
+        _native.launch("kvfp8_norm_rope", device, *args, q.data_ptr(), k.data_ptr(), v.data_ptr(), *_NO_CACHE)
+    return q, k, v
+
+
+def _turn(y, cos, sin):
+    """Pairs (2 i, 2 i + 1) of rows [T, H, D] turned by angles [T, 1, D / 2]."""
+    a, b = y[..., 0::2], y[..., 1::2]
+    return t.stack([cos * a - sin * b, sin * a + cos * b], -1).flatten(-2)
+
+
+def _plain(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, q_weight, k_weight, eps):
+    """(q, k, v) as PyTorch operations in float32."""
+    x = qkv.unflatten(1, (-1, d)).float()
+    inside = ((positions >= 0) & (positions < cos_table.shape[0]))[:, None, None]
+    at = positions.clamp(0, cos_table.shape[0] - 1)
+    cos = t.where(inside, cos_table[at].float()[:, None], 1.0)
+    sin = t.where(inside, sin_table[at].float()[:, None], 0.0)
+    out = []
+    for part, w in ((x[:, :num_q_heads], q_weight), (x[:, num_q_heads:num_q_heads + num_kv_heads], k_weight)):
+        if w is not None:
+            part = part / t.sqrt(part.square().mean(-1, keepdim=True) + eps) * w.float()
+        out.append(_turn(part, cos, sin).to(qkv.dtype))
+    return *out, x[:, num_q_heads + num_kv_heads:].to(qkv.dtype)
+
+
+class NormRopeFunction(t.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, q_weight, k_weight, eps):
+        ctx.save_for_backward(qkv, positions, cos_table, sin_table, q_weight, k_weight)
+        ctx.sizes = (num_q_heads, num_kv_heads, d, eps)
+        ctx.set_materialize_grads(False)
+        return _forward(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, q_weight, k_weight, eps, "norm_rope")
+
+    @staticmethod
+    @t.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        qkv, positions, cos_table, sin_table, q_weight, k_weight = ctx.saved_tensors
+        num_q_heads, num_kv_heads, d, eps = ctx.sizes
+        wanted = [ctx.needs_input_grad[i] for i in (0, 7, 8)]
+        none = (None,) * 10
+        if all(g is None for g in grads):
+            return none
+        tensors = [x for x in (qkv, positions, cos_table, sin_table, q_weight, k_weight, *grads) if x is not None]
+        if not _native.is_plain(*tensors):
+            with t.enable_grad():
+                leaves = [None if x is None else x.detach().requires_grad_(w) for x, w in zip((qkv, q_weight, k_weight), wanted)]
+                outs = _plain(leaves[0], positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, *leaves[1:], eps)
+                pairs = [(o, g) for o, g in zip(outs, grads) if g is not None]
+                into = [x for x, w in zip(leaves, wanted) if w]
+                got = iter(t.autograd.grad([o for o, _ in pairs], into, [g for _, g in pairs], allow_unused=True))
+            dx, dq, dk = (next(got) if w else None for w in wanted)
+        else:
+            gq, gk, gv = map(_c, grads)
+            rows = qkv.shape[0]
+            dx = t.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device) if wanted[0] else None
+            dq = t.empty_like(q_weight, memory_format=t.contiguous_format) if wanted[1] else None
+            dk = t.empty_like(k_weight, memory_format=t.contiguous_format) if wanted[2] else None
+            size = 0
+            if dq is not None or dk is not None:
+                size = _native.lib().kvfp8_norm_rope_backward_workspace_bytes(rows, num_q_heads, num_kv_heads, d)
+            workspace = t.empty(max(size, 1), dtype=t.uint8, device=qkv.device)
+            args, keep = _operands(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, q_weight, k_weight, eps)
+            ptr = _native.ptr
+            _native.launch("kvfp8_norm_rope_backward", qkv.device, *args, ptr(gq), ptr(gk), ptr(gv), ptr(dx), ptr(dq), ptr(dk),
+                           workspace.data_ptr(), size)
+        return dx, None, None, None, None, None, None, dq, dk, None
+
+
+def norm_rope(qkv: t.Tensor, positions: t.Tensor, cos_table: t.Tensor, sin_table: t.Tensor, num_q_heads: int, num_kv_heads: int,
+              q_weight: t.Tensor | None, k_weight: t.Tensor | None, eps: float = 1e-5) -> tuple[t.Tensor, t.Tensor, t.Tensor]:
+    what = "norm_rope"
+    d = _check(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, q_weight, k_weight, what)
+    args = (qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, q_weight, k_weight, eps)
+    given = [x for x in (qkv, positions, cos_table, sin_table, q_weight, k_weight) if x is not None]
+    if not _native.is_plain(*given):
+        _native.require_gpu(*given, what=what)
+        return _plain(*args)
+    if t.is_grad_enabled() and any(x is not None and x.requires_grad for x in (qkv, q_weight, k_weight)):
+        return NormRopeFunction.apply(*args)
+    return _forward(*args, what)
+
+
+@t.no_grad()
+def norm_rope_append(qkv: t.Tensor, positions: t.Tensor, cos_table: t.Tensor, sin_table: t.Tensor, num_q_heads: int,
+                     num_kv_heads: int, q_weight: t.Tensor | None, k_weight: t.Tensor | None, eps: float, paged_kv_cache,
+                     physical_blocks: t.Tensor, block_offsets: t.Tensor, packed: bool = False):
+    what = "norm_rope_append"
+    d = _check(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, q_weight, k_weight, what)
+    cache, blocks, offsets = paged_kv_cache, physical_blocks, block_offsets
+    k_cache, v_cache, rows = cache.k, cache.v, qkv.shape[0]
+    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[2:] != (num_kv_heads, d) or v_cache.dtype != k_cache.dtype:
+        raise ValueError(f"{what}: cache rows [num_blocks, block_size, Hkv, D] that match the rows' heads")
+    if blocks.shape != (rows,) or offsets.shape != (rows,):
+        raise ValueError(f"{what}: one cache location a row")
+    if blocks.dtype not in (t.int32, t.int64) or offsets.dtype not in (t.int32, t.int64):
+        raise ValueError(f"{what}: cache locations must be int32 or int64")
+    k_scales = v_scales = None
+    if cache.quantized:
+        k_scales, v_scales = cache.k_scales, cache.v_scales
+        if (k_cache.dtype != t.float8_e4m3fn or k_scales.dtype != t.float32 or v_scales.dtype != t.float32
+                or k_scales.shape != k_cache.shape[:3] or v_scales.shape != k_cache.shape[:3]):
+            raise ValueError(f"{what}: a quantized cache holds float8_e4m3fn and float32 scales per row")
+    elif k_cache.dtype not in _DTYPES:
+        raise ValueError(f"{what}: unsupported cache dtype {k_cache.dtype}")
+    if any(x is not None and not x.is_contiguous() for x in (k_cache, v_cache, k_scales, v_scales)):
+        raise ValueError(f"{what}: cache tensors must be contiguous")
+    device = _native.require_gpu(qkv, positions, cos_table, sin_table, q_weight, k_weight, k_cache, v_cache, k_scales, v_scales,
+                                 blocks, offsets, what=what)
+    q = _empty(rows, num_q_heads, d, qkv)
+    k, v = (_empty(rows, num_kv_heads, d, qkv) for _ in range(2)) if packed else (None, None)
+    if rows:
+        args, keep = _operands(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, q_weight, k_weight, eps)
+        blocks, offsets = _c(blocks), _c(offsets)
+        code, ptr = _native.TORCH_TO_CODE, _native.ptr
+        _native.launch(
+            "kvfp8_norm_rope", device, *args, q.data_ptr(), ptr(k), ptr(v), blocks.data_ptr(), code[blocks.dtype],
+            offsets.data_ptr(), code[offsets.dtype], k_cache.shape[0], k_cache.shape[1], k_cache.data_ptr(), v_cache.data_ptr(),
+            code[k_cache.dtype], ptr(k_scales), ptr(v_scales))
+    return (q, k, v) if packed else q

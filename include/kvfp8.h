@@ -474,6 +474,47 @@ int kvfp8_token_logprobs_backward(const void* logits_dev, int dtype, int64_t row
                                   const float* stats_dev, const float* grad_logprobs_dev,
                                   const float* grad_entropy_dev, void* grad_logits_dev, void* stream);
 
+/*
+ * Norms of the query and key heads with the rotary embedding, in one pass over fused projection rows
+ * [q heads | k heads | v heads] of head_dim elements (row_stride elements between rows, unit element stride;
+ * f32/f16/bf16). Per head row x of q and k: y = x / sqrt(mean x^2 + eps) * weight (q_weight, k_weight [head_dim], w_dtype;
+ * both NULL: y = x), then kvfp8_rope_inplace's rotation of y by the row's position, all in float32 with one rounding.
+ * A position outside the tables leaves y unrotated. Values are copied.
+ *   q_out [rows, num_q_heads, head_dim], k_out and v_out [rows, num_kv_heads, head_dim], packed, x's dtype; k_out and v_out
+ *   may both be NULL with a cache.
+ *   blocks/offsets not NULL: k (before the rounding to x's dtype) and v are also written to a paged cache at
+ *   (blocks[r], offsets[r]), by the rule of kvfp8_quantize_append (cache_dtype e4m3fn, with scales) or
+ *   kvfp8_store_append (f32/f16/bf16); locations outside the pool are skipped. No two rows share a location.
+ * head_dim even, up to 512; rows * (num_q_heads + 2 num_kv_heads) below 2^31. Any alignment; rows, tables, weights and
+ * outputs that are 16-byte aligned with head_dim a multiple of 8 take wide accesses. The reference has no such norms
+ * (its rotation: reference src/torch_llm/model/rope.py:46-55).
+ */
+int kvfp8_norm_rope(const void* x_dev, int dtype, int64_t rows, int32_t num_q_heads, int32_t num_kv_heads,
+                    int32_t head_dim, int64_t row_stride, const void* positions_dev, int pos_dtype,
+                    const void* cos_table_dev, const void* sin_table_dev, int table_dtype, int64_t table_rows,
+                    const void* q_weight_dev, const void* k_weight_dev, int w_dtype, float eps, void* q_out_dev,
+                    void* k_out_dev, void* v_out_dev, const void* blocks_dev, int blocks_dtype,
+                    const void* offsets_dev, int offsets_dtype, int64_t num_blocks, int32_t block_size,
+                    void* k_cache_dev, void* v_cache_dev, int cache_dtype, float* k_scales_dev, float* v_scales_dev,
+                    void* stream);
+
+/*
+ * Backward of kvfp8_norm_rope: from the gradients of q, k and v (packed, x's dtype; NULL: zeros) those of the rows
+ * (dx [rows, (num_q_heads + 2 num_kv_heads) head_dim] contiguous, x's dtype; NULL: not wanted) and of the weights
+ * (dq_weight, dk_weight [head_dim], w_dtype; NULL: not wanted), float32 sums in a fixed order, one rounding.
+ * The workspace (kvfp8_norm_rope_backward_workspace_bytes, any contents; sizes that the call refuses need 0) is needed
+ * for the weights' gradients only.
+ */
+int64_t kvfp8_norm_rope_backward_workspace_bytes(int64_t rows, int32_t num_q_heads, int32_t num_kv_heads,
+                                                 int32_t head_dim);
+int kvfp8_norm_rope_backward(const void* x_dev, int dtype, int64_t rows, int32_t num_q_heads, int32_t num_kv_heads,
+                             int32_t head_dim, int64_t row_stride, const void* positions_dev, int pos_dtype,
+                             const void* cos_table_dev, const void* sin_table_dev, int table_dtype, int64_t table_rows,
+                             const void* q_weight_dev, const void* k_weight_dev, int w_dtype, float eps,
+                             const void* grad_q_dev, const void* grad_k_dev, const void* grad_v_dev, void* dx_dev,
+                             void* dq_weight_dev, void* dk_weight_dev, void* workspace_dev, int64_t workspace_bytes,
+                             void* stream);
+
 /* Human-readable name of a return code (negative KVFP8_E* or positive hipError_t). */
 const char* kvfp8_strerror(int code);
 

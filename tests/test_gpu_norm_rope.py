@@ -1,0 +1,297 @@
+"""Normed and rotated heads on the GPU, forward, cache write and gradients, against float64."""
+
+from types import SimpleNamespace
+
+import pytest
+import torch as t
+
+from aiproj_amd.inference.paged_kv_cache import PagedKVCache
+from aiproj_amd.kernals.norm_rope import norm_rope, norm_rope_append
+from tests import norm_rope_cases as cases
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32, FP8 = t.bfloat16, t.float16, t.float32, t.float8_e4m3fn
+HALF = {x: t.finfo(x).eps / 2 for x in (BF16, F16, F32)}
+# (rows, q heads, KV heads, head size, type, weights, tables)
+FORMS = [(1, 8, 2, 64, BF16, BF16, F32), (5, 16, 4, 128, BF16, BF16, F32), (67, 32, 8, 80, F16, F32, F32),
+         (3, 6, 3, 96, F32, F32, F32), (33, 4, 4, 128, F16, F16, BF16), (9, 3, 1, 256, BF16, F32, F16),
+         (2, 5, 2, 512, F32, BF16, F32), (17, 7, 1, 40, BF16, F32, F32), (4, 2, 1, 6, F16, BF16, F32), (3, 3, 2, 2, F32, F32, F32),
+         (6, 2, 2, 130, BF16, F16, F16), (5, 1, 1, 510, F16, F32, BF16), (700, 32, 8, 128, BF16, F32, F32),
+         (5, 16, 4, 128, BF16, None, F32), (31, 3, 2, 18, F32, None, F16), (3000, 16, 4, 64, F16, None, F32)]
+IDS = ["-".join(str(x).replace("torch.", "") for x in f) for f in FORMS]
+
+
+def _case(form, **more):
+    n, hq, hkv, d, dtype, weights, tables = form
+    return cases.rows(n, hq, hkv, d, dtype, weights, tables, **more)
+
+
+def _slack(s, mag):
+    """D squares and their sum are off by D / 2 half steps of float32 relatively in the root; ten more operations."""
+    return (s.d / 2 + 16) * 2.0 ** -24 * mag
+
+
+def _check_rows(s, q, k, v):
+    want, mag, values = cases.forward_64(s)
+    got = t.cat([q, k], 1)
+    assert got.dtype == s.qkv.dtype and got.shape == want.shape and q.is_contiguous() and k.is_contiguous()
+    # Subnormal f16 results are off by half of the smallest step.
+    bound = HALF[got.dtype] * want.abs() + _slack(s, mag) + (2.0 ** -25 if got.dtype == F16 else 0.0)
+    assert bool(((got.double() - want).abs() <= bound).all()), float(((got.double() - want).abs() - bound).max())
+    assert t.equal(v.double(), values)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=IDS)
+def test_forward_against_float64(form):
+    s = _case(form)
+    _check_rows(s, *norm_rope(*cases.args(s)))
+
+
+@pytest.mark.parametrize("form", [FORMS[1], FORMS[2], FORMS[3], FORMS[10]])
+def test_strided_and_unaligned_rows(form):
+    s = _case(form)
+    n, width = s.qkv.shape
+    for pad, at in ((8, 8), (3, 1)):
+        wide = t.zeros(n, width + pad, dtype=s.qkv.dtype, device="cuda")
+        wide[:, at:at + width] = s.qkv
+        s.qkv = wide[:, at:at + width]
+        _check_rows(s, *norm_rope(*cases.args(s)))
+    s.qkv = s.qkv.t().contiguous().t()
+    _check_rows(s, *norm_rope(*cases.args(s)))
+    s.positions = s.positions.to(t.int32).repeat_interleave(2)[::2]
+    s.q_weight = s.q_weight.repeat_interleave(2)[::2]
+    s.cos = t.cat([s.cos, s.cos], 1)[:, :s.d // 2]
+    _check_rows(s, *norm_rope(*cases.args(s)))
+    s.qkv = s.qkv[:1].contiguous().expand(n, -1)               # the same row for every position
+    _check_rows(s, *norm_rope(*cases.args(s)))
+
+
+def test_no_rows():
+    s = _case((0, 4, 2, 64, BF16, F32, F32))
+    for x in (s.qkv, s.q_weight, s.k_weight):
+        x.requires_grad_(True)
+    q, k, v = norm_rope(*cases.args(s))
+    assert q.shape == (0, 4, 64) and k.shape == v.shape == (0, 2, 64)
+    dx, dq, dk = t.autograd.grad((q, k, v), (s.qkv, s.q_weight, s.k_weight), (q.detach(), k.detach(), v.detach()))
+    assert dx.shape == s.qkv.shape and not dq.any() and not dk.any()
+
+
+def test_not_a_number_and_infinite_rows():
+    """A head with NaN or an infinity gives NaN in that head alone; a head of zeros gives zeros."""
+    s = _case((6, 4, 2, 64, BF16, F32, F32), positions=t.arange(6))
+    clean = [x.clone() for x in norm_rope(*cases.args(s))]
+    s.qkv[1, 3] = t.nan
+    s.qkv[2, 64 + 5] = t.inf
+    s.qkv[3, 128:192] = 0.0
+    q, k, v = norm_rope(*cases.args(s))
+    assert bool(q[1, 0].isnan().all()) and bool(q[2, 1].isnan().any()) and not bool(q[3, 2].any())
+    for at in ((1, 0), (2, 1), (3, 2)):
+        q[at] = clean[0][at]
+    assert t.equal(q, clean[0]) and t.equal(k, clean[1]) and t.equal(v, clean[2])
+
+
+def _cache(s, dtype, page=8):
+    pool = -(-s.n // page) + 3
+    cache = PagedKVCache(pool, page, s.hkv, s.d, "cuda", dtype)
+    for x in (cache.k, cache.v):
+        x.view(t.uint8 if dtype == FP8 else dtype).fill_(5)
+    if cache.quantized:
+        cache.k_scales.fill_(7.0)
+        cache.v_scales.fill_(7.0)
+    places = t.randperm(pool * page, generator=t.Generator().manual_seed(s.n))[:s.n].cuda()
+    return cache, places // page, places % page
+
+
+def _check_cache(s, cache, blocks, offsets):
+    """k against float64, v against the write of append_kv, every other place as it was."""
+    want, mag, values = cases.forward_64(s)
+    want, mag = want[:, s.hq:], mag[:, s.hq:]
+    other = PagedKVCache(*cache.k.shape, "cuda", cache.cache_dtype)
+    for x, y in ((cache.k, other.k), (cache.v, other.v), (cache.k_scales, other.k_scales), (cache.v_scales, other.v_scales)):
+        if x is not None:
+            y.view(t.uint8 if x.dtype == FP8 else x.dtype).fill_(5 if x.ndim == 4 else 7)
+    other.append_kv(blocks, offsets, values.to(s.qkv.dtype), values.to(s.qkv.dtype))
+    bits = (lambda x: x.view(t.uint8)) if cache.quantized else (lambda x: x)
+    assert t.equal(bits(cache.v), bits(other.v))
+    inside = (blocks >= 0) & (blocks < len(cache.k)) & (offsets >= 0) & (offsets < cache.block_size)
+    blocks, offsets = blocks[inside], offsets[inside]
+    untouched = t.ones(cache.k.shape[:2], dtype=t.bool, device="cuda")
+    untouched[blocks, offsets] = False
+    assert bool((bits(cache.k)[untouched] == 5).all())
+    if cache.quantized:
+        assert t.equal(cache.v_scales, other.v_scales) and bool((cache.k_scales[untouched] == 7.0).all())
+        scale = cache.k_scales[blocks, offsets].double()
+        amax = want[inside].abs().amax(-1)
+        assert bool(((scale - amax / 448).abs() <= (2.0 ** -24 * amax + _slack(s, mag[inside].amax(-1))) / 448).all())
+        got = cache.k.view(t.uint8)[blocks, offsets].view(FP8).double() * scale[..., None]
+        # Half a step of e4m3: 2^-4 of the value, 2^-10 of the scale below its normal range.
+        bound = 2.0 ** -4 * want[inside].abs() + 2.0 ** -10 * scale[..., None] + 2 * _slack(s, mag[inside])
+    else:
+        got = cache.k[blocks, offsets].double()
+        bound = HALF[cache.k.dtype] * want[inside].abs() + _slack(s, mag[inside]) + (2.0 ** -25 if cache.k.dtype == F16 else 0.0)
+    assert bool(((got - want[inside]).abs() <= bound).all()), float(((got - want[inside]).abs() - bound).max())
+
+
+@pytest.mark.parametrize("cache_dtype", [FP8, BF16, F16, F32])
+@pytest.mark.parametrize("form", FORMS, ids=IDS)
+def test_append_against_float64(form, cache_dtype):
+    s = _case(form)
+    cache, blocks, offsets = _cache(s, cache_dtype)
+    q = norm_rope_append(*cases.args(s), cache, blocks, offsets.to(t.int32))
+    plain = norm_rope(*cases.args(s))
+    assert t.equal(q, plain[0])
+    _check_cache(s, cache, blocks, offsets)
+    again, blocks, offsets = _cache(s, cache_dtype)
+    packed = norm_rope_append(*cases.args(s), again, blocks, offsets, packed=True)
+    assert all(t.equal(a, b) for a, b in zip(packed, plain))
+    assert all(x is None or t.equal(x.view(t.uint8), y.view(t.uint8)) for x, y in ((cache.k, again.k), (cache.k_scales, again.k_scales)))
+
+
+def test_rows_outside_the_pool_are_skipped():
+    s = _case(FORMS[2])
+    cache, blocks, offsets = _cache(s, FP8)
+    blocks[3], blocks[5], offsets[7], offsets[8] = -1, len(cache.k), -2, 8
+    norm_rope_append(*cases.args(s), cache, blocks, offsets)
+    _check_cache(s, cache, blocks, offsets)
+
+
+def test_quantized_rows_of_zeros_and_not_a_number():
+    s = _case((4, 2, 1, 64, BF16, F32, F32))
+    s.qkv[1, 128:192] = 0.0
+    s.qkv[2, 130] = t.nan
+    cache, blocks, offsets = _cache(s, FP8)
+    norm_rope_append(*cases.args(s), cache, blocks, offsets)
+    assert float(cache.k_scales[blocks[1], offsets[1], 0]) == 1.0 and not bool(cache.k[blocks[1], offsets[1]].float().any())
+    assert bool(cache.k[blocks[2], offsets[2]].float().isnan().all())
+
+
+def test_rotation_alone_writes_what_append_kv_writes_of_float32_rows():
+    """Without weights and in float32 the cache holds the codes of the rotated rows that norm_rope returns."""
+    s = _case((40, 4, 2, 128, F32, None, F32))
+    cache, blocks, offsets = _cache(s, FP8)
+    _, k, v = norm_rope_append(*cases.args(s), cache, blocks, offsets, packed=True)
+    other, _, _ = _cache(s, FP8)
+    other.append_kv(blocks, offsets, k, v)
+    assert t.equal(cache.k.view(t.uint8), other.k.view(t.uint8)) and t.equal(cache.k_scales, other.k_scales)
+
+
+def _check_grads(s, grads, got):
+    dx, mag, sums = cases.backward_64(s, grads)
+    tiny = 2.0 ** -25 if s.qkv.dtype == F16 else 0.0
+    # Two sums of D terms and about 16 more operations of float32.
+    bound = HALF[s.qkv.dtype] * dx.abs() + (2 * s.d + 32) * 2.0 ** -24 * mag + tiny
+    assert got[0].dtype == s.qkv.dtype and bool(((got[0].double() - dx).abs() <= bound).all())
+    if sums is None:
+        return
+    for y, (want, size), heads in zip(got[1:], sums, (s.hq, s.hkv)):
+        # A term as above, then a sum of rows x heads terms, at most as many half steps.
+        bound = HALF[y.dtype] * want.abs() + (s.d / 2 + 32 + s.n * heads) * 2.0 ** -24 * size + (2.0 ** -25 if y.dtype == F16 else 0.0)
+        assert y.dtype == s.q_weight.dtype and bool(((y.double() - want).abs() <= bound).all())
+
+
+def _leaves(s):
+    return [x.requires_grad_(True) for x in (s.qkv, s.q_weight, s.k_weight) if x is not None]
+
+
+@pytest.mark.parametrize("form", FORMS, ids=IDS)
+def test_gradients_against_float64(form):
+    s = _case(form)
+    leaves = _leaves(s)
+    got = t.autograd.grad(norm_rope(*cases.args(s)), leaves, s.grads)
+    _check_grads(s, s.grads, [x for x in got])
+    again = t.autograd.grad(norm_rope(*cases.args(s)), leaves, s.grads)
+    assert all(t.equal(a, b) for a, b in zip(got, again))       # sums in a fixed order
+
+
+def test_gradients_of_parts():
+    """Outputs that nothing depends on, leaves that want no gradient, gradients of other strides."""
+    s = _case(FORMS[2])
+    leaves = _leaves(s)
+    q, k, v = norm_rope(*cases.args(s))
+    _check_grads(s, [s.grads[0], None, None], t.autograd.grad(q, leaves, s.grads[0], retain_graph=True))
+    _check_grads(s, [None, None, s.grads[2]], t.autograd.grad(v, leaves, s.grads[2], retain_graph=True))
+    strided = [g.transpose(0, 1).contiguous().transpose(0, 1) for g in s.grads]
+    full = t.autograd.grad((q, k, v), leaves, strided, retain_graph=True)
+    expanded = t.ones(1, device="cuda", dtype=q.dtype).expand(s.n, s.hq, s.d)
+    _check_grads(s, [expanded, None, None], t.autograd.grad(q, leaves, expanded, retain_graph=True))
+    _check_grads(s, s.grads, full)
+    assert t.equal(t.autograd.grad((q, k, v), [s.k_weight], s.grads)[0], full[2])
+    for i in range(3):
+        s = _case(FORMS[2])
+        x = (s.qkv, s.q_weight, s.k_weight)[i].requires_grad_(True)
+        assert t.equal(t.autograd.grad(norm_rope(*cases.args(s)), x, s.grads)[0], full[i])
+
+
+def test_strided_rows_have_gradients_of_their_own():
+    s = _case(FORMS[1])
+    wide = t.zeros(s.n, s.qkv.shape[1] + 16, dtype=s.qkv.dtype, device="cuda")
+    wide[:, 8:-8] = s.qkv
+    wide.requires_grad_(True)
+    s.qkv = wide[:, 8:-8]
+    got = t.autograd.grad(norm_rope(*cases.args(s)), wide, s.grads)[0]
+    assert not bool(got[:, :8].any()) and not bool(got[:, -8:].any())
+    _check_grads(SimpleNamespace(**{**vars(s), "q_weight": s.q_weight}), s.grads, [got[:, 8:-8]])
+
+
+def test_transforms_and_second_derivatives_of_the_plain_operations():
+    s = _case((5, 2, 1, 16, F32, F32, F32))
+    fixed = cases.args(s)[1:6]
+
+    def out(qkv, qw, kw):
+        return t.cat([x.flatten(1) for x in norm_rope(qkv, *fixed, qw, kw, s.eps)], 1)
+
+    given = (s.qkv, s.q_weight, s.k_weight)
+    up = t.cat([g.flatten(1) for g in s.grads], 1)
+    _, pull = t.func.vjp(out, *given)
+    for a, b in zip(pull(up), t.autograd.grad(out(*_leaves(s)), _leaves(s), up)):
+        t.testing.assert_close(a, b, rtol=1e-5, atol=1e-5)
+    batched = t.func.vmap(lambda x: out(x, s.q_weight.detach(), s.k_weight.detach()))(t.stack([s.qkv.detach(), 2 * s.qkv.detach()]))
+    t.testing.assert_close(batched[1], out(2 * s.qkv.detach(), s.q_weight.detach(), s.k_weight.detach()), rtol=1e-5, atol=1e-5)
+    ups = t.stack([up, 3 * up])
+    got = t.autograd.grad(out(*_leaves(s)), _leaves(s), ups, is_grads_batched=True)
+    t.testing.assert_close(got[0][1], 3 * got[0][0], rtol=1e-5, atol=1e-5)
+
+
+def test_captured_and_replayed():
+    """Forward, cache write and gradients in one graph, replayed over changed inputs beside eager work."""
+    s = _case(FORMS[1])
+    cache, blocks, offsets = _cache(s, FP8)
+    s.qkv = s.qkv.clone()
+
+    def step():
+        x = s.qkv.detach().requires_grad_(True)
+        w = [y.detach().requires_grad_(True) for y in (s.q_weight, s.k_weight)]
+        outs = norm_rope(x, *cases.args(s)[1:6], *w, s.eps)
+        q = norm_rope_append(s.qkv, *cases.args(s)[1:], cache, blocks, offsets)
+        return [q, *outs, *t.autograd.grad(outs, (x, *w), s.grads)]
+
+    side = t.cuda.Stream()
+    side.wait_stream(t.cuda.current_stream())
+    with t.cuda.stream(side):
+        step()
+    t.cuda.current_stream().wait_stream(side)
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        held = step()
+    for i in range(3):
+        s.qkv.copy_(_case(FORMS[1], seed=i + 1).qkv)
+        s.positions.copy_(_case(FORMS[1], seed=i + 1).positions)
+        graph.replay()
+        got = [x.detach().clone() for x in held]
+        codes = cache.k.view(t.uint8).clone()
+        cache.k.view(t.uint8).fill_(5)
+        want = step()
+        assert all(t.equal(a, b) for a, b in zip(got, want)) and t.equal(codes, cache.k.view(t.uint8))
+        t.cuda.synchronize()
+
+
+def test_on_another_stream():
+    s = _case(FORMS[12])
+    want = norm_rope(*cases.args(s))
+    side = t.cuda.Stream()
+    side.wait_stream(t.cuda.current_stream())
+    with t.cuda.stream(side):
+        got = norm_rope(*cases.args(s))
+    t.cuda.current_stream().wait_stream(side)
+    assert all(t.equal(a, b) for a, b in zip(got, want))

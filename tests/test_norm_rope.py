@@ -1,0 +1,130 @@
+"""Normed and rotated heads without a GPU: refusals of the calls and of the C entries, and the operations in PyTorch."""
+
+import pytest
+import torch as t
+
+from aiproj_amd import _native
+from aiproj_amd.kernals import norm_rope as module
+from aiproj_amd.kernals.norm_rope import norm_rope, norm_rope_append
+from tests import norm_rope_cases as cases
+
+F32, BF16, I32, I64, FP8 = _native.F32, _native.BF16, _native.I32, _native.I64, _native.E4M3FN
+SOME = 4096          # an address that a refused call does not look at
+
+
+def _changed(s, **more):
+    for name, x in more.items():
+        setattr(s, name, x)
+    return s
+
+
+@pytest.mark.parametrize("change", [
+    dict(qkv=t.zeros(4, 3, 16)), dict(qkv=t.zeros(4, 65)), dict(qkv=t.zeros(4, 0)), dict(qkv=t.zeros(4, 64, dtype=t.float64)),
+    dict(positions=t.zeros(3, dtype=t.int64)), dict(positions=t.zeros(4)), dict(cos=t.zeros(9, 7)), dict(cos=t.zeros(0, 8)),
+    dict(sin=t.zeros(200, 8, dtype=t.float16)), dict(hq=0), dict(hkv=-1), dict(q_weight=None), dict(k_weight=t.ones(15)),
+    dict(q_weight=t.ones(16, dtype=t.int32)), dict(k_weight=t.ones(16, dtype=t.float16)), dict(qkv=t.zeros(4, 4 * 514)),
+    dict(qkv=t.zeros(4, 4 * 15))])
+def test_refused_arguments(change):
+    s = _changed(cases.rows(4, 2, 1, 16, t.float32, t.float32, device="cpu"), **change)
+    with pytest.raises(ValueError):
+        norm_rope(*cases.args(s))
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(RuntimeError, match="GPU"):
+        norm_rope(*cases.args(cases.rows(4, 2, 1, 16, t.float32, t.float32, device="cpu")))
+
+
+class Cache:
+    def __init__(self, shape=(3, 4, 1, 16), dtype=t.float8_e4m3fn, quantized=True):
+        self.k, self.v = t.empty(shape, dtype=dtype), t.empty(shape, dtype=dtype)
+        self.quantized, self.block_size = quantized, shape[1]
+        self.k_scales, self.v_scales = (t.empty(shape[:3]) for _ in range(2)) if quantized else (None, None)
+
+
+@pytest.mark.parametrize("cache,blocks", [
+    (Cache((3, 4, 2, 16)), t.zeros(4, dtype=t.int64)), (Cache((3, 4, 1, 18)), t.zeros(4, dtype=t.int64)),
+    (Cache(), t.zeros(3, dtype=t.int64)), (Cache(), t.zeros(4)), (Cache(dtype=t.float16), t.zeros(4, dtype=t.int64)),
+    (Cache(quantized=False), t.zeros(4, dtype=t.int64)), (Cache(dtype=t.float64, quantized=False), t.zeros(4, dtype=t.int64))])
+def test_refused_caches(cache, blocks):
+    s = cases.rows(4, 2, 1, 16, t.float32, t.float32, device="cpu")
+    with pytest.raises(ValueError):
+        norm_rope_append(*cases.args(s), cache, blocks, blocks)
+
+
+def test_strided_caches_are_refused():
+    s, cache = cases.rows(4, 2, 1, 16, t.float32, t.float32, device="cpu"), Cache()
+    cache.v_scales = t.empty(3, 4, 2)[:, :, :1]
+    with pytest.raises(ValueError, match="contiguous"):
+        norm_rope_append(*cases.args(s), cache, t.zeros(4, dtype=t.int64), t.zeros(4, dtype=t.int64))
+
+
+def _entry(rows=4, hq=2, hkv=1, d=16, stride=64, dtype=F32, pos=I64, table=F32, table_rows=9, qw=SOME, kw=SOME, wd=F32, x=SOME):
+    return (x, dtype, rows, hq, hkv, d, stride, SOME, pos, SOME, SOME, table, table_rows, qw, kw, wd, 1e-5)
+
+
+NO_CACHE = (None, I64, None, I64, 0, 0, None, None, FP8, None, None, None)
+
+
+@pytest.mark.parametrize("more,code", [
+    (dict(dtype=FP8), -1), (dict(pos=F32), -1), (dict(table=I32), -1), (dict(wd=FP8), -1), (dict(rows=-1), -2), (dict(hq=0), -2),
+    (dict(hkv=0), -2), (dict(d=0), -2), (dict(d=15), -2), (dict(table_rows=0), -2), (dict(stride=-64), -3), (dict(qw=None), -4),
+    (dict(x=None), -4), (dict(d=514), -6), (dict(rows=2 ** 62), -6), (dict(rows=2 ** 29), -6),
+    (dict(hq=2 ** 31 - 1, hkv=2 ** 31 - 1), -6), (dict(rows=2 ** 63 - 1, hq=2 ** 23), -6)])
+def test_entries_refuse(more, code):
+    for lib in (_native.lib().kvfp8_norm_rope, _native.fn("kvfp8_norm_rope")):
+        assert lib(*_entry(**more), SOME, SOME, SOME, *NO_CACHE) == code
+    for lib in (_native.lib().kvfp8_norm_rope_backward, _native.fn("kvfp8_norm_rope_backward")):
+        assert lib(*_entry(**more), SOME, SOME, SOME, SOME, SOME, SOME, SOME, 1 << 40, None) == code
+
+
+def test_entries_refuse_caches_and_workspaces():
+    forward, backward = _native.lib().kvfp8_norm_rope, _native.lib().kvfp8_norm_rope_backward
+
+    def cached(blocks=SOME, bd=I64, offsets=SOME, od=I32, pool=3, page=4, k=SOME, v=SOME, cd=FP8, ks=SOME, vs=SOME, outs=(SOME, None, None)):
+        return forward(*_entry(), *outs, blocks, bd, offsets, od, pool, page, k, v, cd, ks, vs, None)
+
+    assert cached(bd=F32) == cached(od=FP8) == cached(cd=I32) == -1
+    assert cached(pool=0) == cached(page=-1) == -2
+    assert cached(blocks=None) == cached(offsets=None) == cached(k=None) == cached(vs=None) == -4
+    assert cached(outs=(None, None, None)) == cached(outs=(SOME, SOME, None)) == -4
+    assert forward(*_entry(), SOME, None, None, *NO_CACHE) == -4
+    need = _native.lib().kvfp8_norm_rope_backward_workspace_bytes(4, 2, 1, 16)
+    assert need > 0
+    assert backward(*_entry(), SOME, SOME, SOME, SOME, SOME, SOME, SOME, need - 1, None) == -5
+    assert backward(*_entry(), SOME, SOME, SOME, SOME, SOME, SOME, None, need, None) == -4
+    assert backward(*_entry(qw=None, kw=None), SOME, SOME, SOME, SOME, SOME, None, SOME, need, None) == -4
+
+
+@pytest.mark.parametrize("sizes", [(0, 2, 1, 16), (-1, 2, 1, 16), (4, 0, 1, 16), (2 ** 62, 2, 1, 16), (4, 2, 1, 600),
+                                   (2 ** 63 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 512)])
+def test_workspace_of_sizes_that_are_refused(sizes):
+    assert _native.lib().kvfp8_norm_rope_backward_workspace_bytes(*sizes) == 0
+
+
+@pytest.mark.parametrize("weights", [t.float32, None])
+def test_plain_operations_and_the_gradient_formula(weights):
+    """The operations that transforms take, against the formulas in float64 and against differences."""
+    s = cases.rows(7, 3, 2, 10, t.float32, weights, device="cpu")
+    q, k, v = module._plain(*cases.args(s)[:6], s.d, s.q_weight, s.k_weight, s.eps)
+    want, mag, values = cases.forward_64(s)
+    # 10 squares and their sum, root, quotient and two products, three roundings of the rotation: 32 half steps cover them.
+    assert bool(((t.cat([q, k], 1).double() - want).abs() <= 32 * 2.0 ** -24 * mag).all()) and t.equal(v.double(), values)
+    dx, _, dw = cases.backward_64(s, s.grads)
+    leaves = [None if x is None else x.double().requires_grad_(True) for x in (s.qkv, s.q_weight, s.k_weight)]
+
+    def loss(qkv, qw, kw):
+        y, _, z = cases.forward_64(_changed(cases.rows(7, 3, 2, 10, t.float32, weights, device="cpu"), qkv=qkv, q_weight=qw, k_weight=kw))
+        return (y * t.cat(s.grads[:2], 1).double()).sum() + (z * s.grads[2].double()).sum()
+
+    step = 1e-6
+    for i, want in enumerate([dx] + ([] if dw is None else [g for g, _ in dw])):
+        flat = leaves[i].detach().flatten()
+        for j in range(0, flat.numel(), 7):
+            moved = []
+            for sign in (1, -1):
+                x = flat.clone()
+                x[j] += sign * step
+                moved.append(loss(*(x.view(y.shape) if n == i else y for n, y in enumerate(leaves))).detach())
+            # Central differences of 1e-6: 64-bit sums of 100 magnitude give 1e-8, curvature less.
+            assert abs(float((moved[0] - moved[1]) / (2 * step)) - float(want.flatten()[j])) < 1e-6
