@@ -79,6 +79,12 @@ SIGNATURES = {
                                                                    _I64, _P]),
     "kvfp8_token_logprobs": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _INT, _I32, _P, _P, _P, _P, _P, _P]),
     "kvfp8_token_logprobs_backward": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _INT, _P, _P, _P, _P, _P, _P]),
+    "kvfp8_tree_attention_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32, _INT]),
+    "kvfp8_tree_attention": (_INT, [_P, _INT, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _INT, _P, _P, _I64, _I32, _P, _I64,
+                                    _I64, _P, _INT, _P, _INT, _P, _INT, _P, _INT, _I32, _I32, ctypes.c_float, _P, _P, _I64,
+                                    _P]),
+    "kvfp8_accept_draft": (_INT, [_P, _INT, _P, _INT, _P, _INT, _P, _INT, _I64, _I32, _I32, _P, _INT, _P, _INT, _P, _I64, _I64,
+                                  _I64, _I32, _P, _I32, _I64, _I64, _P, _P, _P, _P]),
     "kvfp8_norm_rope": (_INT, _NORM_ROPE_ARGS + [_P, _P, _P, _P, _INT, _P, _INT, _I64, _I32, _P, _P, _INT, _P, _P, _P]),
     "kvfp8_norm_rope_backward_workspace_bytes": (_I64, [_I64, _I32, _I32, _I32]),
     "kvfp8_norm_rope_backward": (_INT, _NORM_ROPE_ARGS + [_P, _P, _P, _P, _P, _P, _P, _I64, _P]),

@@ -1,0 +1,252 @@
+// Shared pieces of the draft-tree kernels: arguments, a sequence's nodes and tokens, which nodes are above which, and how a
+// batch is cut into work items on the device.
+#pragma once
+
+#include "paged_operands.h"
+#include "kvfp8_decode_common.h"
+
+namespace kvfp8 {
+
+constexpr int kMaxNodes = 256;        // of a sequence
+constexpr int kNodeWords = kMaxNodes / 32;
+
+// Rows of q are the drafted nodes, packed: sequence b has rows [starts[b], starts[b + 1]), of which the first max_nodes are
+// computed. d.slots and d.ctx: its block-table row, and its tokens in the cache with the nodes as the last ones.
+struct TreeArgs {
+    DecodeArgs d;
+    int64_t rows;
+    const void* starts;
+    const void* parents;
+    int32_t starts64, parents64;
+    int32_t seqs, max_nodes;
+    int32_t block_rows;               // (node, q head) pairs of a KV head in a row block
+    int32_t target;                   // items that run at once
+    int32_t least_steps;              // of a chunk, in steps of kStep tokens
+    int32_t q_vec;                    // q rows are 16-byte aligned
+};
+
+namespace {
+
+constexpr int kStep = 64;             // chunks hold whole steps
+constexpr int kXcdCount = 8;          // workgroups are dispatched round-robin over the XCDs
+
+struct TreeSeq {
+    int32_t row0, nodes;              // first row, computed nodes
+    int32_t tokens;                   // in the cache, as far as the block table addresses them
+    int32_t held;                     // tokens before the nodes
+    int64_t slot;
+};
+
+__device__ __forceinline__ int64_t tree_row(const TreeArgs& a, int64_t i) {
+    const int64_t x = load_i(a.starts, a.starts64, i);
+    return x < 0 ? 0 : (x > a.rows ? a.rows : x);
+}
+
+// Sequence b. A slot outside the table, or fewer tokens than nodes: no tokens.
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
+    TreeSeq s;
+    const int64_t r0 = tree_row(a, b), r1 = tree_row(a, b + 1), len = load_i(a.d.ctx, a.d.ctx64, b);
+    const int64_t nodes = r1 > r0 ? r1 - r0 : 0, cap = a.d.bt_width * a.d.block_size;
+    s.slot = load_i(a.d.slots, a.d.slots64, b);
+    const bool ok = s.slot >= 0 && s.slot < a.d.bt_rows && len >= nodes;
+    s.row0 = (int32_t)r0;
+    s.nodes = (int32_t)(nodes < a.max_nodes ? nodes : a.max_nodes);
+    s.tokens = (int32_t)(ok ? (len < cap ? len : cap) : 0);
+    s.held = (int32_t)(ok ? (len - nodes < cap ? len - nodes : cap) : 0);
+    return s;
+}
+
+// Which nodes are above which, as bits: node i sees the nodes of words[i]. Whole workgroup, at least kMaxNodes threads. A
+// node's parent is a node before it; any other number makes it a root. Nodes above are found in rounds, each of which
+// doubles how far up they are known, as many as the deepest needs.
+struct TreeMasks {
+    uint32_t words[kMaxNodes][kNodeWords + 1];           // (an odd stride: rows in different banks; the last word is 0)
+    int32_t up[kMaxNodes];
+};
+
+__device__ __forceinline__ void build_masks(TreeMasks& m, const TreeArgs& a, const TreeSeq& s) {
+    const int i = threadIdx.x;
+    const bool mine = i < s.nodes;
+    if (mine) {
+        const int64_t p = load_i(a.parents, a.parents64, (int64_t)s.row0 + i);
+        m.up[i] = p >= 0 && p < i ? (int32_t)p : -1;
+#pragma unroll
+        for (int w = 0; w <= kNodeWords; ++w) m.words[i][w] = w == i / 32 ? 1u << (i & 31) : 0u;
+    }
+    __syncthreads();
+    for (;;) {
+        const int up = mine ? m.up[i] : -1;
+        uint32_t more[kNodeWords];
+        int next = -1;
+        if (up >= 0) {
+#pragma unroll
+            for (int w = 0; w < kNodeWords; ++w) more[w] = m.words[up][w];
+            next = m.up[up];
+        }
+        if (!__syncthreads_or(up >= 0)) break;           // a node's root is reached in at most 8 rounds
+        if (up >= 0) {
+#pragma unroll
+            for (int w = 0; w < kNodeWords; ++w) m.words[i][w] |= more[w];
+            m.up[i] = next;
+        }
+        __syncthreads();
+    }
+}
+
+// Bit t: token `first` + t counts for node i (t < 32; first and held are wave-uniform).
+__device__ __forceinline__ uint32_t node_bits(const TreeMasks& m, int i, int32_t first, int32_t held) {
+    const int32_t at = first - held;
+    if (at <= -32) return ~0u;
+    if (at < 0) return (m.words[i][0] << -at) | ((1u << -at) - 1u);
+    const int w = at >> 5;
+    if (w >= kNodeWords) return 0u;
+    return (uint32_t)((((uint64_t)m.words[i][w + 1] << 32) | m.words[i][w]) >> (at & 31));
+}
+
+// How a batch is cut. A sequence has columns (row block, KV head) and steps of kStep tokens; a chunk is `chunk` steps of a
+// column. Items are numbered sequence by sequence, in a sequence chunk by chunk, in a chunk head by head: the row blocks
+// that read the same tokens are neighbours.
+struct TreeCut {
+    TreeSeq s;                        // lane's of the first 64 sequences
+    int32_t chunk;                    // steps of a chunk
+    int32_t total;                    // items
+};
+struct TreeItem {
+    TreeSeq s;
+    int32_t first;                    // number of the sequence's first item
+    int32_t blocks;                   // row blocks of the sequence
+    int32_t chunks;                   // of its columns
+};
+
+template <typename T>
+__device__ __forceinline__ T wave_sum(T x) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off);
+    return x;
+}
+
+__device__ __forceinline__ TreeSeq lane_seq(const TreeArgs& a, int b0) {
+    const int b = b0 + (threadIdx.x & 63);
+    TreeSeq s = tree_seq(a, min(b, a.seqs - 1));
+    if (b >= a.seqs) s.nodes = s.tokens = 0;
+    return s;
+}
+__device__ __forceinline__ int32_t tree_blocks(const TreeArgs& a, const TreeSeq& s) {
+    const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
+    return s.tokens > 0 ? (int32_t)((uint32_t)(s.nodes * G + a.block_rows - 1) / (uint32_t)a.block_rows) : 0;
+}
+__device__ __forceinline__ int32_t tree_chunks(const TreeSeq& s, int32_t chunk) {
+    return (int32_t)((uint32_t)((s.tokens + kStep - 1) / kStep + chunk - 1) / (uint32_t)chunk);
+}
+
+// A wave looks through 64 sequences at once, each in its lane; every wave of the call finds the same. Chunks are as short
+// as the work divided by the items that run at once, and up to 1.5 times that while there are more items than those (up to
+// 64 sequences).
+__device__ __forceinline__ TreeCut cut_batch(const TreeArgs& a) {
+    TreeCut c;
+    c.s = lane_seq(a, 0);
+    unsigned long long work = 0;
+    TreeSeq s = c.s;
+    for (int b0 = 0;;) {
+        work += (unsigned long long)tree_blocks(a, s) * (uint32_t)(tree_chunks(s, 1));
+        b0 += 64;
+        if (b0 >= a.seqs) break;
+        s = lane_seq(a, b0);
+    }
+    work = wave_sum(work) * (uint32_t)a.d.num_kv_heads;
+    const uint64_t even = (work + a.target - 1) / (uint32_t)a.target;
+    // (Never more than a table's 2^25 steps.)
+    const int32_t least = (int32_t)(even < (uint64_t)a.least_steps ? a.least_steps : (even < (1ull << 25) ? even : 1ull << 25));
+    auto items = [&](int32_t chunk) __attribute__((always_inline)) {
+        int32_t n = 0;
+        TreeSeq s = c.s;
+        for (int b0 = 0;;) {
+            n += tree_blocks(a, s) * tree_chunks(s, chunk);
+            b0 += 64;
+            if (b0 >= a.seqs) break;
+            s = lane_seq(a, b0);
+        }
+        return wave_sum(n) * a.d.num_kv_heads;
+    };
+    c.chunk = least;
+    c.total = items(least);
+    if (a.seqs <= 64 && c.total > a.target) {
+        for (int i = 1; i <= 8; ++i) {
+            const int32_t chunk = least + (least * i + 15) / 16, n = items(chunk);
+            if (n > a.target) continue;
+            c.chunk = chunk;
+            c.total = n;
+            break;
+        }
+    }
+    return c;
+}
+
+// The sequence that holds item `index` (kByRow: that computes row `index`); false without one.
+template <bool kByRow>
+__device__ __forceinline__ bool find_tree_item(const TreeArgs& a, const TreeCut& c, int32_t index, TreeItem& it) {
+    const int lane = threadIdx.x & 63;
+    int32_t before = 0;
+    TreeSeq s = c.s;
+    for (int b0 = 0;;) {
+        const int32_t blocks = tree_blocks(a, s), chunks = tree_chunks(s, c.chunk), items = blocks * a.d.num_kv_heads * chunks;
+        int32_t incl = items;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int32_t y = __shfl_up(incl, off);
+            if (lane >= off) incl += y;
+        }
+        const int32_t first = before + incl - items;
+        const uint64_t hit = __ballot(kByRow ? index >= s.row0 && index - s.row0 < s.nodes : index >= first && index - first < items);
+        if (hit != 0) {
+            const int at = __builtin_ctzll(hit);
+            it.s.row0 = __builtin_amdgcn_readlane(s.row0, at);
+            it.s.nodes = __builtin_amdgcn_readlane(s.nodes, at);
+            it.s.tokens = __builtin_amdgcn_readlane(s.tokens, at);
+            it.s.held = __builtin_amdgcn_readlane(s.held, at);
+            it.s.slot = __builtin_amdgcn_readlane((int32_t)s.slot, at);    // of a table of less than 2^31 rows, where there are tokens
+            it.blocks = __builtin_amdgcn_readlane(blocks, at);
+            it.chunks = __builtin_amdgcn_readlane(chunks, at);
+            it.first = __builtin_amdgcn_readlane(first, at);
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(incl, 63);
+        b0 += 64;
+        if (b0 >= a.seqs) return false;
+        s = lane_seq(a, b0);
+    }
+}
+
+// What a workgroup does: pairs (node, q head of KV head h) from r0 on against the tokens [lo, hi).
+struct TreeWork {
+    TreeItem it;
+    int32_t index;                    // of the item
+    int32_t h, r0, pairs, lo, hi;
+    const int32_t* table;             // block-table row
+};
+
+// The item of this workgroup; false without one. Each XCD takes one run of items, so that row blocks meet their tokens in
+// the same L2.
+__device__ __forceinline__ bool tree_work(const TreeArgs& a, TreeWork& w) {
+    const TreeCut c = cut_batch(a);
+    const int32_t total = uniform(c.total), per_xcd = (total + kXcdCount - 1) / kXcdCount;
+    const int32_t xcd = (int32_t)(blockIdx.x % kXcdCount), local = (int32_t)(blockIdx.x / kXcdCount);
+    w.index = xcd * per_xcd + local;
+    if (local >= per_xcd || w.index >= total || !find_tree_item<false>(a, c, w.index, w.it)) return false;
+    const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
+    uint32_t rest = (uint32_t)(w.index - w.it.first);
+    const uint32_t column = rest / (uint32_t)w.it.blocks;
+    w.r0 = (int32_t)(rest - column * (uint32_t)w.it.blocks) * a.block_rows;
+    rest = column / (uint32_t)a.d.num_kv_heads;
+    w.h = (int32_t)(column - rest * (uint32_t)a.d.num_kv_heads);
+    w.pairs = w.it.s.nodes * G;
+    const int64_t per = (int64_t)uniform(c.chunk) * kStep, lo = rest * per;
+    w.lo = uniform((int32_t)lo);
+    w.hi = uniform((int32_t)min(lo + per, (int64_t)w.it.s.tokens));
+    w.table = a.d.block_table + uniform64(w.it.s.slot) * a.d.bt_width;
+    return true;
+}
+
+}  // namespace
+
+}  // namespace kvfp8

@@ -205,6 +205,38 @@ static PyObject* py_kvfp8_norm_rope_backward(PyObject* self, PyObject* const* ar
     return PyLong_FromLong(rc);
 }
 
+/* kvfp8_tree_attention: 33 arguments, the scale at 28. */
+static PyObject* py_kvfp8_tree_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+    (void)self;
+    int64_t iv[33];
+    float scale = 0.0f;
+    if (!parse(args, nargs, 33, 28, iv, &scale, "kvfp8_tree_attention")) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = kvfp8_tree_attention(PTR(0), (int)iv[1], iv[2], iv[3], iv[4], (int32_t)iv[5], (int32_t)iv[6], (int32_t)iv[7], PTR(8),
+                              PTR(9), (int)iv[10], (const float*)PTR(11), (const float*)PTR(12), iv[13], (int32_t)iv[14],
+                              (const int32_t*)PTR(15), iv[16], iv[17], PTR(18), (int)iv[19], PTR(20), (int)iv[21], PTR(22),
+                              (int)iv[23], PTR(24), (int)iv[25], (int32_t)iv[26], (int32_t)iv[27], scale, PTR(29), PTR(30),
+                              iv[31], PTR(32));
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+/* kvfp8_accept_draft: 28 arguments. */
+static PyObject* py_kvfp8_accept_draft(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+    (void)self;
+    int64_t iv[28];
+    if (!parse(args, nargs, 28, -1, iv, NULL, "kvfp8_accept_draft")) return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = kvfp8_accept_draft(PTR(0), (int)iv[1], PTR(2), (int)iv[3], PTR(4), (int)iv[5], PTR(6), (int)iv[7], iv[8],
+                            (int32_t)iv[9], (int32_t)iv[10], PTR(11), (int)iv[12], PTR(13), (int)iv[14],
+                            (const int32_t*)PTR(15), iv[16], iv[17], iv[18], (int32_t)iv[19], (void* const*)PTR(20),
+                            (int32_t)iv[21], iv[22], iv[23], (int32_t*)PTR(24), (int32_t*)PTR(25), (int64_t*)PTR(26), PTR(27));
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
 static PyMethodDef methods[] = {
     {"kvfp8_paged_decode", (PyCFunction)(void (*)(void))py_kvfp8_paged_decode, METH_FASTCALL, NULL},
     {"kvfp8_paged_decode_split", (PyCFunction)(void (*)(void))py_kvfp8_paged_decode_split, METH_FASTCALL, NULL},
@@ -218,6 +250,8 @@ static PyMethodDef methods[] = {
     {"kvfp8_token_logprobs_backward", (PyCFunction)(void (*)(void))py_kvfp8_token_logprobs_backward, METH_FASTCALL, NULL},
     {"kvfp8_norm_rope", (PyCFunction)(void (*)(void))py_kvfp8_norm_rope, METH_FASTCALL, NULL},
     {"kvfp8_norm_rope_backward", (PyCFunction)(void (*)(void))py_kvfp8_norm_rope_backward, METH_FASTCALL, NULL},
+    {"kvfp8_tree_attention", (PyCFunction)(void (*)(void))py_kvfp8_tree_attention, METH_FASTCALL, NULL},
+    {"kvfp8_accept_draft", (PyCFunction)(void (*)(void))py_kvfp8_accept_draft, METH_FASTCALL, NULL},
     {NULL, NULL, 0, NULL},
 };
 

@@ -101,11 +101,26 @@ struct RowState {
     float m, l;                       // maximum; this lane's share of the sum
 };
 
-// kFull: all 32 tokens count. Else the first lim_a of tile A and lim_b of tile B do.
-template <int C, int QT, int ES, bool kFull>
+// Which tokens of a step count, of token i = 0..7 of a lane: token 4 (l / 16) + i % 4 of tile i / 4. Here the first lim_a of
+// tile A and lim_b of tile B, for every row.
+struct FirstTokens {
+    int j, lim_a, lim_b;              // j: l / 16
+    static constexpr bool kByRow = false;
+    __device__ __forceinline__ bool row(int i) const { return held(i); }        // for the lane's row
+    __device__ __forceinline__ bool held(int i) const { return 4 * j + (i & 3) < (i < 4 ? lim_a : lim_b); }   // for any row
+};
+
+// What takes the place of the products with V where tokens count for some of the rows only (0 times a value that is not
+// finite would reach the others).
+struct MatrixProducts {};
+
+// kFull: all 32 tokens count. Else those that `counts` says do. `products`: MatrixProducts, or with counts by row what says
+// whether a step's V fits them and adds it otherwise.
+template <int C, int QT, int ES, bool kFull, typename Counts, typename Products = MatrixProducts>
 __device__ __forceinline__ void prefix_step(RowState<C>& st, const PrefixStep<C, ES>& s,
                                             const OpT<Kinds<QT, ES>::kF16> (&q)[Kinds<QT, ES>::kQParts][2 * C],
-                                            float4* stage, int lane, int lim_a, int lim_b, float score_scale) {
+                                            float4* stage, int lane, const Counts& counts, float score_scale,
+                                            const Products& products = Products{}) {
     using K = Kinds<QT, ES>;
     constexpr int VW = C * ES, NB = 4 * C;
     const int j = lane >> 4;
@@ -149,7 +164,7 @@ __device__ __forceinline__ void prefix_step(RowState<C>& st, const PrefixStep<C,
     float sc[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        live[i] = kFull || 4 * j + (i & 3) < (i < 4 ? lim_a : lim_b);
+        live[i] = kFull || counts.row(i);
         const float x = (i < 4 ? sa[i & 3] : sb[i & 3]) * ks[i];
         sc[i] = live[i] ? x : kNegInf;
     }
@@ -166,11 +181,13 @@ __device__ __forceinline__ void prefix_step(RowState<C>& st, const PrefixStep<C,
     }
     st.m = m_new;
     OpT<K::kF16V> pp[K::kPParts];
+    float weight[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float p = fast_exp2(sc[i] - m_use);
         st.l += p;
         float x = live[i] ? p * vs[i] : 0.0f;            // a stale scale may be NaN
+        weight[i] = x;
 #pragma unroll
         for (int part = 0; part < K::kPParts; ++part) {
             const OpE<K::kF16V> hi = (OpE<K::kF16V>)x;
@@ -183,7 +200,13 @@ __device__ __forceinline__ void prefix_step(RowState<C>& st, const PrefixStep<C,
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int w = 0; w < VW; ++w) vr[i][w] = live[i] ? s.v[i][w] : 0u;
+        for (int w = 0; w < VW; ++w) vr[i][w] = kFull || counts.held(i) ? s.v[i][w] : 0u;
+    if constexpr (!kFull && Counts::kByRow) {
+        if (!products.fits(vr)) {                        // wave-uniform
+            products.add(st, weight, live);
+            return;
+        }
+    }
     auto product = [&](OpT<K::kF16V> av, int nb) __attribute__((always_inline)) {
 #pragma unroll
         for (int part = 0; part < K::kPParts; ++part) st.o[nb] = mma(av, pp[part], st.o[nb]);
@@ -224,6 +247,102 @@ struct NarrowLds {
     float merge[NW / 2][4 * (4 * C) + 2][64];
 };
 
+// Q^T operands of the lane's row at src; j: l / 16.
+template <int C, int QT, int ES>
+__device__ __forceinline__ void load_narrow_q(const typename Elem<QT>::T* src, int D, int j, int q_vec,
+                                              OpT<Kinds<QT, ES>::kF16> (&q)[Kinds<QT, ES>::kQParts][2 * C]) {
+    using K = Kinds<QT, ES>;
+    using T = typename Elem<QT>::T;
+#pragma unroll
+    for (int kb = 0; kb < 2 * C; ++kb) {
+        const int dim = ES == 1 ? 64 * (kb >> 1) + 16 * j + 8 * (kb & 1) : 32 * kb + 8 * j;
+        const bool inside = dim < D;
+        const T* p = src + (inside ? dim : 0);
+        float x[8];
+        if (q_vec) {
+            constexpr int kW = 8 * sizeof(T) / 16;
+            uint32_t w[4 * kW];
+#pragma unroll
+            for (int u = 0; u < kW; ++u) {
+                const u32x4_t y = reinterpret_cast<const u32x4_t*>(p)[u];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[4 * u + e] = y[e];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (QT == KVFP8_F32) x[i] = bits_f32(w[i]);
+                else x[i] = Elem<QT>::load((T)((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = Elem<QT>::load(p[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float y = inside ? x[i] : 0.0f;
+#pragma unroll
+            for (int part = 0; part < K::kQParts; ++part) {
+                const OpE<K::kF16> top = (OpE<K::kF16>)y;
+                q[part][kb][i] = top;
+                y = __builtin_isinf(y) ? 0.0f : y - (float)top;      // an infinite q is its first part alone
+            }
+        }
+    }
+}
+
+// The states of a head's waves join pairwise in LDS into its first one; waves without a step have nothing. Wave tw of
+// per_head of head hw; all waves of the workgroup.
+template <int C, int NW>
+__device__ __forceinline__ void join_waves(RowState<C>& st, NarrowLds<C, NW>& lds, int tw, int hw, int per_head, int steps, int lane) {
+    constexpr int NB = 4 * C;
+    for (int half = per_head >> 1; half > 0; half >>= 1) {
+        if (half >= steps) continue;                     // the upper half has no step (workgroup-uniform)
+        if (tw >= half && tw < 2 * half) {
+            float(*mine)[64] = lds.merge[hw * half + tw - half];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mine[4 * nb + i][lane] = st.o[nb][i];
+            mine[4 * NB][lane] = st.m;
+            mine[4 * NB + 1][lane] = st.l;
+        }
+        __syncthreads();
+        if (tw < half) {
+            const float(*other)[64] = lds.merge[hw * half + tw];
+            const float mo = other[4 * NB][lane];
+            const float mn = fmaxf(st.m, mo);
+            const float mu = mn == kNegInf ? 0.0f : mn;
+            const float wa = fast_exp2(st.m - mu), wb = fast_exp2(mo - mu);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st.o[nb][i] = st.o[nb][i] * wa + other[4 * nb + i][lane] * wb;
+            st.l = st.l * wa + other[4 * NB + 1][lane] * wb;
+            st.m = mn;
+        }
+        __syncthreads();
+    }
+}
+
+// A lane's part of state `at`; l: the sum over the row's lanes.
+template <int C>
+__device__ __forceinline__ void store_state(const DecodeArgs& d, int64_t at, const RowState<C>& st, float l, int D, int j) {
+    constexpr int NB = 4 * C;
+    if (j == 0) {
+        d.part_m[at] = st.m;
+        d.part_l[at] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d0 = NB * (4 * j + i);
+        if (d0 >= D) continue;
+        float* acc = d.part_acc + at * D + d0;
+#pragma unroll
+        for (int w = 0; w < NB / 4; ++w)
+            reinterpret_cast<float4*>(acc)[w] = make_float4(st.o[4 * w][i], st.o[4 * w + 1][i], st.o[4 * w + 2][i], st.o[4 * w + 3][i]);
+    }
+}
+
 // The states of an item's pairs, written to part `it.part`. NW waves, all of the workgroup.
 template <int C, int QT, int ES, int NW>
 __device__ __forceinline__ void narrow_run(const PrefixArgs& a, const PrefixItem& it, int heads, int q_vec, NarrowLds<C, NW>& lds) {
@@ -262,42 +381,8 @@ __device__ __forceinline__ void narrow_run(const PrefixArgs& a, const PrefixItem
     {
         const int32_t pair = min(it.r0 + m16, it.pairs - 1);
         const int32_t t = (uint32_t)pair / (uint32_t)G;
-        const T* src = reinterpret_cast<const T*>(a.d.q) + (int64_t)(it.rs + t) * a.d.q_stride_b + (h * G + (pair - t * G)) * a.d.q_stride_h;
-#pragma unroll
-        for (int kb = 0; kb < 2 * C; ++kb) {
-            const int dim = ES == 1 ? 64 * (kb >> 1) + 16 * j + 8 * (kb & 1) : 32 * kb + 8 * j;
-            const bool inside = dim < D;
-            const T* p = src + (inside ? dim : 0);
-            float x[8];
-            if (q_vec) {
-                constexpr int kW = 8 * sizeof(T) / 16;
-                uint32_t w[4 * kW];
-#pragma unroll
-                for (int u = 0; u < kW; ++u) {
-                    const u32x4_t y = reinterpret_cast<const u32x4_t*>(p)[u];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[4 * u + e] = y[e];
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if constexpr (QT == KVFP8_F32) x[i] = bits_f32(w[i]);
-                    else x[i] = Elem<QT>::load((T)((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu));
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = Elem<QT>::load(p[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float y = inside ? x[i] : 0.0f;
-#pragma unroll
-                for (int part = 0; part < K::kQParts; ++part) {
-                    const OpE<K::kF16> top = (OpE<K::kF16>)y;
-                    q[part][kb][i] = top;
-                    y = __builtin_isinf(y) ? 0.0f : y - (float)top;      // an infinite q is its first part alone
-                }
-            }
-        }
+        load_narrow_q<C, QT, ES>(reinterpret_cast<const T*>(a.d.q) + (int64_t)(it.rs + t) * a.d.q_stride_b +
+                                     (h * G + (pair - t * G)) * a.d.q_stride_h, D, j, q_vec, q);
     }
 
     RowState<C> st;
@@ -308,8 +393,9 @@ __device__ __forceinline__ void narrow_run(const PrefixArgs& a, const PrefixItem
     auto compute = [&](const PrefixStep<C, ES>& cur, int32_t t0, const TileRef& ra, const TileRef& rb) __attribute__((always_inline)) {
         const int lim_a = ra.valid ? min(16, hi - t0) : 0;
         const int lim_b = rb.valid ? min(16, hi - t0 - 16) : 0;
-        if (lim_a + lim_b == 32) prefix_step<C, QT, ES, true>(st, cur, q, lds.stage[wave], lane, 16, 16, a.d.score_scale);
-        else prefix_step<C, QT, ES, false>(st, cur, q, lds.stage[wave], lane, lim_a, lim_b, a.d.score_scale);
+        const FirstTokens counts{j, lim_a, lim_b};
+        if (lim_a + lim_b == 32) prefix_step<C, QT, ES, true>(st, cur, q, lds.stage[wave], lane, counts, a.d.score_scale);
+        else prefix_step<C, QT, ES, false>(st, cur, q, lds.stage[wave], lane, counts, a.d.score_scale);
     };
     while (tok < hi) {
         if (tok + stride < hi) issue(buf1, tok + stride, r1a, r1b);
@@ -321,35 +407,7 @@ __device__ __forceinline__ void narrow_run(const PrefixArgs& a, const PrefixItem
         tok += stride;
     }
 
-    // The states of a head's waves join pairwise in LDS into its first one; waves without a step have nothing.
-    const int steps = (hi - lo + 31) >> 5;
-    for (int half = per_head >> 1; half > 0; half >>= 1) {
-        if (half >= steps) continue;                     // the upper half has no step (workgroup-uniform)
-        if (tw >= half && tw < 2 * half) {
-            float(*mine)[64] = lds.merge[hw * half + tw - half];
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mine[4 * nb + i][lane] = st.o[nb][i];
-            mine[4 * NB][lane] = st.m;
-            mine[4 * NB + 1][lane] = st.l;
-        }
-        __syncthreads();
-        if (tw < half) {
-            const float(*other)[64] = lds.merge[hw * half + tw];
-            const float mo = other[4 * NB][lane];
-            const float mn = fmaxf(st.m, mo);
-            const float mu = mn == kNegInf ? 0.0f : mn;
-            const float wa = fast_exp2(st.m - mu), wb = fast_exp2(mo - mu);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) st.o[nb][i] = st.o[nb][i] * wa + other[4 * nb + i][lane] * wb;
-            st.l = st.l * wa + other[4 * NB + 1][lane] * wb;
-            st.m = mn;
-        }
-        __syncthreads();
-    }
+    join_waves<C, NW>(st, lds, tw, hw, per_head, (hi - lo + 31) >> 5, lane);
     if (tw != 0) return;
     const float l = sum_across_rows(st.l);
     const int32_t pair = it.r0 + m16;
@@ -357,19 +415,7 @@ __device__ __forceinline__ void narrow_run(const PrefixArgs& a, const PrefixItem
     const int32_t t = (uint32_t)pair / (uint32_t)G;
     const int hq = h * G + (pair - t * G);
     const int64_t pi = prefix_part(a, it.rs + t, it.part, hq);
-    if (j == 0) {
-        a.d.part_m[pi] = st.m;
-        a.d.part_l[pi] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int d0 = NB * (4 * j + i);
-        if (d0 >= D) continue;
-        float* acc = a.d.part_acc + pi * D + d0;
-#pragma unroll
-        for (int w = 0; w < NB / 4; ++w)
-            reinterpret_cast<float4*>(acc)[w] = make_float4(st.o[4 * w][i], st.o[4 * w + 1][i], st.o[4 * w + 2][i], st.o[4 * w + 3][i]);
-    }
+    store_state<C>(a.d, pi, st, l, D, j);
 }
 
 }  // namespace

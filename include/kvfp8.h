@@ -515,6 +515,56 @@ int kvfp8_norm_rope_backward(const void* x_dev, int dtype, int64_t rows, int32_t
                              void* dq_weight_dev, void* dk_weight_dev, void* workspace_dev, int64_t workspace_bytes,
                              void* stream);
 
+/*
+ * Attention of drafted trees, each behind its sequence's tokens in the paged cache: rows of q are nodes, packed,
+ *   out[r, hq, :] = softmax_t( q[r, hq, :] . khat[t, :] * sm_scale ) @ vhat.
+ * Sequence b has the rows [starts[b], starts[b + 1]) (seqs + 1 entries) and, on block-table row slots[b],
+ * context_lengths[b] tokens, of which the last starts[b + 1] - starts[b] are its nodes, in order. Row i of a sequence attends the
+ * tokens before the nodes, itself and the nodes above it: parents[r] is the number of a node's parent within its
+ * sequence; anything but a smaller node number makes it a root. Keys and values of nodes that a row does not attend do
+ * not reach it, whatever they hold.
+ * Only the first max_nodes (at most 256) rows of a sequence are computed; other rows, and those of no sequence, are not
+ * written. Rows without tokens (a slot outside the table, fewer tokens than nodes, missing pages) are zeros. Cache, block
+ * table, types, alignment and errors as kvfp8_paged_decode; all index arrays int32/int64 on the device. head_dim 1..512;
+ * rows * num_q_heads and seqs * max_nodes * num_q_heads below 2^22; bt_width * block_size below 2^31 - 65536.
+ * q: [rows, Hq, D], element strides (q_stride_r, q_stride_h, 1); out [rows, Hq, D] contiguous.
+ *   workspace: kvfp8_tree_attention_workspace_bytes(...) bytes, 256-byte aligned, any contents; one for each thread and
+ *   stream, as for kvfp8_paged_decode. Sizes that the call refuses need 0.
+ * No reference counterpart: a decode step there has one new token a sequence
+ * (reference src/torch_llm/kernals/decode_attention.py:39-550).
+ */
+int64_t kvfp8_tree_attention_workspace_bytes(int32_t seqs, int32_t max_nodes, int32_t num_q_heads, int32_t num_kv_heads,
+                                             int32_t head_dim, int32_t block_size, int kv_dtype);
+int kvfp8_tree_attention(const void* q_dev, int q_dtype, int64_t q_stride_r, int64_t q_stride_h, int64_t rows,
+                         int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, const void* k_cache_dev,
+                         const void* v_cache_dev, int kv_dtype, const float* k_scales_dev, const float* v_scales_dev,
+                         int64_t num_blocks, int32_t block_size, const int32_t* block_table_dev, int64_t bt_rows,
+                         int64_t bt_width, const void* slots_dev, int slots_dtype, const void* context_lengths_dev,
+                         int ctx_dtype, const void* starts_dev, int starts_dtype, const void* parents_dev,
+                         int parents_dtype, int32_t seqs, int32_t max_nodes, float sm_scale, void* out_dev,
+                         void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/*
+ * The drafted nodes that a model agrees with, and their cache rows moved behind the tokens before the draft. Node 0 of a
+ * sequence counts always; below a node n of the walk comes its child of lowest number whose tokens[] equals best[n]
+ * (the model's choice behind n). With the walk's nodes 0 = i_0 < i_1 < ... < i_(c - 1):
+ *   counts[b] = c, path[b, j] = i_j (-1 from c on; [seqs, max_nodes]), next_tokens[b] = best of node i_(c - 1);
+ *   a sequence without nodes: 0, -1s, -1;
+ *   the cache rows of token context_lengths[b] - n + i_j (n nodes) are copied to context_lengths[b] - n + j, in k, v and
+ *   their scales, in each of `layers` caches, unless either place has no page.
+ * caches: host array of 4 * layers device pointers (k, v, k scales, v scales; the scales unused where scale_bytes is 0);
+ * row_bytes: bytes of a token in k (H_kv * D * element size), scale_bytes: in its scales (H_kv * 4, or 0). Sequences
+ * share no pages that are written, caches no memory. starts, parents, max_nodes, slots and context_lengths as
+ * kvfp8_tree_attention; seqs below 2^17.
+ */
+int kvfp8_accept_draft(const void* tokens_dev, int tokens_dtype, const void* best_dev, int best_dtype,
+                       const void* starts_dev, int starts_dtype, const void* parents_dev, int parents_dtype, int64_t rows,
+                       int32_t seqs, int32_t max_nodes, const void* slots_dev, int slots_dtype,
+                       const void* context_lengths_dev, int ctx_dtype, const int32_t* block_table_dev, int64_t bt_rows,
+                       int64_t bt_width, int64_t num_blocks, int32_t block_size, void* const* caches, int32_t layers,
+                       int64_t row_bytes, int64_t scale_bytes, int32_t* counts_dev, int32_t* path_dev,
+                       int64_t* next_tokens_dev, void* stream);
+
 /* Human-readable name of a return code (negative KVFP8_E* or positive hipError_t). */
 const char* kvfp8_strerror(int code);
 
