@@ -37,17 +37,24 @@ struct TreeSeq {
     int64_t slot;
 };
 
+// Element i of int32 or int64 numbers as two 32-bit loads without a branch, so that several are in flight at once.
+__device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) {
+    const int32_t* const at = reinterpret_cast<const int32_t*>(p) + (is64 ? 2 * i : i);
+    const int32_t lo = at[0], up = at[is64 ? 1 : 0];
+    return ((int64_t)(is64 ? up : lo >> 31) << 32) | (uint32_t)lo;
+}
+
 __device__ __forceinline__ int64_t tree_row(const TreeArgs& a, int64_t i) {
-    const int64_t x = load_i(a.starts, a.starts64, i);
+    const int64_t x = index_at(a.starts, a.starts64, i);
     return x < 0 ? 0 : (x > a.rows ? a.rows : x);
 }
 
 // Sequence b. A slot outside the table, or fewer tokens than nodes: no tokens.
 __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
     TreeSeq s;
-    const int64_t r0 = tree_row(a, b), r1 = tree_row(a, b + 1), len = load_i(a.d.ctx, a.d.ctx64, b);
+    const int64_t r0 = tree_row(a, b), r1 = tree_row(a, b + 1), len = index_at(a.d.ctx, a.d.ctx64, b);
     const int64_t nodes = r1 > r0 ? r1 - r0 : 0, cap = a.d.bt_width * a.d.block_size;
-    s.slot = load_i(a.d.slots, a.d.slots64, b);
+    s.slot = index_at(a.d.slots, a.d.slots64, b);
     const bool ok = s.slot >= 0 && s.slot < a.d.bt_rows && len >= nodes;
     s.row0 = (int32_t)r0;
     s.nodes = (int32_t)(nodes < a.max_nodes ? nodes : a.max_nodes);
@@ -170,7 +177,8 @@ __device__ __forceinline__ TreeCut cut_batch(const TreeArgs& a) {
     };
     c.chunk = least;
     c.total = items(least);
-    if (a.seqs <= 64 && c.total > a.target) {
+    // With as many columns as that no chunk helps.
+    if (a.seqs <= 64 && c.total > a.target && wave_sum(tree_blocks(a, c.s)) * a.d.num_kv_heads <= a.target) {
         for (int i = 1; i <= 8; ++i) {
             const int32_t chunk = least + (least * i + 15) / 16, n = items(chunk);
             if (n > a.target) continue;
@@ -245,6 +253,41 @@ __device__ __forceinline__ bool tree_work(const TreeArgs& a, TreeWork& w) {
     w.hi = uniform((int32_t)min(lo + per, (int64_t)w.it.s.tokens));
     w.table = a.d.block_table + uniform64(w.it.s.slot) * a.d.bt_width;
     return true;
+}
+
+// Whether a dword holds a value that is not finite: codes 0x7F and 0xFF, or a 16-bit exponent of ones.
+template <int ES, bool kF16>
+__device__ __forceinline__ bool not_finite(uint32_t x) {
+    if constexpr (ES == 1) return (((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
+    constexpr uint32_t kInf = kF16 ? 0x7C00u : 0x7F80u;
+    return (x & 0x7FFFu) >= kInf || ((x >> 16) & 0x7FFFu) >= kInf;
+}
+
+// Pages of the two 16-token tiles of a step. They are read a step before their rows (scalar loads, whose wait leaves the
+// rows in flight alone), and there is no branch around the loads of a step: with one, the compiler could not count the
+// loads in flight and would wait for all of them. A tile past the end has the chunk's first page, and counts nothing.
+struct StepPages {
+    int32_t a, b;
+};
+struct StepRefs {
+    TileRef a, b;
+};
+__device__ __forceinline__ StepPages step_pages(const TreeArgs& a, const TreeWork& w, int32_t t0) {
+    auto page = [&](int32_t tok) __attribute__((always_inline)) {
+        const int64_t addr = uniform64((int64_t)(uintptr_t)(w.table + ((tok < w.hi ? tok : w.lo) >> a.d.bs_shift)));
+        return *(const_i32_ptr)(uintptr_t)addr;
+    };
+    t0 = uniform(t0);
+    return StepPages{page(t0), page(t0 + 16)};
+}
+__device__ __forceinline__ StepRefs step_refs(const TreeArgs& a, const TreeWork& w, const StepPages& p, int32_t t0) {
+    auto ref = [&](int32_t page, int32_t tok) __attribute__((always_inline)) {
+        page = uniform(page);
+        const bool ok = page >= 0 && page < a.d.num_blocks && tok < w.hi;
+        return TileRef{ok ? (int64_t)page * a.d.block_size + (tok & (a.d.block_size - 1)) : 0, ok};
+    };
+    t0 = uniform(t0);
+    return StepRefs{ref(p.a, t0), ref(p.b, t0 + 16)};
 }
 
 }  // namespace

@@ -50,27 +50,6 @@ typedef __attribute__((address_space(3))) const u32x2_t lds_u32x2;
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-
-// c += a b of 32 x 16 and 16 x 32 (lane l: A[l % 32][8 (l / 32) + i], B likewise, c[8 (i / 4) + 4 (l / 32) + i % 4][l % 32]).
-template <bool kF16>
-__device__ __forceinline__ f32x16_t mma32(u32x4_t a, u32x4_t b, f32x16_t c) {
-    if constexpr (kF16)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-}
-
-// Over the two lanes of a row.
-__device__ __forceinline__ float max_across_halves(float x) {
-    const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
-    return fmaxf(as_float(a[0]), as_float(a[1]));
-}
-__device__ __forceinline__ float sum_across_halves(float x) {
-    const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
-    return as_float(a[0]) + as_float(a[1]);
-}
-
 // Two codes -> two 16-bit values in a dword.
 template <bool kF16, bool kHi>
 __device__ __forceinline__ uint32_t widen2(uint32_t x) {

@@ -12,8 +12,11 @@ struct TreePlan {
     int64_t items;                    // at most
     int64_t part_l, part_acc, bytes;  // float32 states of items x block_rows pairs: m at 0, l and acc at these byte offsets
 };
-TreePlan tree_mfma_plan(int32_t seqs, int32_t max_nodes, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                        int q_dtype, int kv_dtype);
+TreePlan tree_mfma_plan(int32_t seqs, int32_t max_nodes, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int q_dtype);
+
+// 16-bit q (tree_attention_blocks.hip).
+template <int QT>
+hipError_t launch_tree_blocks(const TreeArgs& a, int kv_dtype, int64_t items, hipStream_t s);
 
 template <int QT>
 hipError_t launch_tree_mfma(TreeArgs a, int kv_dtype, const TreePlan& p, void* workspace, hipStream_t s);

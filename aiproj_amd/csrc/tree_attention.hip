@@ -173,7 +173,7 @@ int run_tree(const TreeArgs& a, int kv_dtype, void* workspace, int64_t workspace
     const bool aligned = (((uintptr_t)a.d.k_cache | (uintptr_t)a.d.v_cache | (uintptr_t)a.d.out) & 15) == 0;
     if (!aligned || !tree_on_mfma(a.d.num_kv_heads, a.d.head_dim, a.d.block_size, QT, kv_dtype))
         return (int)launch_tree_generic<QT>(a, kv_dtype, s);
-    const TreePlan p = tree_mfma_plan(a.seqs, a.max_nodes, a.d.num_q_heads, a.d.num_kv_heads, a.d.head_dim, QT, kv_dtype);
+    const TreePlan p = tree_mfma_plan(a.seqs, a.max_nodes, a.d.num_q_heads, a.d.num_kv_heads, a.d.head_dim, QT);
     if (!workspace || workspace_bytes < p.bytes) return KVFP8_EWORKSPACE;
     return (int)launch_tree_mfma<QT>(a, kv_dtype, p, workspace, s);
 }
@@ -193,7 +193,7 @@ extern "C" int64_t kvfp8_tree_attention_workspace_bytes(int32_t seqs, int32_t ma
     int64_t bytes = 0;
     for (const int q_dtype : {KVFP8_F32, KVFP8_F16, KVFP8_BF16})
         if (tree_on_mfma(num_kv_heads, head_dim, block_size, q_dtype, kv_dtype)) {
-            const int64_t need = tree_mfma_plan(seqs, max_nodes, num_q_heads, num_kv_heads, head_dim, q_dtype, kv_dtype).bytes;
+            const int64_t need = tree_mfma_plan(seqs, max_nodes, num_q_heads, num_kv_heads, head_dim, q_dtype).bytes;
             bytes = bytes > need ? bytes : need;
         }
     return bytes;

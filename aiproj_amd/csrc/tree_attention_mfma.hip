@@ -1,8 +1,9 @@
-// Attention of drafted trees on the gfx950 matrix cores.
+// Attention of drafted trees on the gfx950 matrix cores: float32 queries, and the join of all types.
 //
 // A call is two launches. In the first a workgroup takes an item: pairs (node, q head of a KV head) of a sequence against
 // a chunk of its tokens. Its waves take steps of 32 tokens in turn, each with the pairs in registers, join in LDS and leave
-// a softmax state, or the output where the sequence is one chunk. The second launch joins the states of a row.
+// a softmax state, or the output where the sequence is one chunk. The second launch joins the states of a row. (16-bit queries:
+// tree_attention_blocks.hip.)
 #include "joined_state.h"
 #include "shared_prefix_narrow.h"
 #include "tree_attention.h"
@@ -24,17 +25,9 @@ struct NodeTokens {
     }
 };
 
-// Whether a dword holds a value that is not finite: codes 0x7F and 0xFF, or a 16-bit exponent of ones.
-template <int ES, bool kF16>
-__device__ __forceinline__ bool not_finite(uint32_t x) {
-    if constexpr (ES == 1) return (((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
-    constexpr uint32_t kInf = kF16 ? 0x7C00u : 0x7F80u;
-    return (x & 0x7FFFu) >= kInf || ((x >> 16) & 0x7FFFu) >= kInf;
-}
-
 // V of a step that some rows do not count: with a value that is not finite in it the products go token by token, and a
 // row adds those of its own tokens alone.
-template <int C, int ES, bool kF16>
+template <int C>
 struct NodeProducts {
     const DecodeArgs& d;
     int64_t row_a, row_b;             // first cache rows of the tiles
@@ -46,7 +39,7 @@ struct NodeProducts {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int w = 0; w < VW; ++w) odd = odd || not_finite<ES, kF16>(v[i][w]);
+            for (int w = 0; w < VW; ++w) odd = odd || not_finite<1, false>(v[i][w]);
         return __ballot(odd) == 0;
     }
     __device__ __forceinline__ void add(RowState<C>& st, const float (&weight)[8], const bool (&live)[8]) const {
@@ -65,22 +58,19 @@ struct NodeProducts {
                     for (int nb = 0; nb < NB; ++nb) {
                         const int dim = NB * (4 * j + e) + nb;
                         if (dim >= d.head_dim) continue;
-                        float x;
-                        if constexpr (ES == 1) x = decode_e4m3fn(reinterpret_cast<const uint8_t*>(d.v_cache)[at + dim]);
-                        else x = Elem<kF16 ? KVFP8_F16 : KVFP8_BF16>::load(reinterpret_cast<const uint16_t*>(d.v_cache)[at + dim]);
-                        st.o[nb][e] += w * x;
+                        st.o[nb][e] += w * decode_e4m3fn(reinterpret_cast<const uint8_t*>(d.v_cache)[at + dim]);
                     }
             }
         }
     }
 };
 
-// Blocks of 16 pairs.
-template <int C, int QT, int ES>
+// Blocks of 16 pairs, for float32 queries: in three bf16 parts, whose operands leave no registers for more pairs.
+template <int C>
 __global__ void __launch_bounds__(64 * kTreeWaves)
 tree_narrow_kernel(TreeArgs a) {
+    constexpr int QT = KVFP8_F32, ES = 1;                // 16-bit caches come with q of their type
     using K = Kinds<QT, ES>;
-    using T = typename Elem<QT>::T;
     constexpr int NB = 4 * C, NW = kTreeWaves;
     __shared__ NarrowLds<C, NW> lds;
     __shared__ TreeMasks masks;
@@ -92,27 +82,17 @@ tree_narrow_kernel(TreeArgs a) {
     const int D = a.d.head_dim;
     const int32_t hi = w.hi, held = w.it.s.held;
 
-    auto issue = [&](PrefixStep<C, ES>& dst, int32_t t0, TileRef& ra, TileRef& rb) __attribute__((always_inline)) {
-        auto ref = [&](int32_t tok) __attribute__((always_inline)) {
-            const int64_t addr = uniform64((int64_t)(uintptr_t)(w.table + (tok >> a.d.bs_shift)));
-            const int64_t phys = *(const_i32_ptr)(uintptr_t)addr;
-            const bool ok = phys >= 0 && phys < a.d.num_blocks;
-            return TileRef{ok ? phys * a.d.block_size + (tok & (a.d.block_size - 1)) : 0, ok};
-        };
-        ra = ref(t0);
-        rb = t0 + 16 < hi ? ref(t0 + 16) : TileRef{0, 0};
-        load_prefix_step<C, ES>(dst, a.d, w.h, ra, rb, lane);
-    };
     PrefixStep<C, ES> buf0, buf1;
-    TileRef r0a, r0b, r1a, r1b;
     constexpr int32_t stride = 32 * NW;
     int32_t tok = w.lo + 32 * wave;
-    if (tok < hi) issue(buf0, tok, r0a, r0b);
+    StepRefs r0 = step_refs(a, w, step_pages(a, w, tok), tok), r1;
+    load_prefix_step<C, ES>(buf0, a.d, w.h, r0.a, r0.b, lane);
+    StepPages next = step_pages(a, w, tok + stride);
 
     const int32_t pair = min(w.r0 + m16, w.pairs - 1), node = (uint32_t)pair / (uint32_t)G;
     const int hq = w.h * G + (pair - node * G);
     OpT<K::kF16> q[K::kQParts][2 * C];
-    load_narrow_q<C, QT, ES>(reinterpret_cast<const T*>(a.d.q) + (int64_t)(w.it.s.row0 + node) * a.d.q_stride_b + hq * a.d.q_stride_h,
+    load_narrow_q<C, QT, ES>(reinterpret_cast<const float*>(a.d.q) + (int64_t)(w.it.s.row0 + node) * a.d.q_stride_b + hq * a.d.q_stride_h,
                              D, j, a.q_vec, q);
     if (hi > held) build_masks(masks, a, w.it.s);
 
@@ -122,33 +102,37 @@ tree_narrow_kernel(TreeArgs a) {
     st.m = kNegInf;
     st.l = 0.0f;
     // The steps before the nodes, then those that reach them.
-    auto compute = [&](const PrefixStep<C, ES>& cur, int32_t t0, const TileRef& ra, const TileRef& rb) __attribute__((always_inline)) {
-        const FirstTokens counts{j, ra.valid ? 16 : 0, rb.valid ? 16 : 0};
-        if (counts.lim_a + counts.lim_b == 32) prefix_step<C, QT, ES, true>(st, cur, q, lds.stage[wave], lane, counts, a.d.score_scale);
-        else prefix_step<C, QT, ES, false>(st, cur, q, lds.stage[wave], lane, counts, a.d.score_scale);
+    auto compute = [&](const PrefixStep<C, ES>& cur) __attribute__((always_inline)) {
+        prefix_step<C, QT, ES, true>(st, cur, q, lds.stage[wave], lane, FirstTokens{j, 16, 16}, a.d.score_scale);
+    };
+    auto issue = [&](PrefixStep<C, ES>& dst, StepRefs& refs, int32_t t0) __attribute__((always_inline)) {
+        refs = step_refs(a, w, next, t0);
+        load_prefix_step<C, ES>(dst, a.d, w.h, refs.a, refs.b, lane);
+        next = step_pages(a, w, t0 + stride);
     };
     const int32_t before = min(hi, held) - 31;           // steps that begin below it end before the nodes
-    while (tok < before) {
-        if (tok + stride < hi) issue(buf1, tok + stride, r1a, r1b);
-        compute(buf0, tok, r0a, r0b);
+    while (tok < before && r0.a.valid && r0.b.valid) {
+        issue(buf1, r1, tok + stride);
+        compute(buf0);
         tok += stride;
-        if (tok >= before) {
+        if (tok >= before || !r1.a.valid || !r1.b.valid) {
             buf0 = buf1;
-            r0a = r1a;
-            r0b = r1b;
+            r0 = r1;
             break;
         }
-        if (tok + stride < hi) issue(buf0, tok + stride, r0a, r0b);
-        compute(buf1, tok, r1a, r1b);
+        issue(buf0, r0, tok + stride);
+        compute(buf1);
         tok += stride;
     }
     while (tok < hi) {
-        const FirstTokens first{j, r0a.valid ? min(16, hi - tok) : 0, r0b.valid ? min(16, hi - tok - 16) : 0};
+        issue(buf1, r1, tok + stride);
+        const FirstTokens first{j, r0.a.valid ? min(16, hi - tok) : 0, r0.b.valid ? min(16, hi - tok - 16) : 0};
         const NodeTokens counts{first, hi > held ? node_bits(masks, node, tok, held) : ~0u};
-        const NodeProducts<C, ES, K::kF16V> products{a.d, r0a.row0, r0b.row0, w.h, lane};
+        const NodeProducts<C> products{a.d, r0.a.row0, r0.b.row0, w.h, lane};
         prefix_step<C, QT, ES, false>(st, buf0, q, lds.stage[wave], lane, counts, a.d.score_scale, products);
         tok += stride;
-        if (tok < hi) issue(buf0, tok, r0a, r0b);
+        buf0 = buf1;
+        r0 = r1;
     }
     join_waves<C, NW>(st, lds, wave, 0, NW, (hi - w.lo + 31) >> 5, lane);
     if (wave != 0) return;
@@ -158,7 +142,7 @@ tree_narrow_kernel(TreeArgs a) {
         store_state<C>(a.d, (int64_t)w.index * a.block_rows + m16, st, l, D, j);
         return;
     }
-    T* const out = reinterpret_cast<T*>(a.d.out) + ((int64_t)(w.it.s.row0 + node) * a.d.num_q_heads + hq) * D;
+    float* const out = reinterpret_cast<float*>(a.d.out) + ((int64_t)(w.it.s.row0 + node) * a.d.num_q_heads + hq) * D;
     const bool ok = l > 0.0f || l != l;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -171,53 +155,51 @@ tree_narrow_kernel(TreeArgs a) {
     }
 }
 
-// One wave per (row, q head): the states of its sequence's chunks, where there are several; zeros where it has no tokens.
+// The states of sequences of several chunks, zeros where a sequence has no tokens. A wave takes `run` pairs (row, q head), so
+// that few waves look for their sequence.
 template <int C, int QT>
 __global__ void __launch_bounds__(256)
-tree_join_kernel(TreeArgs a) {
+tree_join_kernel(TreeArgs a, int32_t run) {
     constexpr int kLanes = 16 * C, kPass = 64 / kLanes;
     using T = typename Elem<QT>::T;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int D = a.d.head_dim;
-    const int32_t unit = (int32_t)blockIdx.x * 4 + wave;
-    if (unit >= (int32_t)a.rows * a.d.num_q_heads) return;
-    const int32_t row = (uint32_t)unit / (uint32_t)a.d.num_q_heads, hq = unit - row * a.d.num_q_heads;
+    const int32_t units = (int32_t)a.rows * a.d.num_q_heads, begin = ((int32_t)blockIdx.x * 4 + wave) * run;
+    if (begin >= units) return;
     const TreeCut c = cut_batch(a);
-    TreeItem it;
-    if (!find_tree_item<true>(a, c, row, it) || it.chunks == 1) return;
     const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
-    const int32_t h = (uint32_t)hq / (uint32_t)G, pair = (row - it.s.row0) * G + (hq - h * G);
-    const int32_t block = (uint32_t)pair / (uint32_t)a.block_rows;
     const int d4 = min(lane % kLanes, D / 4 - 1), po = lane / kLanes;
-    const int64_t stride = (int64_t)a.d.num_kv_heads * it.blocks * a.block_rows;
-    const int64_t first = ((int64_t)it.first + (int64_t)h * it.blocks + block) * a.block_rows + (pair - block * a.block_rows);
-    JoinedState st;
+    TreeItem it;
+    bool found = false;
+    int32_t last = -1;
+    for (int32_t unit = begin; unit < min(begin + run, units); ++unit) {
+        const int32_t row = (uint32_t)unit / (uint32_t)a.d.num_q_heads, hq = unit - row * a.d.num_q_heads;
+        if (row != last && !(found && row - it.s.row0 < it.s.nodes)) found = find_tree_item<true>(a, c, row, it);
+        last = row;
+        if (!found || it.chunks == 1) continue;
+        const int32_t h = (uint32_t)hq / (uint32_t)G, pair = (row - it.s.row0) * G + (hq - h * G);
+        const int32_t block = (uint32_t)pair / (uint32_t)a.block_rows;
+        const int64_t stride = (int64_t)a.d.num_kv_heads * it.blocks * a.block_rows;
+        const int64_t first = ((int64_t)it.first + (int64_t)h * it.blocks + block) * a.block_rows + (pair - block * a.block_rows);
+        JoinedState st;
 #pragma unroll 4
-    for (int i = po; i < it.chunks; i += kPass) {
-        const int64_t at = first + i * stride;
-        st.add(a.d.part_m[at], a.d.part_l[at], reinterpret_cast<const float4*>(a.d.part_acc + at * D)[d4]);
+        for (int i = po; i < it.chunks; i += kPass) {
+            const int64_t at = first + i * stride;
+            st.add(a.d.part_m[at], a.d.part_l[at], reinterpret_cast<const float4*>(a.d.part_acc + at * D)[d4]);
+        }
+        st.across<kLanes>();
+        if (po != 0 || 4 * (lane % kLanes) >= D) continue;
+        st.store<QT>(reinterpret_cast<T*>(a.d.out) + (int64_t)unit * D + 4 * d4);
     }
-    st.across<kLanes>();
-    if (po != 0 || 4 * (lane % kLanes) >= D) return;
-    st.store<QT>(reinterpret_cast<T*>(a.d.out) + (int64_t)unit * D + 4 * d4);
 }
 
 size_t tree_align(size_t x) { return (x + 255) & ~(size_t)255; }
 
-template <int C, int QT, int ES>
 hipError_t launch_tree_narrow(const TreeArgs& a, int64_t items, hipStream_t s) {
     const dim3 grid((unsigned)(kXcdCount * ((items + kXcdCount - 1) / kXcdCount)));
-    hipLaunchKernelGGL((tree_narrow_kernel<C, QT, ES>), grid, dim3(64 * kTreeWaves), 0, s, a);
+    if (a.d.head_dim == 64) hipLaunchKernelGGL(tree_narrow_kernel<1>, grid, dim3(64 * kTreeWaves), 0, s, a);
+    else hipLaunchKernelGGL(tree_narrow_kernel<2>, grid, dim3(64 * kTreeWaves), 0, s, a);
     return hipGetLastError();
-}
-
-template <int QT>
-hipError_t launch_tree_narrow(const TreeArgs& a, int kv_dtype, int64_t items, hipStream_t s) {
-    if (kv_dtype == KVFP8_E4M3FN)
-        return a.d.head_dim == 64 ? launch_tree_narrow<1, QT, 1>(a, items, s) : launch_tree_narrow<2, QT, 1>(a, items, s);
-    if constexpr (QT != KVFP8_F32)
-        return a.d.head_dim == 64 ? launch_tree_narrow<1, QT, 2>(a, items, s) : launch_tree_narrow<2, QT, 2>(a, items, s);
-    else return hipErrorInvalidValue;                    // 16-bit caches come with q of their type
 }
 
 }  // namespace
@@ -228,14 +210,12 @@ bool tree_mfma_supported(int32_t head_dim, int32_t block_size, int q_dtype, int 
     return (head_dim == 64 || head_dim == 128) && (kv_dtype == KVFP8_BF16 || kv_dtype == KVFP8_F16) && q_dtype == kv_dtype;
 }
 
-TreePlan tree_mfma_plan(int32_t seqs, int32_t max_nodes, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                        int q_dtype, int kv_dtype) {
+TreePlan tree_mfma_plan(int32_t seqs, int32_t max_nodes, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int q_dtype) {
     TreePlan p = {};
-    (void)q_dtype;
-    (void)kv_dtype;
     const int64_t pairs = (int64_t)max_nodes * (num_q_heads / num_kv_heads);
-    p.block_rows = 16;
-    p.target = device_cus();
+    const bool narrow = q_dtype == KVFP8_F32;
+    p.block_rows = narrow ? 16 : 64;
+    p.target = device_cus() * (narrow ? 1 : 2);          // workgroups that a CU holds
     p.least_steps = 4;
     const int64_t columns = (int64_t)seqs * ((pairs + p.block_rows - 1) / p.block_rows) * num_kv_heads;
     // A chunk is at least the work divided by the target, so there are that many whole ones at most, and a column's last.
@@ -258,11 +238,16 @@ hipError_t launch_tree_mfma(TreeArgs a, int kv_dtype, const TreePlan& p, void* w
     a.least_steps = p.least_steps;
     const int64_t q_size = QT == KVFP8_F32 ? 4 : 2;
     a.q_vec = (uintptr_t)a.d.q % 16 == 0 && a.d.q_stride_b * q_size % 16 == 0 && a.d.q_stride_h * q_size % 16 == 0;
-    const hipError_t err = launch_tree_narrow<QT>(a, kv_dtype, p.items, s);
+    hipError_t err;
+    if constexpr (QT == KVFP8_F32) err = launch_tree_narrow(a, p.items, s);
+    else err = launch_tree_blocks<QT>(a, kv_dtype, p.items, s);
     if (err != hipSuccess) return err;
-    const dim3 grid((unsigned)((a.rows * a.d.num_q_heads + 3) / 4));
-    if (a.d.head_dim == 64) hipLaunchKernelGGL((tree_join_kernel<1, QT>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((tree_join_kernel<2, QT>), grid, dim3(256), 0, s, a);
+    // Eight waves a CU at most.
+    const int64_t units = a.rows * a.d.num_q_heads, waves = 8 * (int64_t)device_cus();
+    const int32_t run = (int32_t)((units + waves - 1) / waves);
+    const dim3 grid((unsigned)((units + 4 * run - 1) / (4 * run)));
+    if (a.d.head_dim == 64) hipLaunchKernelGGL((tree_join_kernel<1, QT>), grid, dim3(256), 0, s, a, run);
+    else hipLaunchKernelGGL((tree_join_kernel<2, QT>), grid, dim3(256), 0, s, a, run);
     return hipGetLastError();
 }
 
