@@ -21,7 +21,6 @@ struct TreeArgs {
     int32_t seqs, max_nodes;
     int32_t block_rows;               // (node, q head) pairs of a KV head in a row block
     int32_t target;                   // items that run at once
-    int32_t least_steps;              // of a chunk, in steps of kStep tokens
     int32_t q_vec;                    // q rows are 16-byte aligned
 };
 
@@ -29,12 +28,13 @@ namespace {
 
 constexpr int kStep = 64;             // chunks hold whole steps
 constexpr int kXcdCount = 8;          // workgroups are dispatched round-robin over the XCDs
+constexpr int kXcdRun = 8;            // neighbouring items of an XCD
 
 struct TreeSeq {
     int32_t row0, nodes;              // first row, computed nodes
     int32_t tokens;                   // in the cache, as far as the block table addresses them
     int32_t held;                     // tokens before the nodes
-    int64_t slot;
+    int64_t slot;                     // of a table of less than 2^31 rows, where there are tokens
 };
 
 // Element i of int32 or int64 numbers as two 32-bit loads without a branch, so that several are in flight at once.
@@ -125,12 +125,17 @@ struct TreeItem {
     int32_t chunks;                   // of its columns
 };
 
-template <typename T>
-__device__ __forceinline__ T wave_sum(T x) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off);
+// The sum of the lanes up to this one, by DPP: rows of 16 lanes, then their ends carried on (row_shr 1, 2, 4, 8, row_bcast 15, 31).
+__device__ __forceinline__ int32_t sum_up_to(int32_t x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
     return x;
 }
+__device__ __forceinline__ int32_t lanes_sum(int32_t x) { return __builtin_amdgcn_readlane(sum_up_to(x), 63); }
 
 __device__ __forceinline__ TreeSeq lane_seq(const TreeArgs& a, int b0) {
     const int b = b0 + (threadIdx.x & 63);
@@ -142,6 +147,25 @@ __device__ __forceinline__ int32_t tree_blocks(const TreeArgs& a, const TreeSeq&
     const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
     return s.tokens > 0 ? (int32_t)((uint32_t)(s.nodes * G + a.block_rows - 1) / (uint32_t)a.block_rows) : 0;
 }
+// 64 sequences, the longest ones first where they have more columns than run at once: items are dispatched in their order, and what
+// begins last is to be short. Each lane finds its sequence's rank by comparison and hands it to the lane of that rank. (61 sequences
+// of 1 to 3060 tokens and 1 to 60 nodes: 118 us in their own order, 105 in this. The sort costs 2 us, for nothing with fewer columns.)
+__device__ __forceinline__ TreeSeq sorted_seq(const TreeArgs& a, int b0) {
+    const int lane = threadIdx.x & 63, count = min(64, a.seqs - b0);
+    const TreeSeq s = lane_seq(a, b0);
+    if (lanes_sum(tree_blocks(a, s)) * a.d.num_kv_heads <= a.target) return s;
+    const uint32_t key = (uint32_t)((s.tokens + kStep - 1) / kStep) * 64 + (63 - lane);        // below 2^32, no two alike
+    int rank = 0;
+    for (int i = 0; i < count; ++i) rank += (uint32_t)__builtin_amdgcn_readlane((int32_t)key, i) > key;
+    if (lane >= count) rank = lane;
+    TreeSeq sorted;
+    sorted.row0 = __builtin_amdgcn_ds_permute(4 * rank, s.row0);
+    sorted.nodes = __builtin_amdgcn_ds_permute(4 * rank, s.nodes);
+    sorted.tokens = __builtin_amdgcn_ds_permute(4 * rank, s.tokens);
+    sorted.held = __builtin_amdgcn_ds_permute(4 * rank, s.held);
+    sorted.slot = __builtin_amdgcn_ds_permute(4 * rank, (int32_t)s.slot);
+    return sorted;
+}
 __device__ __forceinline__ int32_t tree_chunks(const TreeSeq& s, int32_t chunk) {
     return (int32_t)((uint32_t)((s.tokens + kStep - 1) / kStep + chunk - 1) / (uint32_t)chunk);
 }
@@ -151,19 +175,20 @@ __device__ __forceinline__ int32_t tree_chunks(const TreeSeq& s, int32_t chunk) 
 // 64 sequences).
 __device__ __forceinline__ TreeCut cut_batch(const TreeArgs& a) {
     TreeCut c;
-    c.s = lane_seq(a, 0);
-    unsigned long long work = 0;
+    c.s = sorted_seq(a, 0);
+    uint64_t work = 0;
     TreeSeq s = c.s;
     for (int b0 = 0;;) {
-        work += (unsigned long long)tree_blocks(a, s) * (uint32_t)(tree_chunks(s, 1));
+        const uint64_t mine = (uint64_t)tree_blocks(a, s) * (uint32_t)tree_chunks(s, 1);       // below 2^48
+        work += (uint32_t)lanes_sum((int32_t)(mine & 0xFFFFFFu)) + ((uint64_t)(uint32_t)lanes_sum((int32_t)(mine >> 24)) << 24);
         b0 += 64;
         if (b0 >= a.seqs) break;
-        s = lane_seq(a, b0);
+        s = sorted_seq(a, b0);
     }
-    work = wave_sum(work) * (uint32_t)a.d.num_kv_heads;
+    work *= (uint32_t)a.d.num_kv_heads;
     const uint64_t even = (work + a.target - 1) / (uint32_t)a.target;
     // (Never more than a table's 2^25 steps.)
-    const int32_t least = (int32_t)(even < (uint64_t)a.least_steps ? a.least_steps : (even < (1ull << 25) ? even : 1ull << 25));
+    const int32_t least = (int32_t)(even < 1 ? 1 : (even < (1ull << 25) ? even : 1ull << 25));
     auto items = [&](int32_t chunk) __attribute__((always_inline)) {
         int32_t n = 0;
         TreeSeq s = c.s;
@@ -171,14 +196,14 @@ __device__ __forceinline__ TreeCut cut_batch(const TreeArgs& a) {
             n += tree_blocks(a, s) * tree_chunks(s, chunk);
             b0 += 64;
             if (b0 >= a.seqs) break;
-            s = lane_seq(a, b0);
+            s = sorted_seq(a, b0);
         }
-        return wave_sum(n) * a.d.num_kv_heads;
+        return lanes_sum(n) * a.d.num_kv_heads;
     };
     c.chunk = least;
     c.total = items(least);
     // With as many columns as that no chunk helps.
-    if (a.seqs <= 64 && c.total > a.target && wave_sum(tree_blocks(a, c.s)) * a.d.num_kv_heads <= a.target) {
+    if (a.seqs <= 64 && c.total > a.target && lanes_sum(tree_blocks(a, c.s)) * a.d.num_kv_heads <= a.target) {
         for (int i = 1; i <= 8; ++i) {
             const int32_t chunk = least + (least * i + 15) / 16, n = items(chunk);
             if (n > a.target) continue;
@@ -193,17 +218,11 @@ __device__ __forceinline__ TreeCut cut_batch(const TreeArgs& a) {
 // The sequence that holds item `index` (kByRow: that computes row `index`); false without one.
 template <bool kByRow>
 __device__ __forceinline__ bool find_tree_item(const TreeArgs& a, const TreeCut& c, int32_t index, TreeItem& it) {
-    const int lane = threadIdx.x & 63;
     int32_t before = 0;
     TreeSeq s = c.s;
     for (int b0 = 0;;) {
         const int32_t blocks = tree_blocks(a, s), chunks = tree_chunks(s, c.chunk), items = blocks * a.d.num_kv_heads * chunks;
-        int32_t incl = items;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int32_t y = __shfl_up(incl, off);
-            if (lane >= off) incl += y;
-        }
+        const int32_t incl = sum_up_to(items);
         const int32_t first = before + incl - items;
         const uint64_t hit = __ballot(kByRow ? index >= s.row0 && index - s.row0 < s.nodes : index >= first && index - first < items);
         if (hit != 0) {
@@ -212,7 +231,7 @@ __device__ __forceinline__ bool find_tree_item(const TreeArgs& a, const TreeCut&
             it.s.nodes = __builtin_amdgcn_readlane(s.nodes, at);
             it.s.tokens = __builtin_amdgcn_readlane(s.tokens, at);
             it.s.held = __builtin_amdgcn_readlane(s.held, at);
-            it.s.slot = __builtin_amdgcn_readlane((int32_t)s.slot, at);    // of a table of less than 2^31 rows, where there are tokens
+            it.s.slot = __builtin_amdgcn_readlane((int32_t)s.slot, at);
             it.blocks = __builtin_amdgcn_readlane(blocks, at);
             it.chunks = __builtin_amdgcn_readlane(chunks, at);
             it.first = __builtin_amdgcn_readlane(first, at);
@@ -221,7 +240,7 @@ __device__ __forceinline__ bool find_tree_item(const TreeArgs& a, const TreeCut&
         before += __builtin_amdgcn_readlane(incl, 63);
         b0 += 64;
         if (b0 >= a.seqs) return false;
-        s = lane_seq(a, b0);
+        s = sorted_seq(a, b0);
     }
 }
 
@@ -233,14 +252,14 @@ struct TreeWork {
     const int32_t* table;             // block-table row
 };
 
-// The item of this workgroup; false without one. Each XCD takes one run of items, so that row blocks meet their tokens in
-// the same L2.
+// The item of this workgroup; false without one. Each XCD takes runs of neighbouring items in turn: row blocks meet their tokens in
+// the same L2, and long sequences spread over all XCDs. (Single items: 427 us instead of 415 for 8 sequences of 32768 tokens and
+// four row blocks; one run an XCD: 111 instead of 100 for 61 ragged ones.)
 __device__ __forceinline__ bool tree_work(const TreeArgs& a, TreeWork& w) {
     const TreeCut c = cut_batch(a);
-    const int32_t total = uniform(c.total), per_xcd = (total + kXcdCount - 1) / kXcdCount;
-    const int32_t xcd = (int32_t)(blockIdx.x % kXcdCount), local = (int32_t)(blockIdx.x / kXcdCount);
-    w.index = xcd * per_xcd + local;
-    if (local >= per_xcd || w.index >= total || !find_tree_item<false>(a, c, w.index, w.it)) return false;
+    const uint32_t local = blockIdx.x / kXcdCount, turn = local / (uint32_t)kXcdRun;
+    w.index = (int32_t)((turn * kXcdCount + blockIdx.x % kXcdCount) * kXcdRun + (local - turn * kXcdRun));
+    if (w.index >= uniform(c.total) || !find_tree_item<false>(a, c, w.index, w.it)) return false;
     const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
     uint32_t rest = (uint32_t)(w.index - w.it.first);
     const uint32_t column = rest / (uint32_t)w.it.blocks;

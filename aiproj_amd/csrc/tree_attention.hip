@@ -23,6 +23,12 @@ __device__ __forceinline__ float cached(const void* p, int64_t i) {
     else return Elem<KVT>::load(reinterpret_cast<const typename Elem<KVT>::T*>(p)[i]);
 }
 
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off);
+    return x;
+}
+
 // A workgroup per (row, q head). Its waves take steps of 64 tokens in turn: each lane scores a token, then the lanes add
 // the weighted values of the dims l, l + 64, ... token by token (those that do not count are passed over).
 template <int KVT, int QT, int ND>
@@ -171,7 +177,7 @@ int tree_shift(int32_t x) {
 template <int QT>
 int run_tree(const TreeArgs& a, int kv_dtype, void* workspace, int64_t workspace_bytes, hipStream_t s) {
     const bool aligned = (((uintptr_t)a.d.k_cache | (uintptr_t)a.d.v_cache | (uintptr_t)a.d.out) & 15) == 0;
-    if (!aligned || !tree_on_mfma(a.d.num_kv_heads, a.d.head_dim, a.d.block_size, QT, kv_dtype))
+    if (!aligned || a.d.score_scale == 0.0f || !tree_on_mfma(a.d.num_kv_heads, a.d.head_dim, a.d.block_size, QT, kv_dtype))
         return (int)launch_tree_generic<QT>(a, kv_dtype, s);
     const TreePlan p = tree_mfma_plan(a.seqs, a.max_nodes, a.d.num_q_heads, a.d.num_kv_heads, a.d.head_dim, QT);
     if (!workspace || workspace_bytes < p.bytes) return KVFP8_EWORKSPACE;

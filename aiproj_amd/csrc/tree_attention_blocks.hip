@@ -12,7 +12,7 @@
 //                               reads of those rows
 // Operand types as in shared_prefix_narrow.h.
 //
-// Two workgroups share a CU (216 VGPRs, 77 KB of LDS each), so that one computes while the other begins or joins. Microseconds of
+// Two workgroups share a CU (236 VGPRs, 77 KB of LDS each), so that one computes while the other begins or joins. Microseconds of
 // a call against blocks of 16 pairs (tree_attention_mfma.hip, which also takes 16-bit queries when built for them), and against
 // blocks of 32, 64 and 128 of eight waves, alone on their CU, cache in e4m3fn, head size 128:
 //   sequences, nodes, tokens, q / KV heads           16    8 x 32    8 x 64   8 x 128    4 x 64
@@ -149,6 +149,9 @@ tree_block_kernel(TreeArgs a) {
     for (int i = 0; i + 1 < S; ++i) push(i);
 
     // Q^T operands: lane (pair l % 32 of the tile, l / 32); pairs past the last repeat it and are never stored.
+    // With the scale's sign, so that the largest score is that of the largest product.
+    const float scale = fabsf(a.d.score_scale);
+    const uint32_t turn = a.d.score_scale < 0.0f ? 0x80008000u : 0u;
     u32x4_t q[KS];
     const int32_t pair = min(w.r0 + 32 * tile + col, w.pairs - 1), node = (uint32_t)pair / (uint32_t)G;
     const int32_t hq = w.h * G + (pair - node * G);
@@ -166,7 +169,7 @@ tree_block_kernel(TreeArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[e] = (uint32_t)p[2 * e] | ((uint32_t)p[2 * e + 1] << 16);
             }
-            q[s] = inside ? x : u32x4_t{0u, 0u, 0u, 0u};
+            q[s] = inside ? x ^ turn : u32x4_t{0u, 0u, 0u, 0u};
         }
     }
     if (end > held) build_masks(lds.masks, a, w.it.s);
@@ -199,23 +202,47 @@ tree_block_kernel(TreeArgs a) {
         const uint8_t* const here = &lds.ring[group][0][0] + slot * R::kStepBytes;
         lds_u8* const at = (lds_u8*)here;
         const float4* const scales = reinterpret_cast<const float4*>(here + 64 * R::kRow);
+        // All operands are asked for at once: two waves a SIMD hide little of LDS' latency.
+        u32x4_t kx[2 * C * ES], vx[2][N];
+#pragma unroll
+        for (int u = 0; u < 2 * C * ES; ++u) kx[u] = *(lds_u32x4*)(at + (k_off ^ (32u * u)));
+        f32x4_t ks[4], vs[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            if constexpr (ES == 1) ks[g] = __builtin_bit_cast(f32x4_t, scales[2 * g + hi]);
+            if constexpr (ES == 1) vs[g] = __builtin_bit_cast(f32x4_t, scales[8 + 2 * g + hi]);
+        }
+#pragma unroll
+        for (int pp = 0; pp < 2; ++pp)
+#pragma unroll
+            for (int nb = 0; nb < N; ++nb) {
+                if constexpr (ES == 1) {
+                    const v2i_t x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(at + ((v_off[0] ^ (32u * nb)) + 16 * pp * R::kRow)));
+                    vx[pp][nb] = u32x4_t{(uint32_t)x.x, (uint32_t)x.y, 0u, 0u};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint2 x = __builtin_bit_cast(
+                            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + ((v_off[e] ^ (64u * nb)) + 16 * pp * R::kRow))));
+                        vx[pp][nb][2 * e] = x.x;
+                        vx[pp][nb][2 * e + 1] = x.y;
+                    }
+                }
+            }
+        __builtin_amdgcn_sched_barrier(0);
         f32x16_t sc;
 #pragma unroll
         for (int u = 0; u < 2 * C * ES; ++u) {
-            const u32x4_t x = *(lds_u32x4*)(at + (k_off ^ (32u * u)));
             if constexpr (ES == 1) {
-                sc = mma32<kF16>(__builtin_bit_cast(u32x4_t, widen8<kF16>(x[0], x[1])), q[2 * u], u == 0 ? f32x16_t{} : sc);
-                sc = mma32<kF16>(__builtin_bit_cast(u32x4_t, widen8<kF16>(x[2], x[3])), q[2 * u + 1], sc);
+                sc = mma32<kF16>(__builtin_bit_cast(u32x4_t, widen8<kF16>(kx[u][0], kx[u][1])), q[2 * u], u == 0 ? f32x16_t{} : sc);
+                sc = mma32<kF16>(__builtin_bit_cast(u32x4_t, widen8<kF16>(kx[u][2], kx[u][3])), q[2 * u + 1], sc);
             } else {
-                sc = mma32<kF16>(x, q[u], u == 0 ? f32x16_t{} : sc);
+                sc = mma32<kF16>(kx[u], q[u], u == 0 ? f32x16_t{} : sc);
             }
         }
+        if constexpr (ES == 1) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            f32x4_t ks = {a.d.score_scale, a.d.score_scale, a.d.score_scale, a.d.score_scale};
-            if constexpr (ES == 1) ks *= __builtin_bit_cast(f32x4_t, scales[2 * g + hi]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[4 * g + e] *= ks[e];
+            for (int x = 0; x < 16; ++x) sc[x] *= ks[x >> 2][x & 3];
         }
         // Rows of V that count for no pair (stale pages may hold NaN) and those with a value that is not finite are zeros in the
         // products, and their scales zeros: a weight of 0 would not keep them from a pair. The latter (`odd`) come one by one.
@@ -254,6 +281,7 @@ tree_block_kernel(TreeArgs a) {
         float mx = sc[0];
 #pragma unroll
         for (int x = 1; x < 16; ++x) mx = fmaxf(mx, sc[x]);
+        mx *= scale;
         if (__ballot(mx > lim)) {
             const float top = max_across_halves(mx);
             const bool fresh = lim == kNegInf;
@@ -268,16 +296,14 @@ tree_block_kernel(TreeArgs a) {
         u32x4_t pop[kParts][2];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            f32x4_t vs = {1.0f, 1.0f, 1.0f, 1.0f};
-            if constexpr (ES == 1) vs = __builtin_bit_cast(f32x4_t, scales[8 + 2 * g + hi]);
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
                 float y[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float p = fast_exp2(sc[4 * g + 2 * v + e] - ref);
+                    const float p = fast_exp2(__builtin_fmaf(sc[4 * g + 2 * v + e], scale, -ref));
                     l += p;
-                    y[e] = ES == 1 ? p * vs[2 * v + e] : p;
+                    y[e] = ES == 1 ? p * vs[g][2 * v + e] : p;
                     if (!kWhole && ((gone >> (8 * g + 4 * hi + 2 * v + e)) & 1) != 0) y[e] = 0.0f;
                 }
 #pragma unroll
@@ -304,17 +330,8 @@ tree_block_kernel(TreeArgs a) {
 #pragma unroll
             for (int nb = 0; nb < N; ++nb) {
                 u32x4_t av;
-                if constexpr (ES == 1) {
-                    const v2i_t x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(at + ((v_off[0] ^ (32u * nb)) + 16 * pp * R::kRow)));
-                    av = __builtin_bit_cast(u32x4_t, fp8x8((uint32_t)x.x & keep[0], (uint32_t)x.y & keep[1]));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + ((v_off[e] ^ (64u * nb)) + 16 * pp * R::kRow))));
-                        av[2 * e] = x.x & keep[2 * e];
-                        av[2 * e + 1] = x.y & keep[2 * e + 1];
-                    }
-                }
+                if constexpr (ES == 1) av = __builtin_bit_cast(u32x4_t, fp8x8(vx[pp][nb][0] & keep[0], vx[pp][nb][1] & keep[1]));
+                else av = vx[pp][nb] & keep;
 #pragma unroll
                 for (int part = 0; part < kParts; ++part) o[nb] = mma32<kF16V>(av, pop[part][pp], o[nb]);
             }
@@ -329,7 +346,7 @@ tree_block_kernel(TreeArgs a) {
                 s = __shfl(s, 32 * ((tt >> 2) & 1) + col);
                 if (s == kNegInf) continue;              // it does not count for the pair (or at a weight of 0)
                 const int64_t row = ((tt < 16 ? refs.a.row0 : refs.b.row0) + (tt & 15)) * a.d.num_kv_heads + w.h;
-                const float weight = fast_exp2(s - ref) * (ES == 1 ? a.d.v_scales[row] : 1.0f);
+                const float weight = fast_exp2(__builtin_fmaf(s, scale, -ref)) * (ES == 1 ? a.d.v_scales[row] : 1.0f);
 #pragma unroll
                 for (int nb = 0; nb < N; ++nb)
 #pragma unroll
@@ -424,7 +441,7 @@ tree_block_kernel(TreeArgs a) {
 
 template <int C, int QT, int ES>
 hipError_t launch_blocks(const TreeArgs& a, int64_t items, hipStream_t s) {
-    const dim3 grid((unsigned)(kXcdCount * ((items + kXcdCount - 1) / kXcdCount)));
+    const dim3 grid((unsigned)tree_grid(items));
     hipLaunchKernelGGL((tree_block_kernel<C, QT, ES>), grid, dim3(64 * kBlockWaves), 0, s, a);
     return hipGetLastError();
 }

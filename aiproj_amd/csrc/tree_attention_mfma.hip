@@ -196,7 +196,7 @@ tree_join_kernel(TreeArgs a, int32_t run) {
 size_t tree_align(size_t x) { return (x + 255) & ~(size_t)255; }
 
 hipError_t launch_tree_narrow(const TreeArgs& a, int64_t items, hipStream_t s) {
-    const dim3 grid((unsigned)(kXcdCount * ((items + kXcdCount - 1) / kXcdCount)));
+    const dim3 grid((unsigned)tree_grid(items));
     if (a.d.head_dim == 64) hipLaunchKernelGGL(tree_narrow_kernel<1>, grid, dim3(64 * kTreeWaves), 0, s, a);
     else hipLaunchKernelGGL(tree_narrow_kernel<2>, grid, dim3(64 * kTreeWaves), 0, s, a);
     return hipGetLastError();
@@ -216,7 +216,6 @@ TreePlan tree_mfma_plan(int32_t seqs, int32_t max_nodes, int32_t num_q_heads, in
     const bool narrow = q_dtype == KVFP8_F32;
     p.block_rows = narrow ? 16 : 64;
     p.target = device_cus() * (narrow ? 1 : 2);          // workgroups that a CU holds
-    p.least_steps = 4;
     const int64_t columns = (int64_t)seqs * ((pairs + p.block_rows - 1) / p.block_rows) * num_kv_heads;
     // A chunk is at least the work divided by the target, so there are that many whole ones at most, and a column's last.
     p.items = p.target + columns;
@@ -235,15 +234,15 @@ hipError_t launch_tree_mfma(TreeArgs a, int kv_dtype, const TreePlan& p, void* w
     a.d.part_acc = reinterpret_cast<float*>(ws + p.part_acc);
     a.block_rows = p.block_rows;
     a.target = p.target;
-    a.least_steps = p.least_steps;
     const int64_t q_size = QT == KVFP8_F32 ? 4 : 2;
     a.q_vec = (uintptr_t)a.d.q % 16 == 0 && a.d.q_stride_b * q_size % 16 == 0 && a.d.q_stride_h * q_size % 16 == 0;
     hipError_t err;
     if constexpr (QT == KVFP8_F32) err = launch_tree_narrow(a, p.items, s);
     else err = launch_tree_blocks<QT>(a, kv_dtype, p.items, s);
     if (err != hipSuccess) return err;
-    // Eight waves a CU at most.
-    const int64_t units = a.rows * a.d.num_q_heads, waves = 8 * (int64_t)device_cus();
+    // Sixteen waves a CU at most: each looks for its sequence, which takes longer than a row (ragged sequences: 19 us with 8, 16 with
+    // 16, 23 with a wave for every row).
+    const int64_t units = a.rows * a.d.num_q_heads, waves = 16 * (int64_t)device_cus();
     const int32_t run = (int32_t)((units + waves - 1) / waves);
     const dim3 grid((unsigned)((units + 4 * run - 1) / (4 * run)));
     if (a.d.head_dim == 64) hipLaunchKernelGGL((tree_join_kernel<1, QT>), grid, dim3(256), 0, s, a, run);
