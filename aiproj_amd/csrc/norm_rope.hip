@@ -11,9 +11,15 @@
 //   dx = inv (h w - (x inv) mean_d(h w x inv)),  and the gradient of the values as it is.
 //
 // Layout: a head row is held by LPR lanes with eight elements (four pairs) each, so that 128 dims take 16 lanes and one
-// 16-byte load a lane. A group of LPR lanes takes a run of kHeads heads of one token, whose loads are issued together
-// and which share the position, the angles and the weights' cache lines.
+// 16-byte load a lane. A group of LPR lanes takes a run of up to kHeads heads of one section (q, k or v), the same heads of one
+// token after another: the weights and their gradients' sums stay in registers, the heads of a token share the angles, and their
+// loads are issued together.
+//
+// Bound by HBM: 16384 tokens of 32 + 8 heads of 128 in bfloat16 take 73 us forward (403 MB, 5.5 TB/s) and 122 us backward (570 MB,
+// 4.7 TB/s); 65536 tokens of 16 + 4 heads with packed outputs and an e4m3fn cache 190 us (873 MB, 4.6 TB/s). Sums across a row's
+// lanes by DPP, the hardware's reciprocal root and 16-bit roundings in pairs keep the vector ALU below that.
 #include "kvfp8_common.h"
+#include "mfma_tiles.h"
 
 namespace kvfp8 {
 
@@ -21,13 +27,14 @@ namespace {
 
 constexpr int kNrThreads = 256;
 constexpr int kNrElems = 8;
+constexpr int kNrTokens = 4;
 
 struct NormRopeArgs {
     const void* x;
     int64_t rows, row_stride;
     int32_t num_q_heads, num_kv_heads, head_dim;
-    uint32_t runs;                        // of heads, per token
-    uint32_t total;                       // rows x runs, below 2^31
+    uint32_t q_runs, kv_runs;             // of heads, per section
+    uint32_t step;                        // tokens taken at once: group g begins with run g % runs of token g / runs
     const void* positions;
     int32_t pos64;
     const void* cos_table;
@@ -63,53 +70,108 @@ __device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) 
     return is64 ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t)reinterpret_cast<const int32_t*>(p)[i];
 }
 
-// Elements d0 .. d0 + N - 1 of a row of type DT, zeros past D. VEC: the row starts at a multiple of the access and D is a
-// multiple of N.
+// Elements d0 .. d0 + N - 1 of a row of type DT as they are stored, zeros past D. VEC: the row starts at a multiple of the access
+// and D is a multiple of N.
+template <int DT, int N>
+struct alignas(sizeof(typename Elem<DT>::T) * N < 16 ? sizeof(typename Elem<DT>::T) * N : 16) Raw {
+    typename Elem<DT>::T e[N];
+};
 template <int DT, int N, bool VEC>
-__device__ __forceinline__ void load_run(const void* row, int d0, int D, float (&x)[N]) {
-    using T = typename Elem<DT>::T;
-    const T* p = reinterpret_cast<const T*>(row) + d0;
+__device__ __forceinline__ Raw<DT, N> load_raw(const typename Elem<DT>::T* row, int d0, int D) {
+    Raw<DT, N> raw = {};
     if constexpr (VEC) {
-        struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Run { T e[N]; };
-        Run raw = {};
-        if (d0 < D) raw = *reinterpret_cast<const Run*>(p);
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = Elem<DT>::load(raw.e[i]);
+        if (d0 < D) raw = *reinterpret_cast<const Raw<DT, N>*>(row + d0);
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = d0 + i < D ? Elem<DT>::load(p[i]) : 0.0f;
+        for (int i = 0; i < N; ++i)
+            if (d0 + i < D) raw.e[i] = row[d0 + i];
     }
+    return raw;
+}
+template <int DT, int N, bool VEC>
+__device__ __forceinline__ void store_raw(typename Elem<DT>::T* row, int d0, int D, const Raw<DT, N>& raw) {
+    if constexpr (VEC) {
+        if (d0 < D) *reinterpret_cast<Raw<DT, N>*>(row + d0) = raw;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (d0 + i < D) row[d0 + i] = raw.e[i];
+    }
+}
+template <int DT, int N>
+__device__ __forceinline__ void widen(const Raw<DT, N>& raw, float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = Elem<DT>::load(raw.e[i]);
 }
 
 template <int N, bool VEC>
 __device__ __forceinline__ void load_any(const void* row, int dtype, int d0, int D, float (&x)[N]) {
-    if (dtype == KVFP8_F32) load_run<KVFP8_F32, N, VEC>(row, d0, D, x);
-    else if (dtype == KVFP8_F16) load_run<KVFP8_F16, N, VEC>(row, d0, D, x);
-    else load_run<KVFP8_BF16, N, VEC>(row, d0, D, x);
+    if (dtype == KVFP8_F32) widen(load_raw<KVFP8_F32, N, VEC>(reinterpret_cast<const float*>(row), d0, D), x);
+    else if (dtype == KVFP8_F16) widen(load_raw<KVFP8_F16, N, VEC>(reinterpret_cast<const uint16_t*>(row), d0, D), x);
+    else widen(load_raw<KVFP8_BF16, N, VEC>(reinterpret_cast<const uint16_t*>(row), d0, D), x);
 }
 
 template <int DT, bool VEC>
-__device__ __forceinline__ void store_run8(void* row, int d0, int D, const float (&x)[kNrElems]) {
-    using T = typename Elem<DT>::T;
-    T* p = reinterpret_cast<T*>(row) + d0;
-    if constexpr (VEC) {
-        struct alignas(16) Run { T e[kNrElems]; };
-        Run raw;
+__device__ __forceinline__ void store_run8(typename Elem<DT>::T* row, int d0, int D, const float (&x)[kNrElems]) {
+    Raw<DT, kNrElems> raw;
+    if constexpr (DT == KVFP8_F32) {
 #pragma unroll
-        for (int i = 0; i < kNrElems; ++i) raw.e[i] = Elem<DT>::store(x[i]);
-        if (d0 < D) *reinterpret_cast<Run*>(p) = raw;
+        for (int i = 0; i < kNrElems; ++i) raw.e[i] = x[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < kNrElems; ++i)
-            if (d0 + i < D) p[i] = Elem<DT>::store(x[i]);
+        for (int i = 0; i < kNrElems; i += 2) {
+            const uint32_t two = pack2<DT == KVFP8_F16>(x[i], x[i + 1]);
+            raw.e[i] = (uint16_t)two;
+            raw.e[i + 1] = (uint16_t)(two >> 16);
+        }
     }
+    store_raw<DT, kNrElems, VEC>(row, d0, D, raw);
 }
 
+// Sum (largest) of the LPR lanes of a row, the same in each: 16 lanes by DPP (quads, half rows and rows mirrored).
+template <int CTRL>
+__device__ __forceinline__ uint32_t row_dpp(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true);
+}
+template <int LPR, typename Fold>
+__device__ __forceinline__ uint32_t row_fold(uint32_t x, Fold fold) {
+    x = fold(x, row_dpp<0xB1>(x));
+    x = fold(x, row_dpp<0x4E>(x));
+    x = fold(x, row_dpp<0x141>(x));
+    if constexpr (LPR >= 16) x = fold(x, row_dpp<0x140>(x));
+    if constexpr (LPR >= 32) x = fold(x, (uint32_t)__shfl_xor((int)x, 16, 64));
+    if constexpr (LPR >= 64) x = fold(x, (uint32_t)__shfl_xor((int)x, 32, 64));
+    return x;
+}
 template <int LPR>
 __device__ __forceinline__ float row_sum(float x) {
-#pragma unroll
-    for (int s = 1; s < LPR; s <<= 1) x += __shfl_xor(x, s, 64);
-    return x;
+    return bits_f32(row_fold<LPR>(f32_bits(x), [](uint32_t a, uint32_t b) { return f32_bits(bits_f32(a) + bits_f32(b)); }));
+}
+
+// 1 / sqrt(x): the hardware's estimate (one unit in the last place) but for subnormal numbers, which it takes for zeros.
+__device__ __forceinline__ float inverse_root(float x) {
+    return x < 1.17549435e-38f ? 1.0f / sqrtf(x) : __builtin_amdgcn_rsqf(x);
+}
+
+// The heads of a group: `count` ones from `first` on of a section (0 q, 1 k, 2 v) of `heads`, behind `before` others in a row of x.
+struct HeadRun {
+    int section, first, count, heads, before;
+    uint32_t token;
+};
+template <int LPR, int kHeads>
+__device__ __forceinline__ HeadRun head_run(const NormRopeArgs& a) {
+    HeadRun r;
+    const uint32_t runs = a.q_runs + 2 * a.kv_runs, group = blockIdx.x * (kNrThreads / LPR) + threadIdx.x / LPR;
+    r.token = group / runs;
+    uint32_t run = group - r.token * runs;
+    if (r.token >= a.step) r.token = (uint32_t)a.rows;   // the last workgroup's groups past the last whole token: none
+    r.section = run < a.q_runs ? 0 : (run < a.q_runs + a.kv_runs ? 1 : 2);
+    run -= r.section == 0 ? 0 : (r.section == 1 ? a.q_runs : a.q_runs + a.kv_runs);
+    r.heads = r.section == 0 ? a.num_q_heads : a.num_kv_heads;
+    r.first = (int)run * kHeads;
+    r.count = min(kHeads, r.heads - r.first);
+    r.before = r.section == 0 ? 0 : a.num_q_heads + (r.section == 2 ? a.num_kv_heads : 0);
+    return r;
 }
 
 // The four angles of a lane's pairs.
@@ -118,9 +180,8 @@ struct Angles {
 };
 
 template <bool VEC>
-__device__ __forceinline__ Angles load_angles(const NormRopeArgs& a, int64_t token, int d0) {
+__device__ __forceinline__ Angles load_angles(const NormRopeArgs& a, int64_t pos, int d0) {
     Angles g;
-    const int64_t pos = index_at(a.positions, a.pos64, token);
     const int half = a.head_dim / 2;
     if (pos >= 0 && pos < a.table_rows) {
         const int64_t es = a.table_dtype == KVFP8_F32 ? 4 : 2;
@@ -163,60 +224,63 @@ __global__ void __launch_bounds__(kNrThreads)
 norm_rope_kernel(NormRopeArgs a) {
     using T = typename Elem<DT>::T;
     const int D = a.head_dim, lane = threadIdx.x % LPR, d0 = kNrElems * lane;
-    const int heads = a.num_q_heads + 2 * a.num_kv_heads, first_v = a.num_q_heads + a.num_kv_heads;
-    const uint32_t stride = gridDim.x * (kNrThreads / LPR);
-    for (uint32_t unit = blockIdx.x * (kNrThreads / LPR) + threadIdx.x / LPR; unit < a.total; unit += stride) {
-        const uint32_t token = unit / a.runs;
-        const int h0 = (int)(unit - token * a.runs) * kHeads;
-        const T* const src = reinterpret_cast<const T*>(a.x) + (int64_t)token * a.row_stride;
-        float x[kHeads][kNrElems];
+    const HeadRun r = head_run<LPR, kHeads>(a);
+    if (r.token >= a.rows) return;
+    const bool is_v = r.section == 2, cached = r.section != 0 && a.blocks != nullptr;
+    const float per_dim = 1.0f / (float)D;
+    float w[kNrElems] = {};
+    if (a.q_weight != nullptr && !is_v) load_any<kNrElems, VEC>(r.section == 0 ? a.q_weight : a.k_weight, a.w_dtype, d0, D, w);
+    T* const outs = reinterpret_cast<T*>(r.section == 0 ? a.q_out : (is_v ? a.v_out : a.k_out));
+    for (int64_t token = r.token; token < a.rows; token += a.step) {
+        const int64_t pos = is_v ? 0 : index_at(a.positions, a.pos64, token);
+        const T* const src = reinterpret_cast<const T*>(a.x) + token * a.row_stride + (int64_t)(r.before + r.first) * D;
+        Raw<DT, kNrElems> raw[kHeads];
 #pragma unroll
-        for (int u = 0; u < kHeads; ++u) load_run<DT, kNrElems, VEC>(src + (int64_t)min(h0 + u, heads - 1) * D, d0, D, x[u]);
+        for (int u = 0; u < kHeads; ++u) raw[u] = load_raw<DT, kNrElems, VEC>(src + (int64_t)min(u, r.count - 1) * D, d0, D);
         int64_t block = -1, offset = -1;
-        if (a.blocks != nullptr && h0 + kHeads > a.num_q_heads) {
+        if (cached) {
             block = index_at(a.blocks, a.blocks64, token);
             offset = index_at(a.offsets, a.offsets64, token);
         }
-        Angles g;
-        if (h0 < first_v) g = load_angles<VEC>(a, token, d0);
+        const bool inside = block >= 0 && block < a.num_blocks && offset >= 0 && offset < a.block_size;
+        Angles g = {};
+        if (!is_v) g = load_angles<VEC>(a, pos, d0);
 #pragma unroll
         for (int u = 0; u < kHeads; ++u) {
-            const int h = h0 + u;
-            if (h >= heads) break;                       // the same for the lanes of a row
-            if (h < first_v) {
+            if (u >= r.count) break;                     // the same for the lanes of a row
+            T* const out = outs == nullptr ? nullptr : outs + (token * r.heads + r.first + u) * D;
+            float x[kNrElems];
+            widen(raw[u], x);
+            if (is_v) {
+                if (out != nullptr) store_raw<DT, kNrElems, VEC>(out, d0, D, raw[u]);
+            } else {
                 if (a.q_weight != nullptr) {
-                    float w[kNrElems], sum = 0.0f;
-                    load_any<kNrElems, VEC>(h < a.num_q_heads ? a.q_weight : a.k_weight, a.w_dtype, d0, D, w);
+                    float sum = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < kNrElems; ++i) sum += x[u][i] * x[u][i];
-                    const float inv = 1.0f / sqrtf(row_sum<LPR>(sum) / (float)D + a.eps);
+                    for (int i = 0; i < kNrElems; ++i) sum += x[i] * x[i];
+                    const float inv = inverse_root(row_sum<LPR>(sum) * per_dim + a.eps);
 #pragma unroll
-                    for (int i = 0; i < kNrElems; ++i) x[u][i] = (x[u][i] * inv) * w[i];
+                    for (int i = 0; i < kNrElems; ++i) x[i] = (x[i] * inv) * w[i];
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float y0 = x[u][2 * i], y1 = x[u][2 * i + 1];
-                    x[u][2 * i] = g.c[i] * y0 - g.s[i] * y1;
-                    x[u][2 * i + 1] = g.s[i] * y0 + g.c[i] * y1;
+                    const float y0 = x[2 * i], y1 = x[2 * i + 1];
+                    x[2 * i] = g.c[i] * y0 - g.s[i] * y1;
+                    x[2 * i + 1] = g.s[i] * y0 + g.c[i] * y1;
                 }
+                if (out != nullptr) store_run8<DT, VEC>(out, d0, D, x);
             }
-            const bool is_q = h < a.num_q_heads, is_v = h >= first_v;
-            const int nh = is_q ? a.num_q_heads : a.num_kv_heads, hh = is_q ? h : (is_v ? h - first_v : h - a.num_q_heads);
-            T* const out = reinterpret_cast<T*>(is_q ? a.q_out : (is_v ? a.v_out : a.k_out));
-            if (out != nullptr) store_run8<DT, VEC>(out + ((int64_t)token * nh + hh) * D, d0, D, x[u]);
-            if (is_q || a.blocks == nullptr) continue;
-            const bool inside = block >= 0 && block < a.num_blocks && offset >= 0 && offset < a.block_size;
-            const int64_t slot = (block * a.block_size + offset) * nh + hh;
+            if (!cached) continue;
+            const int64_t slot = (block * a.block_size + offset) * r.heads + r.first + u;
             void* const cache = is_v ? a.v_cache : a.k_cache;
             if (a.cache_dtype == KVFP8_E4M3FN) {
                 uint32_t amax = 0;
 #pragma unroll
-                for (int i = 0; i < kNrElems; ++i) amax = max(amax, abs_bits(x[u][i]));
-#pragma unroll
-                for (int s = 1; s < LPR; s <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, s, 64));
+                for (int i = 0; i < kNrElems; ++i) amax = max(amax, abs_bits(x[i]));
+                amax = row_fold<LPR>(amax, [](uint32_t p, uint32_t q) { return max(p, q); });
                 if (!inside) continue;
                 const float scale = row_scale(amax);
-                const uint2 codes = encode_run(x[u], amax, scale);
+                const uint2 codes = encode_run(x, amax, scale);
                 uint8_t* const dst = reinterpret_cast<uint8_t*>(cache) + slot * D + d0;
                 if constexpr (VEC) {
                     if (d0 < D) *reinterpret_cast<uint2*>(dst) = codes;
@@ -227,85 +291,77 @@ norm_rope_kernel(NormRopeArgs a) {
                 }
                 if (lane == 0) (is_v ? a.v_scales : a.k_scales)[slot] = scale;
             } else if (inside) {
-                if (a.cache_dtype == KVFP8_F32) store_run8<KVFP8_F32, VEC>(reinterpret_cast<float*>(cache) + slot * D, d0, D, x[u]);
-                else if (a.cache_dtype == KVFP8_F16) store_run8<KVFP8_F16, VEC>(reinterpret_cast<uint16_t*>(cache) + slot * D, d0, D, x[u]);
-                else store_run8<KVFP8_BF16, VEC>(reinterpret_cast<uint16_t*>(cache) + slot * D, d0, D, x[u]);
+                if (a.cache_dtype == KVFP8_F32) store_run8<KVFP8_F32, VEC>(reinterpret_cast<float*>(cache) + slot * D, d0, D, x);
+                else if (a.cache_dtype == KVFP8_F16) store_run8<KVFP8_F16, VEC>(reinterpret_cast<uint16_t*>(cache) + slot * D, d0, D, x);
+                else store_run8<KVFP8_BF16, VEC>(reinterpret_cast<uint16_t*>(cache) + slot * D, d0, D, x);
             }
         }
     }
 }
 
-// Gradients. The weights' sums stay in registers over a workgroup's units, join across its rows in LDS in a fixed
-// order, and leave as one partial sum a workgroup and weight.
+// Gradients. The weights' sums stay in registers over a group's tokens, join across the workgroup's groups of a section in LDS
+// in a fixed order, and leave as one partial sum a workgroup and weight.
 template <int DT, int LPR, bool VEC, int kHeads>
-__global__ void __launch_bounds__(kNrThreads)
+__global__ void __launch_bounds__(kNrThreads, 4)
 norm_rope_backward_kernel(NormRopeArgs a) {
     using T = typename Elem<DT>::T;
     constexpr int kGroups = kNrThreads / LPR;
     __shared__ float sums[kGroups][LPR * kNrElems];
     const int D = a.head_dim, lane = threadIdx.x % LPR, group = threadIdx.x / LPR, d0 = kNrElems * lane;
-    const int heads = a.num_q_heads + 2 * a.num_kv_heads, first_v = a.num_q_heads + a.num_kv_heads;
-    const bool normed = a.q_weight != nullptr, summed = a.part != nullptr;
-    float dw[2][kNrElems];
-#pragma unroll
-    for (int i = 0; i < kNrElems; ++i) dw[0][i] = dw[1][i] = 0.0f;
-    const uint32_t stride = gridDim.x * kGroups;
-    for (uint32_t unit = blockIdx.x * kGroups + group; unit < a.total; unit += stride) {
-        const uint32_t token = unit / a.runs;
-        const int h0 = (int)(unit - token * a.runs) * kHeads;
-        const T* const src = reinterpret_cast<const T*>(a.x) + (int64_t)token * a.row_stride;
-        float x[kHeads][kNrElems], g[kHeads][kNrElems];
+    const HeadRun r = head_run<LPR, kHeads>(a);
+    const int heads = a.num_q_heads + 2 * a.num_kv_heads;
+    const bool is_v = r.section == 2, normed = a.q_weight != nullptr && !is_v, summed = a.part != nullptr;
+    const float per_dim = 1.0f / (float)D;
+    float w[kNrElems] = {}, dw[kNrElems] = {};
+    if (normed) load_any<kNrElems, VEC>(r.section == 0 ? a.q_weight : a.k_weight, a.w_dtype, d0, D, w);
+    const T* const grads = reinterpret_cast<const T*>(r.section == 0 ? a.gq : (is_v ? a.gv : a.gk));
+    for (int64_t token = r.token; token < a.rows; token += a.step) {
+        const int64_t pos = is_v ? 0 : index_at(a.positions, a.pos64, token);
+        const T* const src = reinterpret_cast<const T*>(a.x) + token * a.row_stride + (int64_t)(r.before + r.first) * D;
+        Raw<DT, kNrElems> rx[kHeads], rg[kHeads];
 #pragma unroll
         for (int u = 0; u < kHeads; ++u) {
-            const int h = min(h0 + u, heads - 1);
-            const bool is_q = h < a.num_q_heads, is_v = h >= first_v;
-            const int nh = is_q ? a.num_q_heads : a.num_kv_heads, hh = is_q ? h : (is_v ? h - first_v : h - a.num_q_heads);
-            const T* const grad = reinterpret_cast<const T*>(is_q ? a.gq : (is_v ? a.gv : a.gk));
-            if (grad != nullptr) {
-                load_run<DT, kNrElems, VEC>(grad + ((int64_t)token * nh + hh) * D, d0, D, g[u]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kNrElems; ++i) g[u][i] = 0.0f;
-            }
-            if (normed && !is_v) load_run<DT, kNrElems, VEC>(src + (int64_t)h * D, d0, D, x[u]);
+            const int at = min(u, r.count - 1);
+            rx[u] = rg[u] = {};
+            if (grads != nullptr) rg[u] = load_raw<DT, kNrElems, VEC>(grads + (token * r.heads + r.first + at) * D, d0, D);
+            if (normed) rx[u] = load_raw<DT, kNrElems, VEC>(src + (int64_t)at * D, d0, D);
         }
-        Angles t;
-        if (h0 < first_v) t = load_angles<VEC>(a, token, d0);
+        Angles t = {};
+        if (!is_v) t = load_angles<VEC>(a, pos, d0);
 #pragma unroll
         for (int u = 0; u < kHeads; ++u) {
-            const int h = h0 + u;
-            if (h >= heads) break;
-            if (h < first_v) {
+            if (u >= r.count) break;
+            T* const dx = a.dx == nullptr ? nullptr : reinterpret_cast<T*>(a.dx) + (token * heads + r.before + r.first + u) * D;
+            if (is_v) {
+                if (dx != nullptr) store_raw<DT, kNrElems, VEC>(dx, d0, D, rg[u]);
+                continue;
+            }
+            float g[kNrElems];
+            widen(rg[u], g);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float y0 = g[u][2 * i], y1 = g[u][2 * i + 1];
-                    g[u][2 * i] = t.c[i] * y0 + t.s[i] * y1;
-                    g[u][2 * i + 1] = t.c[i] * y1 - t.s[i] * y0;
+            for (int i = 0; i < 4; ++i) {
+                const float y0 = g[2 * i], y1 = g[2 * i + 1];
+                g[2 * i] = t.c[i] * y0 + t.s[i] * y1;
+                g[2 * i + 1] = t.c[i] * y1 - t.s[i] * y0;
+            }
+            if (normed) {
+                float x[kNrElems], sum = 0.0f, dot = 0.0f;
+                widen(rx[u], x);
+#pragma unroll
+                for (int i = 0; i < kNrElems; ++i) {
+                    sum += x[i] * x[i];
+                    dot += (g[i] * w[i]) * x[i];
                 }
-                if (normed) {
-                    const bool is_q = h < a.num_q_heads;
-                    float w[kNrElems], sum = 0.0f, dot = 0.0f;
-                    load_any<kNrElems, VEC>(is_q ? a.q_weight : a.k_weight, a.w_dtype, d0, D, w);
+                const float inv = inverse_root(row_sum<LPR>(sum) * per_dim + a.eps);
+                const float mean = row_sum<LPR>(dot) * inv * per_dim;
 #pragma unroll
-                    for (int i = 0; i < kNrElems; ++i) {
-                        sum += x[u][i] * x[u][i];
-                        dot += (g[u][i] * w[i]) * x[u][i];
-                    }
-                    const float inv = 1.0f / sqrtf(row_sum<LPR>(sum) / (float)D + a.eps);
-                    const float mean = row_sum<LPR>(dot) * inv / (float)D;
-#pragma unroll
-                    for (int i = 0; i < kNrElems; ++i) {
-                        const float xh = x[u][i] * inv, s = g[u][i] * xh;
-                        if (summed) {
-                            dw[0][i] += is_q ? s : 0.0f;
-                            dw[1][i] += is_q ? 0.0f : s;
-                        }
-                        g[u][i] = inv * (g[u][i] * w[i] - xh * mean);
-                    }
+                for (int i = 0; i < kNrElems; ++i) {
+                    const float xh = x[i] * inv;
+                    dw[i] += g[i] * xh;
+                    g[i] = inv * (g[i] * w[i] - xh * mean);
                 }
             }
-            if (a.dx != nullptr)
-                store_run8<DT, VEC>(reinterpret_cast<T*>(a.dx) + ((int64_t)token * heads + h) * D, d0, D, g[u]);
+            if (dx != nullptr) store_run8<DT, VEC>(dx, d0, D, g);
         }
     }
     if (!summed) return;
@@ -313,7 +369,7 @@ norm_rope_backward_kernel(NormRopeArgs a) {
     for (int k = 0; k < 2; ++k) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kNrElems; ++i) sums[group][d0 + i] = dw[k][i];
+        for (int i = 0; i < kNrElems; ++i) sums[group][d0 + i] = r.section == k ? dw[i] : 0.0f;
         __syncthreads();
         for (int d = threadIdx.x; d < D; d += kNrThreads) {
             float total = 0.0f;
@@ -352,7 +408,7 @@ bool nr_index(int d) { return d == KVFP8_I32 || d == KVFP8_I64; }
 int64_t nr_size(int d) { return d == KVFP8_F32 ? 4 : 2; }
 
 constexpr int kNrMaxDim = 64 * kNrElems;
-constexpr int64_t kNrMaxBlocks = (int64_t)1 << 20;
+constexpr int64_t kNrMaxHeads = 4096;
 
 int check_norm_rope(const void* x, int dtype, int64_t rows, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                     int64_t row_stride, const void* positions, int pos_dtype, const void* cos_table, const void* sin_table,
@@ -361,7 +417,7 @@ int check_norm_rope(const void* x, int dtype, int64_t rows, int32_t num_q_heads,
     if (rows < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || head_dim % 2 != 0 || table_rows <= 0)
         return KVFP8_ESHAPE;
     const int64_t heads = (int64_t)num_q_heads + 2 * (int64_t)num_kv_heads;
-    if (head_dim > kNrMaxDim || heads >= ((int64_t)1 << 24) || rows >= ((int64_t)1 << 31) / heads) return KVFP8_ELIMIT;
+    if (head_dim > kNrMaxDim || heads > kNrMaxHeads || rows >= ((int64_t)1 << 31) / heads) return KVFP8_ELIMIT;
     if (rows > 0 && row_stride < 0) return KVFP8_ESTRIDE;
     if ((q_weight == nullptr) != (k_weight == nullptr)) return KVFP8_ENULL;
     if (rows > 0 && (!x || !positions || !cos_table || !sin_table)) return KVFP8_ENULL;
@@ -382,31 +438,36 @@ int lanes_of(int head_dim) {
     return lpr;
 }
 
-// Heads of a run. Few rows: one, for as many workgroups as there are; many: four.
+// Heads of a run. With rows enough for every lane of the device and 16-byte accesses of 16-bit elements four, else one. Forward in
+// microseconds with runs of 1 / 4, bfloat16, 32 + 8 heads of 128: 512 rows 5.6 / 5.5 (below: 1.0 less with one), 1024 rows 8.2 / 6.8,
+// 16384 rows 93 / 73; backward of 16384 rows 139 / 117. float32, whose runs of four need twice the registers: 4096 rows 32 / 36, and
+// backward 56 / 79.
 constexpr int kNrRun = 4;
-int run_of(int64_t rows, int64_t heads, int lanes) {
-    return rows * heads * lanes >= (int64_t)device_cus() * 8 * kNrThreads ? kNrRun : 1;
+int run_of(int64_t rows, int64_t heads, int dtype, bool vec, int lanes) {
+    return vec && dtype != KVFP8_F32 && rows * heads * lanes >= (int64_t)device_cus() * 8 * kNrThreads ? kNrRun : 1;
 }
 
-template <bool kBackward, int DT, int LPR, bool VEC>
-hipError_t launch_norm_rope(const NormRopeArgs& a, int run, unsigned blocks, hipStream_t s) {
-    if constexpr (kBackward) {
-        if (run == 1) hipLaunchKernelGGL((norm_rope_backward_kernel<DT, LPR, VEC, 1>), dim3(blocks), dim3(kNrThreads), 0, s, a);
-        else hipLaunchKernelGGL((norm_rope_backward_kernel<DT, LPR, VEC, kNrRun>), dim3(blocks), dim3(kNrThreads), 0, s, a);
-    } else {
-        if (run == 1) hipLaunchKernelGGL((norm_rope_kernel<DT, LPR, VEC, 1>), dim3(blocks), dim3(kNrThreads), 0, s, a);
-        else hipLaunchKernelGGL((norm_rope_kernel<DT, LPR, VEC, kNrRun>), dim3(blocks), dim3(kNrThreads), 0, s, a);
-    }
+template <bool kBackward, int DT, int LPR, bool VEC, int kHeads>
+hipError_t launch_norm_rope(const NormRopeArgs& a, unsigned blocks, hipStream_t s) {
+    if constexpr (kBackward) hipLaunchKernelGGL((norm_rope_backward_kernel<DT, LPR, VEC, kHeads>), dim3(blocks), dim3(kNrThreads), 0, s, a);
+    else hipLaunchKernelGGL((norm_rope_kernel<DT, LPR, VEC, kHeads>), dim3(blocks), dim3(kNrThreads), 0, s, a);
     return hipGetLastError();
+}
+
+template <bool kBackward, int DT, int LPR>
+hipError_t launch_norm_rope(const NormRopeArgs& a, int run, unsigned blocks, hipStream_t s) {
+    if constexpr (DT != KVFP8_F32)
+        if (run != 1) return launch_norm_rope<kBackward, DT, LPR, true, kNrRun>(a, blocks, s);
+    return launch_norm_rope<kBackward, DT, LPR, true, 1>(a, blocks, s);
 }
 
 template <bool kBackward, int DT>
 hipError_t launch_norm_rope(const NormRopeArgs& a, bool vec, int lanes, int run, unsigned blocks, hipStream_t s) {
-    if (!vec) return launch_norm_rope<kBackward, DT, 64, false>(a, run, blocks, s);
-    if (lanes == 8) return launch_norm_rope<kBackward, DT, 8, true>(a, run, blocks, s);
-    if (lanes == 16) return launch_norm_rope<kBackward, DT, 16, true>(a, run, blocks, s);
-    if (lanes == 32) return launch_norm_rope<kBackward, DT, 32, true>(a, run, blocks, s);
-    return launch_norm_rope<kBackward, DT, 64, true>(a, run, blocks, s);
+    if (!vec) return launch_norm_rope<kBackward, DT, 64, false, 1>(a, blocks, s);
+    if (lanes == 8) return launch_norm_rope<kBackward, DT, 8>(a, run, blocks, s);
+    if (lanes == 16) return launch_norm_rope<kBackward, DT, 16>(a, run, blocks, s);
+    if (lanes == 32) return launch_norm_rope<kBackward, DT, 32>(a, run, blocks, s);
+    return launch_norm_rope<kBackward, DT, 64>(a, run, blocks, s);
 }
 
 template <bool kBackward>
@@ -418,11 +479,19 @@ hipError_t launch_norm_rope(const NormRopeArgs& a, int dtype, bool vec, int lane
     }
 }
 
-// Workgroups of the backward: at most what the device holds at once, as each leaves partial sums. By sizes alone
-// (64 lanes a row, runs of one head), as the workspace is asked for without pointers.
+// Workgroups of the backward: at most what the device holds at once, as each leaves partial sums, and groups for every head of a
+// token. By sizes alone (64 lanes a row, runs of one head), as the workspace is asked for without pointers.
 int64_t backward_blocks(int64_t rows, int64_t heads) {
-    const int64_t per = kNrThreads / 64, most = (int64_t)device_cus() * 4, wanted = (rows * heads + per - 1) / per;
+    const int64_t per = kNrThreads / 64, held = (int64_t)device_cus() * 4, most = held > heads / per + 1 ? held : heads / per + 1;
+    const int64_t wanted = (rows * heads + per - 1) / per;
     return wanted < most ? wanted : most;
+}
+
+// The runs and how many tokens so many workgroups take at once.
+void set_runs(NormRopeArgs& a, int run, int lanes, int64_t blocks) {
+    a.q_runs = (uint32_t)((a.num_q_heads + run - 1) / run);
+    a.kv_runs = (uint32_t)((a.num_kv_heads + run - 1) / run);
+    a.step = (uint32_t)(blocks * (kNrThreads / lanes) / (a.q_runs + 2 * a.kv_runs));
 }
 
 }  // namespace
@@ -488,19 +557,21 @@ extern "C" int kvfp8_norm_rope(const void* x, int dtype, int64_t rows, int32_t n
                                               (uintptr_t)a.v_cache) % 16 == 0;
     const int lanes = vec ? lanes_of(head_dim) : 64;
     const int64_t heads = (int64_t)num_q_heads + 2 * (int64_t)num_kv_heads;
-    const int run = run_of(rows, heads, lanes);
-    a.runs = (uint32_t)((heads + run - 1) / run);
-    a.total = (uint32_t)(rows * a.runs);
-    const int64_t per = kNrThreads / lanes, wanted = (a.total + per - 1) / per;
-    return (int)launch_norm_rope<false>(a, dtype, vec, lanes, run, wanted < kNrMaxBlocks ? wanted : kNrMaxBlocks,
-                                        reinterpret_cast<hipStream_t>(stream));
+    const int run = run_of(rows, heads, dtype, vec, lanes);
+    const int64_t runs = (num_q_heads + run - 1) / run + 2 * (int64_t)((num_kv_heads + run - 1) / run), per = kNrThreads / lanes;
+    // A group takes up to kNrTokens tokens, so that the weights are read seldom, while there are workgroups enough.
+    int64_t tokens = rows * runs / (per * device_cus() * 16);
+    tokens = tokens < 1 ? 1 : (tokens > kNrTokens ? kNrTokens : tokens);
+    const int64_t wanted = ((rows + tokens - 1) / tokens * runs + per - 1) / per;
+    set_runs(a, run, lanes, wanted);
+    return (int)launch_norm_rope<false>(a, dtype, vec, lanes, run, wanted, reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int64_t kvfp8_norm_rope_backward_workspace_bytes(int64_t rows, int32_t num_q_heads, int32_t num_kv_heads,
                                                             int32_t head_dim) {
     if (rows <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0) return 0;
     const int64_t heads = (int64_t)num_q_heads + 2 * (int64_t)num_kv_heads;
-    if (head_dim > kNrMaxDim || heads >= ((int64_t)1 << 24) || rows >= ((int64_t)1 << 31) / heads) return 0;
+    if (head_dim > kNrMaxDim || heads > kNrMaxHeads || rows >= ((int64_t)1 << 31) / heads) return 0;
     return backward_blocks(rows, heads) * 2 * head_dim * 4;
 }
 
@@ -549,9 +620,8 @@ extern "C" int kvfp8_norm_rope_backward(const void* x, int dtype, int64_t rows, 
         const bool vec = nr_vectors(a, dtype) &&
                          ((uintptr_t)grad_q | (uintptr_t)grad_k | (uintptr_t)grad_v | (uintptr_t)dx) % 16 == 0;
         const int lanes = vec ? lanes_of(head_dim) : 64;
-        const int run = run_of(rows, heads, lanes);
-        a.runs = (uint32_t)((heads + run - 1) / run);
-        a.total = (uint32_t)(rows * a.runs);
+        const int run = run_of(rows, heads, dtype, vec, lanes);
+        set_runs(a, run, lanes, blocks);
         const hipError_t err = launch_norm_rope<true>(a, dtype, vec, lanes, run, blocks, s);
         if (err != hipSuccess) return (int)err;
     }

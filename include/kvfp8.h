@@ -485,7 +485,7 @@ int kvfp8_token_logprobs_backward(const void* logits_dev, int dtype, int64_t row
  *   blocks/offsets not NULL: k (before the rounding to x's dtype) and v are also written to a paged cache at
  *   (blocks[r], offsets[r]), by the rule of kvfp8_quantize_append (cache_dtype e4m3fn, with scales) or
  *   kvfp8_store_append (f32/f16/bf16); locations outside the pool are skipped. No two rows share a location.
- * head_dim even, up to 512; rows * (num_q_heads + 2 num_kv_heads) below 2^31. Any alignment; rows, tables, weights and
+ * head_dim even, up to 512; num_q_heads + 2 num_kv_heads up to 4096, times rows below 2^31. Any alignment; rows, tables, weights and
  * outputs that are 16-byte aligned with head_dim a multiple of 8 take wide accesses. The reference has no such norms
  * (its rotation: reference src/torch_llm/model/rope.py:46-55).
  */

@@ -128,3 +128,12 @@ def test_plain_operations_and_the_gradient_formula(weights):
                 moved.append(loss(*(x.view(y.shape) if n == i else y for n, y in enumerate(leaves))).detach())
             # Central differences of 1e-6: 64-bit sums of 100 magnitude give 1e-8, curvature less.
             assert abs(float((moved[0] - moved[1]) / (2 * step)) - float(want.flatten()[j])) < 1e-6
+
+
+@pytest.mark.parametrize("heads, code", [((4094, 1), -3), ((4096, 1), -6), ((2, 2048), -6)])
+def test_entries_refuse_more_than_4096_heads(heads, code):
+    """Of the three the first fits, and is refused for the row stride behind it alone."""
+    args = _entry(hq=heads[0], hkv=heads[1], stride=-1)
+    assert _native.lib().kvfp8_norm_rope(*args, SOME, SOME, SOME, *NO_CACHE) == code
+    assert _native.lib().kvfp8_norm_rope_backward(*args, SOME, SOME, SOME, SOME, SOME, SOME, SOME, 1 << 40, None) == code
+    assert (_native.lib().kvfp8_norm_rope_backward_workspace_bytes(4, *heads, 16) > 0) == (code == -3)
