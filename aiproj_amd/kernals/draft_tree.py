@@ -156,25 +156,27 @@ def accept_draft(tokens: t.Tensor, best: t.Tensor, tree: DraftTree, caches, cach
     seqs, most = starts.shape[0] - 1, tree.max_nodes
     if most == 0:
         raise ValueError(f"{what}: max_nodes is at least 1")
-    shape, dtype, row_bytes, scale_bytes, addresses = (1, 1, 1, 1), None, 1, 0, array("Q")
-    for cache in caches:
-        k, v = cache.k, cache.v
-        parts = (k, v, cache.k_scales, cache.v_scales) if cache.quantized else (k, v)
-        if dtype is None:
-            shape, dtype, quantized = k.shape, k.dtype, cache.quantized
+    shape, row_bytes, scale_bytes, addresses, index, same = (1, 1, 1, 1), 1, 0, array("Q"), device.index, True
+    for i, cache in enumerate(caches):
+        k, v, quantized = cache.k, cache.v, cache.quantized
+        if i == 0:
+            shape, dtype, scaled = k.shape, k.dtype, quantized
             if len(shape) != 4 or shape[1] & (shape[1] - 1) or dtype not in _native.TORCH_TO_CODE:
                 raise ValueError(f"{what}: cache rows [num_blocks, block_size, Hkv, D], the block size a power of two")
-            row_bytes, scale_bytes = shape[2] * shape[3] * k.element_size(), 4 * shape[2] if quantized else 0
-        if k.shape != shape or v.shape != shape or k.dtype != dtype or v.dtype != dtype or cache.quantized != quantized:
+            row_bytes, scale_bytes, scale_shape = shape[2] * shape[3] * k.element_size(), 4 * shape[2] if scaled else 0, shape[:3]
+        if k.shape != shape or v.shape != shape or k.dtype != dtype or v.dtype != dtype or quantized != scaled:
             raise ValueError(f"{what}: caches of one shape and type")
-        if quantized and any(x.dtype != t.float32 or x.shape != shape[:3] for x in parts[2:]):
-            raise ValueError(f"{what}: a quantized cache holds float32 scales per row")
-        for x in parts:
-            if x.get_device() != device.index or not x.is_contiguous():
-                raise ValueError(f"{what}: cache tensors are contiguous and on the tokens' device")
-            addresses.append(x.data_ptr())
-        if not quantized:
-            addresses.extend((0, 0))
+        same = same and k.get_device() == v.get_device() == index and k.is_contiguous() and v.is_contiguous()
+        if scaled:
+            ks, vs = cache.k_scales, cache.v_scales
+            if ks.dtype != t.float32 or vs.dtype != t.float32 or ks.shape != scale_shape or vs.shape != scale_shape:
+                raise ValueError(f"{what}: a quantized cache holds float32 scales per row")
+            same = same and ks.get_device() == vs.get_device() == index and ks.is_contiguous() and vs.is_contiguous()
+            addresses.extend((k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()))
+        else:
+            addresses.extend((k.data_ptr(), v.data_ptr(), 0, 0))
+    if not same:
+        raise ValueError(f"{what}: cache tensors are contiguous and on the tokens' device")
     counts = t.empty(seqs, dtype=t.int32, device=device)
     path = t.empty((seqs, most), dtype=t.int32, device=device)
     next_tokens = t.empty(seqs, dtype=t.int64, device=device)
