@@ -25,6 +25,10 @@ once: with `prefix_len`, `prefill(prompts, prefix)` runs it through the model as
 and the prompts and every later step behind it (`kernals/shared_prefix_attention.py`). With
 `logprobs`, every step records the log probability of the token it chose, the entropy and that many
 alternatives (`kernals/token_logprobs.py`) in `scores`, rows in decode order like `history`.
+
+Drafted continuations, from whatever proposes them, are checked in one pass with `verify(drafts)`
+(`kernals/draft_tree.py`): every sequence gains the tokens of the path that the model would have chosen
+step by step, and its choice behind them.
 """
 
 from __future__ import annotations
@@ -33,6 +37,7 @@ import torch as t
 
 from aiproj_amd.inference.page_allocator import CacheContainer, PageAllocator
 from aiproj_amd.inference.paged_kv_cache import PagedKVCache
+from aiproj_amd.kernals.draft_tree import DraftTree, accept_draft
 from aiproj_amd.kernals.shared_prefix_attention import SharedPrefix
 from aiproj_amd.kernals.token_logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 from aiproj_amd.model.transformer import StepMeta, TransformerLM
@@ -167,3 +172,35 @@ class GreedyDecoder:
         """Advance the allocator's committed lengths (host and device) by the `steps`
         tokens each sequence's decode steps wrote into the cache."""
         self.allocator.advance_batch(list(range(self.batch)), [steps] * self.batch)
+
+    def verify(self, drafts: list[tuple[list[int], list[int]]]) -> list[list[int]]:
+        """One pass over the model's choice and a tree of guesses behind it, for each sequence: `drafts[i]` is the guessed
+        tokens and the number of the node that each follows, 0 the last chosen token and n the n-th guess. Returns what each
+        sequence gains: the guesses that the model agrees with, and its next choice. The tokens are committed, and step,
+        generate or verify go on behind them; `history` has steps only. Reads the result on the host."""
+        if self.prefix is not None or self.logprobs is not None:
+            raise ValueError("GreedyDecoder: verify takes neither a shared prefix nor logprobs")
+        if self.slots is None or len(drafts) != self.batch:
+            raise ValueError("GreedyDecoder: verify takes a draft for each sequence, after prefill")
+        if any(len(guesses) != len(above) or any(p < 0 for p in above) for guesses, above in drafts):
+            raise ValueError("GreedyDecoder: a draft is guesses and the node that each follows")
+        sizes = [1 + len(guesses) for guesses, _ in drafts]
+        lengths = [self.allocator.get_seq_len(i) for i in range(self.batch)]
+        if any(n + size > self.max_len for n, size in zip(lengths, sizes)):
+            raise ValueError(f"GreedyDecoder: a draft passes the {self.max_len} tokens that are reserved")
+        parents = [[-1, *above] for _, above in drafts]
+        tree = DraftTree.from_parents(parents, self.device)
+        nodes, depths, tokens = t.tensor([[i for n in sizes for i in range(n)], [d for own in DraftTree.depths(parents) for d in own],
+                                          [x for guesses, _ in drafts for x in (0, *guesses)]], device=self.device)
+        tokens[tree.starts[:-1].long()] = self.tokens
+        held = self.allocator.seq_lens[self.slots].long().repeat_interleave(t.tensor(sizes, device=self.device), output_size=len(nodes))
+        ctx = self.allocator.create_container(self.slots, tree.starts, held + nodes, validate=False)
+        logits = self.model(tokens, StepMeta("verify", held + depths, ctx, tree=tree), self.caches)
+        got = accept_draft(tokens, logits.argmax(-1), tree, self.caches, ctx)
+        self.tokens.copy_(got.next_tokens)
+        self.positions.add_(got.counts)
+        self.context_lengths.add_(got.counts)
+        counts, path, last = got.counts.tolist(), got.path.tolist(), got.next_tokens.tolist()
+        self.allocator.advance_batch(list(range(self.batch)), counts)
+        self.steps_left = min(self.steps_left, self.max_len - max(n + c for n, c in zip(lengths, counts)))
+        return [[*(drafts[i][0][node - 1] for node in path[i][1:counts[i]]), last[i]] for i in range(self.batch)]

@@ -26,7 +26,9 @@ the projections and the FFN are `RowLinear`: the HIP kernel `skinny_linear_kerne
 few rows of a decode step, which then also does RoPE and the activation, plain GEMMs (hipBLASLt through torch) otherwise; prompt
 (prefill) attention is the varlen causal HIP kernel behind `flash_attention_forward`,
 as the reference calls its FlashAttentionFunction there (`attention.py:103-110`). Sequences that
-share a prefix in the cache (`StepMeta.prefix`) attend it through `shared_prefix_attention`.
+share a prefix in the cache (`StepMeta.prefix`) attend it through `shared_prefix_attention`, trees of drafted
+tokens (mode "verify") through `tree_attention`. With `ModelConfig.qk_norm` every query and key head has an RMSNorm
+before its rotation (the reference has none): both and the cache write are one launch of `norm_rope_kernel`.
 """
 
 from __future__ import annotations
@@ -39,10 +41,12 @@ from torch import nn
 from torch.nn import functional as F
 
 from aiproj_amd import _native
-from aiproj_amd.kernals.decode_attention import append_decode_attention
+from aiproj_amd.kernals.decode_attention import append_decode_attention, decode_attention_wrapper
+from aiproj_amd.kernals.draft_tree import DraftTree, append_tree_attention, tree_attention
 from aiproj_amd.kernals.flash_attention import flash_attention_forward
+from aiproj_amd.kernals.norm_rope import norm_rope_append
 from aiproj_amd.kernals.shared_prefix_attention import (SharedPrefix, append_shared_prefix_decode_attention,
-                                                        shared_prefix_prefill_attention)
+                                                        shared_prefix_decode_attention, shared_prefix_prefill_attention)
 from aiproj_amd.model.rmsnorm import add_rmsnorm, rmsnorm_forward
 
 
@@ -59,19 +63,21 @@ class ModelConfig:
     rms_eps: float = 1e-5
     max_seq_len: int = 2048
     init_std: float = 0.02
+    qk_norm: bool = False              # RMSNorm of every query and key head before the rotation
 
 
 @dataclass
 class StepMeta:
     """What one forward needs besides the tokens (the reference's BatchMeta)."""
 
-    mode: str                          # "prefill" or "decode"
+    mode: str                          # "prefill", "decode" or "verify" (the nodes of drafted trees)
     token_positions: t.Tensor          # [T] int64, position of every packed token
     cache_context: object              # CacheContainer: slots, physical_blocks, block_offsets, ...
     cu_seqlens: t.Tensor | None = None  # prefill only: [B + 1] offsets of the packed prompts (device)
     max_seqlen: int = 0                 # prefill only: longest prompt (host int)
     prefix: SharedPrefix | None = None  # prefixes in the cache that the sequences continue
     all_logits: bool = False            # prefill only: logits of every token, not of each prompt's last
+    tree: DraftTree | None = None       # verify only
 
 
 class RoPE(nn.Module):
@@ -206,11 +212,18 @@ class Attention(nn.Module):
         self.qkv_proj = RowLinear(cfg.d_model, self.q_dim + 2 * self.kv_dim)
         self.o_proj = RowLinear(self.q_dim, cfg.d_model)
         self.rope = RoPE(cfg.head_dim, cfg.max_seq_len, cfg.rope_theta)
+        if cfg.qk_norm:
+            self.q_norm = nn.Parameter(t.ones(cfg.head_dim))
+            self.k_norm = nn.Parameter(t.ones(cfg.head_dim))
 
     def forward(self, h: t.Tensor, meta: StepMeta, cache) -> t.Tensor:
         cfg = self.cfg
         ctx = meta.cache_context
         proj = self.qkv_proj
+        if (meta.mode == "verify") != (meta.tree is not None) or (meta.tree is not None and meta.prefix is not None):
+            raise ValueError("Attention: mode verify comes with a tree, and without a shared prefix")
+        if cfg.qk_norm:
+            return self._normed(proj(h), meta, cache)
         # A decode step's rotation is done by the projection's kernel (`kvfp8_skinny_linear_rope`).
         if (meta.mode != "prefill" and h.shape[0] <= _SKINNY_ROWS and isinstance(proj, RowLinear) and proj.unobserved()
                 and not RoPE.replaced(self.rope) and proj.weight.shape[0] == self.q_dim + 2 * self.kv_dim
@@ -230,6 +243,24 @@ class Attention(nn.Module):
         self.rope.apply_(qkv, meta.token_positions, cfg.num_q_heads + cfg.num_kv_heads)
         return self._attend(qkv, meta, cache)
 
+    def _normed(self, qkv: t.Tensor, meta: StepMeta, cache) -> t.Tensor:
+        """Norms, rotation and cache write of fused rows, then the attention and the output projection."""
+        cfg, ctx, rope = self.cfg, meta.cache_context, self.rope
+        if RoPE.replaced(rope):
+            raise ValueError("Attention: qk_norm rotates with the tables of this module's RoPE")
+        prompts = meta.mode == "prefill"
+        got = norm_rope_append(qkv, meta.token_positions, rope.cos_table, rope.sin_table, cfg.num_q_heads, cfg.num_kv_heads,
+                               self.q_norm, self.k_norm, cfg.rms_eps, cache, ctx.physical_blocks, ctx.block_offsets, packed=prompts)
+        if prompts:
+            out = self._attend_prompts(*got, meta, cache)
+        elif meta.mode == "verify":
+            out = tree_attention(got, cache, ctx, meta.tree)
+        elif meta.prefix is not None:
+            out = shared_prefix_decode_attention(got, cache, ctx, meta.prefix)
+        else:
+            out = decode_attention_wrapper(got, cache, ctx)
+        return self.o_proj(out.reshape(-1, self.q_dim))
+
     def _attend_prompts(self, q: t.Tensor, k: t.Tensor, v: t.Tensor, meta: StepMeta, cache) -> t.Tensor:
         scale = 1.0 / math.sqrt(self.cfg.head_dim)
         if meta.prefix is not None:
@@ -248,6 +279,8 @@ class Attention(nn.Module):
             # q, k and v are views into the fused projection; the kernel takes packed rows.
             out = self._attend_prompts(q.contiguous(), k.contiguous(), v.contiguous(), meta, cache)
             cache.append_kv(ctx.physical_blocks, ctx.block_offsets, k, v)
+        elif meta.mode == "verify":
+            out = append_tree_attention(q, k, v, cache, ctx, meta.tree)
         elif meta.prefix is not None:
             out = append_shared_prefix_decode_attention(q, k, v, cache, ctx, meta.prefix)
         else:
@@ -316,8 +349,8 @@ class TransformerLM(nn.Module):
 
     @t.no_grad()
     def forward(self, tokens: t.Tensor, meta: StepMeta, caches) -> t.Tensor:
-        """Logits [B, vocab]: of every token in decode mode (one per sequence), of each
-        prompt's last token in prefill mode (of every token with `all_logits`)."""
+        """Logits [B, vocab]: of every token in decode mode (one per sequence) and in verify mode (every node), of
+        each prompt's last token in prefill mode (of every token with `all_logits`)."""
         eps = self.cfg.rms_eps
         x = self.embed(tokens)
         h, _ = rmsnorm_forward(x, self.layers[0].mixer_norm, eps)

@@ -1,0 +1,220 @@
+"""Drafted trees and normed heads in the decoder model: GreedyDecoder.verify, and the operators as it runs them together."""
+
+import pytest
+import torch as t
+
+from aiproj_amd.inference.greedy_decoder import GreedyDecoder
+from aiproj_amd.inference.page_allocator import PageAllocator
+from aiproj_amd.inference.paged_kv_cache import PagedKVCache
+from aiproj_amd.kernals.shared_prefix_attention import SharedPrefix
+from aiproj_amd.model.transformer import ModelConfig, StepMeta, TransformerLM
+
+SIZES = dict(vocab_size=256, d_model=256, num_layers=2, num_q_heads=8, num_kv_heads=2, head_dim=64, d_ff=512, max_seq_len=256)
+# Logits of one model through two orders of its products, as the decoder model's other tests take them.
+RTOL, ATOL = 3e-2, 1e-1
+
+
+def _model(qk_norm, dtype=t.bfloat16):
+    g = t.Generator(device="cuda").manual_seed(3)
+    model = TransformerLM(ModelConfig(**SIZES, qk_norm=qk_norm)).to(device="cuda", dtype=dtype).init_weights(g).eval()
+    if qk_norm:
+        with t.no_grad():
+            for layer in model.layers:
+                for w in (layer.attn.q_norm, layer.attn.k_norm):
+                    w.copy_(1.0 + 0.3 * t.randn(w.shape, generator=g, device="cuda"))
+    return model
+
+
+@pytest.fixture(scope="module", params=[False, True], ids=["plain", "qk_norm"])
+def model(request):
+    return _model(request.param)
+
+
+def _tokens(*shape, seed=0):
+    return t.randint(0, SIZES["vocab_size"], shape, generator=t.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def _whole_logits(model, row):
+    """Logits of every token of one sequence, as a prompt."""
+    n = len(row)
+    alloc = PageAllocator(-(-n // 16), 16, 1, n, "cuda")
+    caches = [PagedKVCache(alloc.num_blocks, 16, 2, 64, "cuda", t.bfloat16) for _ in range(SIZES["num_layers"])]
+    slots, cu, pos = t.tensor([alloc.allocate_request(0, n)], device="cuda"), t.tensor([0, n], dtype=t.int32, device="cuda"), t.arange(n, device="cuda")
+    ctx = alloc.create_container(slots, cu, pos, validate=False)
+    return model(row, StepMeta("prefill", pos, ctx, cu_seqlens=cu, max_seqlen=n, all_logits=True), caches).float()
+
+
+class _Watched:
+    """The model, with the last call's logits kept."""
+
+    def __init__(self, model):
+        self.model, self.cfg = model, model.cfg
+
+    def __call__(self, tokens, meta, caches):
+        self.tokens, self.logits = tokens, self.model(tokens, meta, caches)
+        return self.logits
+
+
+def _plain_forward(model, row):
+    """The model in float64 from its formulas, logits of every token."""
+    cfg, x = model.cfg, model.embed.weight.double()[row]
+    norm = lambda y, w: y / t.sqrt((y * y).mean(-1, keepdim=True) + cfg.rms_eps) * w.double()
+    rope = model.layers[0].attn.rope
+    c, s = rope.cos_table[:len(row)].double()[:, None], rope.sin_table[:len(row)].double()[:, None]
+    turn = lambda y: t.stack([c * y[..., ::2] - s * y[..., 1::2], s * y[..., ::2] + c * y[..., 1::2]], -1).flatten(-2)
+    for layer in model.layers:
+        a = layer.attn
+        qkv = (norm(x, layer.mixer_norm) @ a.qkv_proj.weight.double().T).unflatten(1, (-1, cfg.head_dim))
+        q, k, v = qkv.split([cfg.num_q_heads, cfg.num_kv_heads, cfg.num_kv_heads], 1)
+        q, k = turn(norm(q, a.q_norm)), turn(norm(k, a.k_norm))
+        k, v = (y.repeat_interleave(cfg.num_q_heads // cfg.num_kv_heads, 1) for y in (k, v))
+        outs = []
+        for h in range(cfg.num_q_heads):
+            scores = q[:, h] @ k[:, h].T.contiguous() / cfg.head_dim ** 0.5
+            outs.append(scores.masked_fill(t.ones_like(scores).triu(1).bool(), float("-inf")).softmax(-1) @ v[:, h].contiguous())
+        x = x + t.stack(outs, 1).flatten(1) @ a.o_proj.weight.double().T
+        gate, up = (norm(x, layer.ffn_norm) @ layer.ffn.gate_up.weight.double().T).chunk(2, -1)
+        x = x + (t.nn.functional.silu(gate) * up) @ layer.ffn.down.weight.double().T
+    return norm(x, model.final_norm) @ model.embed.weight.double().T
+
+
+@pytest.mark.gpu
+def test_normed_heads_against_the_formulas():
+    model, row = _model(True), _tokens(70, seed=4)
+    t.testing.assert_close(_whole_logits(model, row).double(), _plain_forward(model, row), rtol=RTOL, atol=ATOL)
+
+
+@pytest.mark.gpu
+def test_normed_heads_decode_like_a_prompt():
+    """Eight forced steps after a prompt, and behind a shared prefix."""
+    model, rows = _model(True), _tokens(3, 30, seed=5)
+    want = [_whole_logits(model, row) for row in rows]
+    for prefix in (0, 13):
+        own = rows if prefix == 0 else t.cat([rows[:1, :prefix].expand(3, -1), rows[:, prefix:]], 1)
+        want = [_whole_logits(model, row) for row in own]
+        decoder = GreedyDecoder(model, 3, 30 - prefix, cache_dtype=t.bfloat16, prefix_len=prefix)
+        decoder.prefill(own[:, prefix:22], own[0, :prefix] if prefix else None)
+        for i in range(22, 30):
+            decoder.tokens.copy_(own[:, i])
+            got = decoder.step().float()
+            for b in range(3):
+                t.testing.assert_close(got[b], want[b][i], rtol=RTOL, atol=ATOL)
+
+
+# Guesses follow node 0, each other in a chain, or branch; a draft without guesses is a plain step.
+TREES = [([0, 1, 2, 3], [0, 0, 1, 1, 2, 5, 0], []), ([0, 0, 0], [0, 1, 1, 3, 3, 5, 6, 7, 8, 9, 10], [0])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache_dtype", [t.bfloat16, t.float8_e4m3fn])
+def test_verified_drafts(model, cache_dtype):
+    """Rounds of drafts whose guesses are partly the model's choices. Each round's logits are those of the nodes' paths as prompts;
+    the tokens gained are the walk along them; and the cache holds the kept nodes: the next round and the last step rest on it."""
+    batch, length, watched = 3, 21, _Watched(model)
+    decoder = GreedyDecoder(watched, batch, 100, cache_dtype=cache_dtype)
+    prompts = _tokens(batch, length, seed=6)
+    first = decoder.prefill(prompts)
+    text = [[*prompts[b].tolist(), int(first[b])] for b in range(batch)]
+    tol = dict(rtol=RTOL, atol=ATOL) if cache_dtype == t.bfloat16 else dict(rtol=RTOL, atol=4 * ATOL)   # codes: 2^-4 against 2^-9
+    gained = 0
+    for turn in range(4):
+        trees = TREES[turn % 2]
+        drafts = []
+        for b in range(batch):
+            guesses, paths = [], [text[b]]
+            for n, above in enumerate(trees[b]):
+                best = _whole_logits(model, t.tensor(paths[above], device="cuda"))[-1].topk(3).indices.tolist()
+                guesses.append(best[(n + turn) % 3 if n % 3 == 2 else 0])
+                paths.append([*paths[above], guesses[-1]])
+            drafts.append((guesses, trees[b]))
+        new = decoder.verify(drafts)
+        start = 0
+        for b, (guesses, above) in enumerate(drafts):
+            logits = watched.logits[start:start + 1 + len(guesses)].float()
+            assert watched.tokens[start].item() == text[b][-1]
+            start += len(logits)
+            paths = [text[b]]
+            for g, p in zip(guesses, above):
+                paths.append([*paths[p], g])
+            for node, path in enumerate(paths):
+                t.testing.assert_close(logits[node], _whole_logits(model, t.tensor(path, device="cuda"))[-1], **tol)
+            best, at, walk = logits.argmax(-1).tolist(), 0, []
+            while True:
+                walk.append(best[at])
+                below = [n for n in range(1, len(paths)) if above[n - 1] == at and guesses[n - 1] == best[at]]
+                if not below:
+                    break
+                at = below[0]
+            assert new[b] == walk
+            gained += len(walk)
+            text[b] += walk
+            assert decoder.allocator.get_seq_len(b) == len(text[b]) - 1
+    assert gained > 4 * batch                                  # some guesses were kept, or nothing was moved
+    assert decoder.tokens.tolist() == [x[-1] for x in text]
+    got = decoder.step().float()
+    for b in range(batch):
+        t.testing.assert_close(got[b], _whole_logits(model, t.tensor(text[b], device="cuda"))[-1], **tol)
+    assert decoder.context_lengths.tolist() == [len(x) + 1 for x in text]
+
+
+@pytest.mark.gpu
+def test_captured_steps_go_on_behind_a_draft(model):
+    """A step's graph captured before a draft, replayed after it: lengths and positions are its buffers'."""
+    decoder, other = (GreedyDecoder(model, 2, 60, cache_dtype=t.bfloat16) for _ in range(2))
+    prompts = _tokens(2, 17, seed=8)
+    for d in (decoder, other):
+        d.prefill(prompts)
+    decoder.generate(3)
+    other.generate(3, use_graph=False)
+    drafts = [([5, 6], [0, 0]), ([7], [0])]
+    assert decoder.verify(drafts) == other.verify(drafts)
+    assert t.equal(decoder.generate(4), other.generate(4, use_graph=False))
+
+
+@pytest.mark.gpu
+def test_drafts_up_to_the_last_reserved_token(model):
+    decoder = GreedyDecoder(model, 1, 24)
+    decoder.prefill(_tokens(1, 20, seed=9))
+    with pytest.raises(ValueError, match="reserved"):
+        decoder.verify([([1] * 4, [0, 1, 2, 3])])
+    got = decoder.verify([([1] * 3, [0, 1, 2])])
+    assert decoder.steps_left == 24 - 20 - len(got[0])
+    with pytest.raises(AssertionError):
+        decoder.generate(decoder.steps_left + 1)
+
+
+def test_refused_drafts():
+    cpu = TransformerLM(ModelConfig(**SIZES))
+    decoder = GreedyDecoder(cpu, 2, 40, cache_dtype=t.float32, device="cpu")
+    with pytest.raises(ValueError, match="after prefill"):
+        decoder.verify([([], []), ([], [])])
+    decoder.slots = t.tensor([decoder.allocator.allocate_request(i, 40) for i in range(2)])
+    for drafts, match in (([([], [])], "each sequence"), ([([], []), ([3], [])], "node that each"), ([([], []), ([3], [-1])], "node that each"),
+                          ([([], []), ([3], [1])], "parents before"), ([([], []), ([3] * 40, list(range(40)))], "reserved")):
+        with pytest.raises(ValueError, match=match):
+            decoder.verify(drafts)
+    for more in (dict(prefix_len=4), dict(logprobs=2)):
+        other = GreedyDecoder(cpu, 2, 40, cache_dtype=t.float32, device="cpu", **more)
+        other.prefix = SharedPrefix.one(0, 4, 2, "cpu") if "prefix_len" in more else None
+        with pytest.raises(ValueError, match="shared prefix nor logprobs"):
+            other.verify([([], []), ([], [])])
+
+
+def test_refused_steps():
+    attn = TransformerLM(ModelConfig(**SIZES, qk_norm=True)).layers[0].attn
+    h = t.zeros(1, SIZES["d_model"])
+    with pytest.raises(ValueError, match="verify comes with a tree"):
+        attn(h, StepMeta("verify", t.zeros(1), None), None)
+    with pytest.raises(ValueError, match="verify comes with a tree"):
+        attn(h, StepMeta("decode", t.zeros(1), None, tree=object()), None)
+    with pytest.raises(ValueError, match="without a shared prefix"):
+        attn(h, StepMeta("verify", t.zeros(1), None, tree=object(), prefix=object()), None)
+    attn.rope.apply_ = lambda *a: None
+    with pytest.raises(ValueError, match="this module's RoPE"):
+        attn(h, StepMeta("decode", t.zeros(1), None), None)
+
+
+def test_plain_models_keep_their_parameters():
+    names = set(dict(TransformerLM(ModelConfig(**SIZES)).named_parameters()))
+    normed = set(dict(TransformerLM(ModelConfig(**SIZES, qk_norm=True)).named_parameters()))
+    assert normed - names == {f"layers.{i}.attn.{n}" for i in range(2) for n in ("q_norm", "k_norm")} and not names - normed
