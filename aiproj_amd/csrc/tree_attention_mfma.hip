@@ -156,40 +156,56 @@ tree_narrow_kernel(TreeArgs a) {
 }
 
 // The states of sequences of several chunks, zeros where a sequence has no tokens. A wave takes `run` pairs (row, q head), so
-// that few waves look for their sequence.
+// that few waves look for their sequence, and up to four pairs of a row at once, so that their states are read together.
 template <int C, int QT>
 __global__ void __launch_bounds__(256)
 tree_join_kernel(TreeArgs a, int32_t run) {
-    constexpr int kLanes = 16 * C, kPass = 64 / kLanes;
+    constexpr int kLanes = 16 * C, kPass = 64 / kLanes, kPairs = 4;
     using T = typename Elem<QT>::T;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int D = a.d.head_dim;
     const int32_t units = (int32_t)a.rows * a.d.num_q_heads, begin = ((int32_t)blockIdx.x * 4 + wave) * run;
-    if (begin >= units) return;
+    const int32_t end = min(begin + run, units);
+    if (begin >= end) return;
     const TreeCut c = cut_batch(a);
     const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
     const int d4 = min(lane % kLanes, D / 4 - 1), po = lane / kLanes;
     TreeItem it;
     bool found = false;
     int32_t last = -1;
-    for (int32_t unit = begin; unit < min(begin + run, units); ++unit) {
+    for (int32_t unit = begin; unit < end;) {
         const int32_t row = (uint32_t)unit / (uint32_t)a.d.num_q_heads, hq = unit - row * a.d.num_q_heads;
+        const int32_t count = min(min(kPairs, end - unit), a.d.num_q_heads - hq);
         if (row != last && !(found && row - it.s.row0 < it.s.nodes)) found = find_tree_item<true>(a, c, row, it);
         last = row;
-        if (!found || it.chunks == 1) continue;
-        const int32_t h = (uint32_t)hq / (uint32_t)G, pair = (row - it.s.row0) * G + (hq - h * G);
-        const int32_t block = (uint32_t)pair / (uint32_t)a.block_rows;
-        const int64_t stride = (int64_t)a.d.num_kv_heads * it.blocks * a.block_rows;
-        const int64_t first = ((int64_t)it.first + (int64_t)h * it.blocks + block) * a.block_rows + (pair - block * a.block_rows);
-        JoinedState st;
-#pragma unroll 4
-        for (int i = po; i < it.chunks; i += kPass) {
-            const int64_t at = first + i * stride;
-            st.add(a.d.part_m[at], a.d.part_l[at], reinterpret_cast<const float4*>(a.d.part_acc + at * D)[d4]);
+        if (!found || it.chunks == 1) {
+            unit += count;
+            continue;
         }
-        st.across<kLanes>();
-        if (po != 0 || 4 * (lane % kLanes) >= D) continue;
-        st.store<QT>(reinterpret_cast<T*>(a.d.out) + (int64_t)unit * D + 4 * d4);
+        const int64_t stride = (int64_t)a.d.num_kv_heads * it.blocks * a.block_rows;
+        int64_t first[kPairs];
+#pragma unroll
+        for (int u = 0; u < kPairs; ++u) {
+            const int32_t q = hq + min(u, count - 1), h = (uint32_t)q / (uint32_t)G, pair = (row - it.s.row0) * G + (q - h * G);
+            const int32_t block = (uint32_t)pair / (uint32_t)a.block_rows;
+            first[u] = ((int64_t)it.first + (int64_t)h * it.blocks + block) * a.block_rows + (pair - block * a.block_rows);
+        }
+        JoinedState st[kPairs];
+#pragma unroll 2
+        for (int i = po; i < it.chunks; i += kPass) {
+#pragma unroll
+            for (int u = 0; u < kPairs; ++u) {
+                const int64_t at = first[u] + i * stride;
+                st[u].add(a.d.part_m[at], a.d.part_l[at], reinterpret_cast<const float4*>(a.d.part_acc + at * D)[d4]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kPairs; ++u) {
+            if (u >= count) break;
+            st[u].template across<kLanes>();
+            if (po == 0 && 4 * (lane % kLanes) < D) st[u].template store<QT>(reinterpret_cast<T*>(a.d.out) + (int64_t)(unit + u) * D + 4 * d4);
+        }
+        unit += count;
     }
 }
 
