@@ -20,6 +20,10 @@
 //   32, 16, 4080, 32 / 8                            184       118        83       116        88
 //   61, 1 to 60, 1 to 3060, 16 / 4                  221       153       144       163       118
 //   8, 64, 32768, 32 / 8                            951       576       419       402       399
+// The vector ALU and the matrix cores bound it where there are rows enough: per step 215 and 16 instructions, of which two waves a
+// SIMD hide little from each other. The waves' priority is higher at the loads and the products (8 sequences of 32768 tokens: 377 us
+// with it, 399 without), and all of a step's operands leave LDS at its begin (393 against 403). With one row block HBM bounds it: 32
+// sequences of 4096 tokens 74 us without the join, 269 MB, 3.6 TB/s.
 #include "joined_state.h"
 #include "shared_prefix_narrow.h"
 #include "tree_attention.h"
@@ -230,6 +234,7 @@ tree_block_kernel(TreeArgs a) {
                 }
             }
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
         f32x16_t sc;
 #pragma unroll
         for (int u = 0; u < 2 * C * ES; ++u) {
@@ -240,6 +245,7 @@ tree_block_kernel(TreeArgs a) {
                 sc = mma32<kF16>(kx[u], q[u], u == 0 ? f32x16_t{} : sc);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         if constexpr (ES == 1) {
 #pragma unroll
             for (int x = 0; x < 16; ++x) sc[x] *= ks[x >> 2][x & 3];
@@ -317,6 +323,7 @@ tree_block_kernel(TreeArgs a) {
                 }
             }
         }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int pp = 0; pp < 2; ++pp) {
             u32x4_t keep = {~0u, ~0u, ~0u, ~0u};         // bytes or 16-bit values by token
@@ -336,6 +343,7 @@ tree_block_kernel(TreeArgs a) {
                 for (int part = 0; part < kParts; ++part) o[nb] = mma32<kF16V>(av, pop[part][pp], o[nb]);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         if constexpr (!kWhole) {
 #pragma unroll 1
             for (uint32_t left = odd; left != 0; left &= left - 1) {
@@ -367,7 +375,9 @@ tree_block_kernel(TreeArgs a) {
         __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(R::kPerStep * (S - 2)) : "memory");
         __builtin_amdgcn_s_barrier();
         __asm__ volatile("" ::: "memory");
+        __builtin_amdgcn_s_setprio(2);
         push((int)((uint32_t)(n + S - 1) % (uint32_t)S));
+        __builtin_amdgcn_s_setprio(0);
     };
     const int32_t rounds = (end - w.lo + stride - 1) / stride;
     const int32_t plain = uniform((min(min(end, held), paged_until(a, w)) - w.lo) / stride);
