@@ -1,9 +1,14 @@
 """Attention of drafted trees against float64 over the cache as it is stored."""
 
+import math
+import random
+from types import SimpleNamespace
+
 import pytest
 import torch as t
 
 from aiproj_amd.inference.paged_kv_cache import PagedKVCache
+from aiproj_amd.kernals import draft_tree
 from aiproj_amd.kernals.decode_attention import decode_attention_wrapper
 from aiproj_amd.kernals.draft_tree import DraftTree, append_tree_attention, tree_attention
 from tests import draft_tree_cases as cases
@@ -277,3 +282,28 @@ def test_no_rows_and_no_sequences():
     assert tree_attention(c.q[:0], c.cache, c.ctx, DraftTree(c.tree.starts, c.tree.parents[:0], 4)).shape == (0, 4, 64)
     c.ctx.cache_slots, c.ctx.context_lengths = c.ctx.cache_slots[:0], c.ctx.context_lengths[:0]
     assert tree_attention(c.q, c.cache, c.ctx, DraftTree(c.tree.starts[:1], c.tree.parents, 4)).shape == (2, 4, 64)
+
+
+@pytest.mark.parametrize("q_dtype,cache_dtype", [(F16, FP8), (BF16, BF16), (F32, FP8), (F16, F32)])
+@pytest.mark.parametrize("batch", [64, 150])
+def test_more_columns_than_run_at_once(q_dtype, cache_dtype, batch):
+    """Sequences of all lengths, which are then taken in the order of their lengths, 64 by 64."""
+    rng = random.Random(batch)
+    held = [rng.choice((0, 1, 15, 40, 64, 90, 150)) for _ in range(batch)]
+    held[batch // 2], held[-1] = 1700, 900
+    c = cases.case(held, [rng.randint(0, 20) for _ in range(batch)], 32, 8, 64, q_dtype, cache_dtype)
+    c.ctx.context_lengths[3], c.ctx.cache_slots[9] = -1, -1
+    _check(c, tree_attention(c.q, c.cache, c.ctx, c.tree))
+
+
+@pytest.mark.parametrize("form", [FORMS[0], FORMS[1], FORMS[9], FORMS[17]])
+def test_scales_of_either_sign(form, monkeypatch):
+    """A negative scale is that of the negated queries, and 0 weighs all tokens alike."""
+    hq, hkv, d, q_dtype, cache_dtype, page = form
+    c = cases.case([70, 5], [20, 9], hq, hkv, d, q_dtype, cache_dtype, page)
+    for root, factor in ((lambda d: -math.sqrt(d), -1.0), (lambda d: float("inf"), 0.0)):
+        monkeypatch.setattr(draft_tree, "math", SimpleNamespace(sqrt=root))
+        got, q = tree_attention(c.q, c.cache, c.ctx, c.tree), c.q
+        c.q = q * factor
+        _check(c, got)
+        c.q = q
