@@ -409,6 +409,7 @@ int64_t nr_size(int d) { return d == KVFP8_F32 ? 4 : 2; }
 
 constexpr int kNrMaxDim = 64 * kNrElems;
 constexpr int64_t kNrMaxHeads = 4096;
+constexpr int64_t kNrMaxBlocks = (int64_t)1 << 20;        // of a launch, which holds less than 2^32 threads
 
 int check_norm_rope(const void* x, int dtype, int64_t rows, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                     int64_t row_stride, const void* positions, int pos_dtype, const void* cos_table, const void* sin_table,
@@ -562,7 +563,8 @@ extern "C" int kvfp8_norm_rope(const void* x, int dtype, int64_t rows, int32_t n
     // A group takes up to kNrTokens tokens, so that the weights are read seldom, while there are workgroups enough.
     int64_t tokens = rows * runs / (per * device_cus() * 16);
     tokens = tokens < 1 ? 1 : (tokens > kNrTokens ? kNrTokens : tokens);
-    const int64_t wanted = ((rows + tokens - 1) / tokens * runs + per - 1) / per;
+    int64_t wanted = ((rows + tokens - 1) / tokens * runs + per - 1) / per;
+    wanted = wanted < kNrMaxBlocks ? wanted : kNrMaxBlocks;
     set_runs(a, run, lanes, wanted);
     return (int)launch_norm_rope<false>(a, dtype, vec, lanes, run, wanted, reinterpret_cast<hipStream_t>(stream));
 }

@@ -295,3 +295,21 @@ def test_on_another_stream():
         got = norm_rope(*cases.args(s))
     t.cuda.current_stream().wait_stream(side)
     assert all(t.equal(a, b) for a, b in zip(got, want))
+
+
+def test_more_rows_than_workgroups():
+    """Rows of a few elements, so many that a launch's workgroups take more of them each than they would else."""
+    n, d = 6_000_000, 2
+    gen = t.Generator(device="cuda").manual_seed(1)
+    x, w = t.randn(n, 3 * d, generator=gen, device="cuda"), t.tensor([0.5, 2.0], device="cuda")
+    pos = t.arange(n, device="cuda", dtype=t.int32) % 50
+    angle = t.arange(50, device="cuda", dtype=t.float64)[:, None]
+    cos, sin = angle.cos().float(), angle.sin().float()
+    q, k, v = norm_rope(x, pos, cos, sin, 1, 1, w, w, 1e-5)
+    heads = x.double().view(n, 3, d)[:, :2]
+    y = heads / t.sqrt((heads * heads).mean(-1, keepdim=True) + 1e-5) * w.double()
+    c, s = (z.double()[pos.long()][:, None] for z in (cos, sin))
+    want = t.stack([c[..., 0] * y[..., 0] - s[..., 0] * y[..., 1], s[..., 0] * y[..., 0] + c[..., 0] * y[..., 1]], -1)
+    # Sixteen half steps of float32 of either product, as in _slack.
+    bound = (d / 2 + 16) * 2.0 ** -24 * y.abs().sum(-1, keepdim=True)
+    assert bool(((t.cat([q, k], 1).double() - want).abs() <= bound).all()) and t.equal(v[:, 0], x[:, 2 * d:])
