@@ -184,12 +184,16 @@ class GreedyDecoder:
             raise ValueError("GreedyDecoder: verify takes a draft for each sequence, after prefill")
         if any(len(guesses) != len(above) or any(p < 0 for p in above) for guesses, above in drafts):
             raise ValueError("GreedyDecoder: a draft is guesses and the node that each follows")
+        if any(not 0 <= x < self.model.cfg.vocab_size for guesses, _ in drafts for x in guesses):
+            raise ValueError("GreedyDecoder: a guess is a token of the model's vocabulary")
         sizes = [1 + len(guesses) for guesses, _ in drafts]
         lengths = [self.allocator.get_seq_len(i) for i in range(self.batch)]
         if any(n + size > self.max_len for n, size in zip(lengths, sizes)):
             raise ValueError(f"GreedyDecoder: a draft passes the {self.max_len} tokens that are reserved")
         parents = [[-1, *above] for _, above in drafts]
         tree = DraftTree.from_parents(parents, self.device)
+        if self.positions.tolist() != lengths:
+            raise ValueError("GreedyDecoder: commit the steps before a draft")
         nodes, depths, tokens = t.tensor([[i for n in sizes for i in range(n)], [d for own in DraftTree.depths(parents) for d in own],
                                           [x for guesses, _ in drafts for x in (0, *guesses)]], device=self.device)
         tokens[tree.starts[:-1].long()] = self.tokens

@@ -188,9 +188,12 @@ def test_refused_drafts():
     decoder = GreedyDecoder(cpu, 2, 40, cache_dtype=t.float32, device="cpu")
     with pytest.raises(ValueError, match="after prefill"):
         decoder.verify([([], []), ([], [])])
+    decoder.positions[1] = 3                                   # as after steps that were not committed
     decoder.slots = t.tensor([decoder.allocator.allocate_request(i, 40) for i in range(2)])
     for drafts, match in (([([], [])], "each sequence"), ([([], []), ([3], [])], "node that each"), ([([], []), ([3], [-1])], "node that each"),
-                          ([([], []), ([3], [1])], "parents before"), ([([], []), ([3] * 40, list(range(40)))], "reserved")):
+                          ([([], []), ([3], [1])], "parents before"), ([([], []), ([3] * 40, list(range(40)))], "reserved"),
+                          ([([], []), ([256], [0])], "vocabulary"), ([([], []), ([-1], [0])], "vocabulary"),
+                          ([([], []), ([3], [0])], "commit the steps")):
         with pytest.raises(ValueError, match=match):
             decoder.verify(drafts)
     for more in (dict(prefix_len=4), dict(logprobs=2)):
