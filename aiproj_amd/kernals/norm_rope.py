@@ -10,9 +10,10 @@ functions take). Both happen in float32 with one rounding to the rows' type, one
 
 * `norm_rope(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, q_weight, k_weight, eps) -> (q, k, v)`:
   packed q [T, Hq, D], k and v [T, Hkv, D] of rows [T, (Hq + 2 Hkv) D] (float32, float16 or bfloat16, unit element
-  stride, any row stride). Differentiable once in qkv and both weights: one launch of `norm_rope_backward_kernel` and
-  one for the weights (`kvfp8_norm_rope_backward`), sums in a fixed order. Calls and gradients that a transform, mode or
-  trace looks at take PyTorch operations in float32, which have derivatives of every kind and order.
+  stride, any row stride). Differentiable once in qkv and both weights (tables that require gradients are refused): one
+  launch of `norm_rope_backward_kernel` and one for the weights (`kvfp8_norm_rope_backward`), sums in a fixed order. Calls
+  and gradients that a transform, mode or trace looks at take PyTorch operations in float32, which have derivatives of
+  every kind and order.
 * `norm_rope_append(..., eps, paged_kv_cache, physical_blocks, block_offsets, packed=False)`: the same, and k and v
   written to the paged cache on the way: what `append_kv` writes of them, where k is quantized (or stored) from its
   float32 values, without the rounding to the rows' type before. Returns q, or (q, k, v) with `packed`, for the attention
@@ -25,6 +26,8 @@ most 512. The reference has neither (its rotation: `model/rope.py:46-55`).
 """
 
 from __future__ import annotations
+
+import functools
 
 import torch as t
 
@@ -72,6 +75,12 @@ def _operands(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d
             code[positions.dtype], cos_table.data_ptr(), sin_table.data_ptr(), code[cos_table.dtype], cos_table.shape[0],
             ptr(q_weight), ptr(k_weight), code[t.float32 if q_weight is None else q_weight.dtype], float(eps))
     return args, (qkv, positions, cos_table, sin_table, q_weight, k_weight)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(rows, num_q_heads, num_kv_heads, d) -> int:
+    """kvfp8_norm_rope_backward_workspace_bytes, which depends on shapes only (cached per shape)."""
+    return _native.lib().kvfp8_norm_rope_backward_workspace_bytes(rows, num_q_heads, num_kv_heads, d)
 
 
 _NO_CACHE = (None, _native.I64, None, _native.I64, 0, 0, None, None, _native.E4M3FN, None, None)
@@ -146,7 +155,7 @@ class NormRopeFunction(t.autograd.Function):
             dk = t.empty_like(k_weight, memory_format=t.contiguous_format) if wanted[2] else None
             size = 0
             if dq is not None or dk is not None:
-                size = _native.lib().kvfp8_norm_rope_backward_workspace_bytes(rows, num_q_heads, num_kv_heads, d)
+                size = _workspace_bytes(rows, num_q_heads, num_kv_heads, d)
             workspace = t.empty(max(size, 1), dtype=t.uint8, device=qkv.device)
             args, keep = _operands(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, q_weight, k_weight, eps)
             ptr = _native.ptr
@@ -164,6 +173,8 @@ def norm_rope(qkv: t.Tensor, positions: t.Tensor, cos_table: t.Tensor, sin_table
     if not _native.is_plain(*given):
         _native.require_gpu(*given, what=what)
         return _plain(*args)
+    if t.is_grad_enabled() and (cos_table.requires_grad or sin_table.requires_grad):
+        raise ValueError(f"{what}: the tables have no gradients")
     if t.is_grad_enabled() and any(x is not None and x.requires_grad for x in (qkv, q_weight, k_weight)):
         return NormRopeFunction.apply(*args)
     return _forward(*args, what)

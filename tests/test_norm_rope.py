@@ -137,3 +137,13 @@ def test_entries_refuse_more_than_4096_heads(heads, code):
     assert _native.lib().kvfp8_norm_rope(*args, SOME, SOME, SOME, *NO_CACHE) == code
     assert _native.lib().kvfp8_norm_rope_backward(*args, SOME, SOME, SOME, SOME, SOME, SOME, SOME, 1 << 40, None) == code
     assert (_native.lib().kvfp8_norm_rope_backward_workspace_bytes(4, *heads, 16) > 0) == (code == -3)
+
+
+@pytest.mark.parametrize("which", ["cos", "sin"])
+def test_tables_with_gradients_are_refused(which):
+    s = cases.rows(3, 2, 1, 8, t.float32, t.float32, device="cpu")
+    getattr(s, which).requires_grad_()
+    with pytest.raises(ValueError, match="tables have no gradients"):
+        norm_rope(*cases.args(s))
+    with t.no_grad(), pytest.raises(RuntimeError):          # without gradients the rows' device is what is wrong
+        norm_rope(*cases.args(s))
