@@ -180,7 +180,6 @@ def norm_rope(qkv: t.Tensor, positions: t.Tensor, cos_table: t.Tensor, sin_table
     return _forward(*args, what)
 
 
-@t.no_grad()
 def norm_rope_append(qkv: t.Tensor, positions: t.Tensor, cos_table: t.Tensor, sin_table: t.Tensor, num_q_heads: int,
                      num_kv_heads: int, q_weight: t.Tensor | None, k_weight: t.Tensor | None, eps: float, paged_kv_cache,
                      physical_blocks: t.Tensor, block_offsets: t.Tensor, packed: bool = False):
@@ -202,7 +201,8 @@ def norm_rope_append(qkv: t.Tensor, positions: t.Tensor, cos_table: t.Tensor, si
             raise ValueError(f"{what}: a quantized cache holds float8_e4m3fn and float32 scales per row")
     elif k_cache.dtype not in _DTYPES:
         raise ValueError(f"{what}: unsupported cache dtype {k_cache.dtype}")
-    if any(x is not None and not x.is_contiguous() for x in (k_cache, v_cache, k_scales, v_scales)):
+    scales = k_scales is None or k_scales.is_contiguous() and v_scales.is_contiguous()
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and scales):
         raise ValueError(f"{what}: cache tensors must be contiguous")
     device = _native.require_gpu(qkv, positions, cos_table, sin_table, q_weight, k_weight, k_cache, v_cache, k_scales, v_scales,
                                  blocks, offsets, what=what)
