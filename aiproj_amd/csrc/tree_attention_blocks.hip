@@ -5,8 +5,11 @@
 // widens the codes on the way from there. Per step (MFMA 32x32x16: A[row = l % 32][k = 8 (l / 32) + i], B likewise,
 // D[row = 8 (i / 4) + 4 (l / 32) + i % 4][col = l % 32]):
 //   S^T[token, pair] = K Q^T    A = K rows, 16 bytes a lane and read; B = Q^T, loaded once
-//   softmax                     t = score x (k_scale x sm_scale x log2(e)), e2(t - reference), float32, online, base 2; the
-//                               reference follows a pair's maximum only where that exceeds it by 2^8
+//   softmax                     t = (score x sm_scale x log2(e)) x k_scale, e2(t - reference), float32, online, base 2; the
+//                               reference follows a pair's maximum only where that exceeds it by 2^8. The product is rounded
+//                               before the reference, which is such a product, is taken off: fused, the largest key's weight
+//                               would be 2^(what its rounding took off), infinite or 0 from scores of 2^31 on (the operation
+//                               more costs 0 to 2% of a call; with k_scale x sm_scale first, 2% to 6% for f16 q)
 //   O^T[d, pair] += V^T P'^T    P' = e2() v_scale from the score registers: score i of lane l is token 8 (i / 4) + 4 (l / 32)
 //                               + i % 4, so a product of 16 tokens takes scores 8 pp .. + 7 of both halves; V^T by transposing
 //                               reads of those rows
@@ -153,9 +156,6 @@ tree_block_kernel(TreeArgs a) {
     for (int i = 0; i + 1 < S; ++i) push(i);
 
     // Q^T operands: lane (pair l % 32 of the tile, l / 32); pairs past the last repeat it and are never stored.
-    // With the scale's sign, so that the largest score is that of the largest product.
-    const float scale = fabsf(a.d.score_scale);
-    const uint32_t turn = a.d.score_scale < 0.0f ? 0x80008000u : 0u;
     u32x4_t q[KS];
     const int32_t pair = min(w.r0 + 32 * tile + col, w.pairs - 1), node = (uint32_t)pair / (uint32_t)G;
     const int32_t hq = w.h * G + (pair - node * G);
@@ -173,7 +173,7 @@ tree_block_kernel(TreeArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[e] = (uint32_t)p[2 * e] | ((uint32_t)p[2 * e + 1] << 16);
             }
-            q[s] = inside ? x ^ turn : u32x4_t{0u, 0u, 0u, 0u};
+            q[s] = inside ? x : u32x4_t{0u, 0u, 0u, 0u};
         }
     }
     if (end > held) build_masks(lds.masks, a, w.it.s);
@@ -246,6 +246,8 @@ tree_block_kernel(TreeArgs a) {
             }
         }
         __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) sc[x] *= a.d.score_scale;
         if constexpr (ES == 1) {
 #pragma unroll
             for (int x = 0; x < 16; ++x) sc[x] *= ks[x >> 2][x & 3];
@@ -287,7 +289,6 @@ tree_block_kernel(TreeArgs a) {
         float mx = sc[0];
 #pragma unroll
         for (int x = 1; x < 16; ++x) mx = fmaxf(mx, sc[x]);
-        mx *= scale;
         if (__ballot(mx > lim)) {
             const float top = max_across_halves(mx);
             const bool fresh = lim == kNegInf;
@@ -307,7 +308,7 @@ tree_block_kernel(TreeArgs a) {
                 float y[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float p = fast_exp2(__builtin_fmaf(sc[4 * g + 2 * v + e], scale, -ref));
+                    const float p = fast_exp2(sc[4 * g + 2 * v + e] - ref);
                     l += p;
                     y[e] = ES == 1 ? p * vs[g][2 * v + e] : p;
                     if (!kWhole && ((gone >> (8 * g + 4 * hi + 2 * v + e)) & 1) != 0) y[e] = 0.0f;
@@ -354,7 +355,7 @@ tree_block_kernel(TreeArgs a) {
                 s = __shfl(s, 32 * ((tt >> 2) & 1) + col);
                 if (s == kNegInf) continue;              // it does not count for the pair (or at a weight of 0)
                 const int64_t row = ((tt < 16 ? refs.a.row0 : refs.b.row0) + (tt & 15)) * a.d.num_kv_heads + w.h;
-                const float weight = fast_exp2(__builtin_fmaf(s, scale, -ref)) * (ES == 1 ? a.d.v_scales[row] : 1.0f);
+                const float weight = fast_exp2(s - ref) * (ES == 1 ? a.d.v_scales[row] : 1.0f);
 #pragma unroll
                 for (int nb = 0; nb < N; ++nb)
 #pragma unroll
