@@ -294,7 +294,9 @@ tree_block_kernel(TreeArgs a) {
             const bool fresh = lim == kNegInf;
             const float to = fresh ? (top == kNegInf ? 0.0f : top) : fmaxf(top, ref);
             const float alpha = fresh ? 0.0f : fast_exp2(ref - to);
-            lim = fresh && top == kNegInf ? kNegInf : to + kTreeLag;
+            // From 2^27 on the sum may round to 2^4 more, and a weight of 2^16 is past float16's numbers.
+            const float most = to + kTreeLag;
+            lim = fresh && top == kNegInf ? kNegInf : (most - to > kTreeLag ? to : most);
             ref = to;
             l *= alpha;
 #pragma unroll

@@ -1,5 +1,7 @@
 """Attention of drafted trees at scores of any size, against float64."""
 
+import math
+
 import pytest
 import torch as t
 
@@ -85,3 +87,24 @@ def test_outlier_channels_of_float16(form):
     c.q = t.zeros_like(c.q)
     c.q[..., 0] = 6e4
     _check(c, form, tree_attention(c.q, c.cache, c.ctx, c.tree), 30)
+
+
+def test_scores_a_step_past_what_the_reference_allows():
+    """A reference at which 2^8 more rounds to 2^16 more: the weights of the scores there are past float16's largest number. Tokens 0,
+    128, .. have a score of 134601552 (base 2), tokens 64, 192, .. the next float32, 16 above it."""
+    held, d = 250, 64
+    c = cases.case([held] * 80, [1] * 80, 16, 8, d, F16, F16)
+    gen = t.Generator(device="cpu").manual_seed(1)
+    for b in range(80):
+        k, v = t.zeros(held + 1, 8, d), t.randn(held + 1, 8, d, generator=gen).clamp(-3, 3)
+        k[::64, :, 0] = 13016.0
+        k[64::128, :, 1] = 1.0
+        _write(c, b, k, v)
+    c.q = t.zeros_like(c.q)
+    c.q[..., 0], c.q[..., 1] = 57344.0, 64.0
+    got = tree_attention(c.q, c.cache, c.ctx, c.tree)
+    rows, want, size = cases.attention_64(c)
+    # The scores are 8 apart (base e), their float32 values 11: the lower ones weigh e^-8 or e^-11, of values up to 3 that are not the
+    # higher ones'. The others are roundings.
+    bound = HALF[F16] * want.abs() + (HALF[F16] + 2.0 ** -12) * size + 2.0 ** -25 + 2 * 3 * math.exp(-8)
+    assert bool(got.isfinite().all()) and bool(((got[rows].double() - want).abs() <= bound).all())
