@@ -331,7 +331,9 @@ prefix_wide_kernel(PrefixArgs a, PrefixGrid grid) {
         const bool fresh = lim == kNegInf;
         const float to = fresh ? (top == kNegInf ? 0.0f : top) : fmaxf(top, ref);
         alpha = fresh ? 0.0f : __builtin_amdgcn_exp2f(ref - to);
-        lim = fresh && top == kNegInf ? kNegInf : to + kLag;
+        // From 2^27 on the sum may round to 2^4 more, and a weight of 2^16 is past float16's numbers.
+        const float most = to + kLag;
+        lim = fresh && top == kNegInf ? kNegInf : (most - to > kLag ? to : most);
         ref = to;
         l *= alpha;
         return true;
