@@ -121,6 +121,7 @@ struct TreeCut {
 struct TreeItem {
     TreeSeq s;
     int32_t first;                    // number of the sequence's first item
+    int32_t first_state;              // where the states of its items begin, which sequences of several chunks have
     int32_t blocks;                   // row blocks of the sequence
     int32_t chunks;                   // of its columns
 };
@@ -218,11 +219,12 @@ __device__ __forceinline__ TreeCut cut_batch(const TreeArgs& a) {
 // The sequence that holds item `index` (kByRow: that computes row `index`); false without one.
 template <bool kByRow>
 __device__ __forceinline__ bool find_tree_item(const TreeArgs& a, const TreeCut& c, int32_t index, TreeItem& it) {
-    int32_t before = 0;
+    int32_t before = 0, before_states = 0;
     TreeSeq s = c.s;
     for (int b0 = 0;;) {
         const int32_t blocks = tree_blocks(a, s), chunks = tree_chunks(s, c.chunk), items = blocks * a.d.num_kv_heads * chunks;
-        const int32_t incl = sum_up_to(items);
+        const int32_t states = chunks > 1 ? items : 0;
+        const int32_t incl = sum_up_to(items), incl_states = sum_up_to(states);
         const int32_t first = before + incl - items;
         const uint64_t hit = __ballot(kByRow ? index >= s.row0 && index - s.row0 < s.nodes : index >= first && index - first < items);
         if (hit != 0) {
@@ -235,9 +237,11 @@ __device__ __forceinline__ bool find_tree_item(const TreeArgs& a, const TreeCut&
             it.blocks = __builtin_amdgcn_readlane(blocks, at);
             it.chunks = __builtin_amdgcn_readlane(chunks, at);
             it.first = __builtin_amdgcn_readlane(first, at);
+            it.first_state = before_states + __builtin_amdgcn_readlane(incl_states - states, at);
             return true;
         }
         before += __builtin_amdgcn_readlane(incl, 63);
+        before_states += __builtin_amdgcn_readlane(incl_states, 63);
         b0 += 64;
         if (b0 >= a.seqs) return false;
         s = sorted_seq(a, b0);
@@ -247,7 +251,7 @@ __device__ __forceinline__ bool find_tree_item(const TreeArgs& a, const TreeCut&
 // What a workgroup does: pairs (node, q head of KV head h) from r0 on against the tokens [lo, hi).
 struct TreeWork {
     TreeItem it;
-    int32_t index;                    // of the item
+    int32_t state;                    // number of the item's states, where its sequence has several chunks
     int32_t h, r0, pairs, lo, hi;
     const int32_t* table;             // block-table row
 };
@@ -258,10 +262,11 @@ struct TreeWork {
 __device__ __forceinline__ bool tree_work(const TreeArgs& a, TreeWork& w) {
     const TreeCut c = cut_batch(a);
     const uint32_t local = blockIdx.x / kXcdCount, turn = local / (uint32_t)kXcdRun;
-    w.index = (int32_t)((turn * kXcdCount + blockIdx.x % kXcdCount) * kXcdRun + (local - turn * kXcdRun));
-    if (w.index >= uniform(c.total) || !find_tree_item<false>(a, c, w.index, w.it)) return false;
+    const int32_t index = (int32_t)((turn * kXcdCount + blockIdx.x % kXcdCount) * kXcdRun + (local - turn * kXcdRun));
+    if (index >= uniform(c.total) || !find_tree_item<false>(a, c, index, w.it)) return false;
     const int32_t G = (uint32_t)a.d.num_q_heads / (uint32_t)a.d.num_kv_heads;
-    uint32_t rest = (uint32_t)(w.index - w.it.first);
+    uint32_t rest = (uint32_t)(index - w.it.first);
+    w.state = w.it.first_state + (int32_t)rest;
     const uint32_t column = rest / (uint32_t)w.it.blocks;
     w.r0 = (int32_t)(rest - column * (uint32_t)w.it.blocks) * a.block_rows;
     rest = column / (uint32_t)a.d.num_kv_heads;

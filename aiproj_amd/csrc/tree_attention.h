@@ -10,7 +10,7 @@ bool tree_mfma_supported(int32_t head_dim, int32_t block_size, int q_dtype, int 
 struct TreePlan {
     int32_t block_rows, target;
     int64_t items;                    // at most
-    int64_t part_l, part_acc, bytes;  // float32 states of items x block_rows pairs: m at 0, l and acc at these byte offsets
+    int64_t part_l, part_acc, bytes;  // float32 states of block_rows pairs an item: m at 0, l and acc at these byte offsets
 };
 TreePlan tree_mfma_plan(int32_t seqs, int32_t max_nodes, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int q_dtype);
 

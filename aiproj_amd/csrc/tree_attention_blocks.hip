@@ -426,7 +426,7 @@ tree_block_kernel(TreeArgs a) {
     l = sum_across_halves(l);
     if (w.r0 + 32 * tile + col >= w.pairs) return;
     if (w.it.chunks > 1) {
-        const int64_t at = (int64_t)w.index * a.block_rows + 32 * tile + col;
+        const int64_t at = (int64_t)w.state * a.block_rows + 32 * tile + col;
         if (hi == 0) {
             a.d.part_m[at] = m;
             a.d.part_l[at] = l;

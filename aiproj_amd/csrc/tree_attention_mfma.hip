@@ -140,7 +140,7 @@ tree_narrow_kernel(TreeArgs a) {
     const float l = sum_across_rows(st.l);
     if (w.r0 + m16 >= w.pairs) return;
     if (w.it.chunks > 1) {
-        store_state<C>(a.d, (int64_t)w.index * a.block_rows + m16, st, l, D, j);
+        store_state<C>(a.d, (int64_t)w.state * a.block_rows + m16, st, l, D, j);
         return;
     }
     float* const out = reinterpret_cast<float*>(a.d.out) + ((int64_t)(w.it.s.row0 + node) * a.d.num_q_heads + hq) * D;
@@ -189,7 +189,7 @@ tree_join_kernel(TreeArgs a, int32_t run) {
         for (int u = 0; u < kPairs; ++u) {
             const int32_t q = hq + min(u, count - 1), h = (uint32_t)q / (uint32_t)G, pair = (row - it.s.row0) * G + (q - h * G);
             const int32_t block = (uint32_t)pair / (uint32_t)a.block_rows;
-            first[u] = ((int64_t)it.first + (int64_t)h * it.blocks + block) * a.block_rows + (pair - block * a.block_rows);
+            first[u] = ((int64_t)it.first_state + (int64_t)h * it.blocks + block) * a.block_rows + (pair - block * a.block_rows);
         }
         JoinedState st[kPairs];
 #pragma unroll 2
@@ -234,9 +234,10 @@ TreePlan tree_mfma_plan(int32_t seqs, int32_t max_nodes, int32_t num_q_heads, in
     p.block_rows = narrow ? 16 : 64;
     p.target = device_cus() * (narrow ? 1 : 2);          // workgroups that a CU holds
     const int64_t columns = (int64_t)seqs * ((pairs + p.block_rows - 1) / p.block_rows) * num_kv_heads;
-    // A chunk is at least the work divided by the target, so there are that many whole ones at most, and a column's last.
+    // A chunk is at least the work divided by the target, so there are that many whole ones at most, and a column's last. Columns
+    // of several chunks, whose items alone leave states, have fewer than two for each whole one.
     p.items = p.target + columns;
-    const int64_t states = p.items * p.block_rows;
+    const int64_t states = (p.items < 2 * p.target ? p.items : 2 * p.target) * p.block_rows;
     p.part_l = (int64_t)tree_align((size_t)states * 4);
     p.part_acc = 2 * p.part_l;
     p.bytes = p.part_acc + (int64_t)tree_align((size_t)states * head_dim * 4);
