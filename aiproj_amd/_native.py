@@ -232,6 +232,19 @@ def is_plain(*tensors: torch.Tensor) -> bool:
     return True
 
 
+def refuse_gradients(*tensors, what: str) -> None:
+    """For an operator without derivatives: its results would have none of a graph that is being recorded, or of dual
+    tensors, and nothing would say so."""
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                raise ValueError(f"{what}: no gradients; call it under torch.no_grad(), or with detached tensors")
+    if _forward_ad._current_level >= 0:
+        for x in tensors:
+            if x is not None and _forward_ad.unpack_dual(x).tangent is not None:
+                raise ValueError(f"{what}: no forward-mode derivatives; call it with the primal tensors")
+
+
 def require_gpu(*tensors, what: str) -> torch.device:
     """All tensors on one GPU device; the FP8 path has no CPU implementation. The common
     case compares device indices (get_device: -1 on the CPU) without building device

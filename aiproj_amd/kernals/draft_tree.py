@@ -25,7 +25,8 @@ size 64 or 128 with q of their type, pages of 16 tokens and more, 16-byte aligne
 to a vector-ALU kernel.
 
 Nothing is synchronized with the host and no device value is read: trees, lengths and pages may change between replays of a
-captured call. No gradients. The reference has no counterpart: a decode step there has one new token a sequence
+captured call. No gradients: queries, keys and values that require them are refused while a graph is recorded, and dual
+tensors always. The reference has no counterpart: a decode step there has one new token a sequence
 (`kernals/decode_attention.py:39-191`).
 """
 
@@ -114,6 +115,7 @@ def tree_attention(q: t.Tensor, paged_kv_cache, cache_batch_context, tree: Draft
         raise ValueError(f"{what}: one parent a row of q")
     if q.dtype not in _Q_DTYPES:
         raise ValueError(f"{what}: unsupported q dtype {q.dtype}")
+    _native.refuse_gradients(q, what=what)
     device = _native.require_gpu(q, k, v, k_scales, v_scales, table, starts, parents, slots, lens, what=what)
     output = t.empty((rows, hq, d), dtype=q.dtype, device=device)
     seqs = starts.shape[0] - 1
@@ -137,6 +139,7 @@ def tree_attention(q: t.Tensor, paged_kv_cache, cache_batch_context, tree: Draft
 def append_tree_attention(q: t.Tensor, ks: t.Tensor, vs: t.Tensor, paged_kv_cache, cache_batch_context, tree: DraftTree) -> t.Tensor:
     """`paged_kv_cache.append_kv(ctx.physical_blocks, ctx.block_offsets, ks, vs)` and the attention over the cache with the nodes."""
     ctx = cache_batch_context
+    _native.refuse_gradients(q, ks, vs, what="append_tree_attention")
     paged_kv_cache.append_kv(ctx.physical_blocks, ctx.block_offsets, ks, vs)
     return tree_attention(q, paged_kv_cache, ctx, tree)
 

@@ -17,8 +17,8 @@ functions take). Both happen in float32 with one rounding to the rows' type, one
 * `norm_rope_append(..., eps, paged_kv_cache, physical_blocks, block_offsets, packed=False)`: the same, and k and v
   written to the paged cache on the way: what `append_kv` writes of them, where k is quantized (or stored) from its
   float32 values, without the rounding to the rows' type before. Returns q, or (q, k, v) with `packed`, for the attention
-  of prompts. No gradients. Token locations as in `append_kv`: those outside the pool are skipped (padded rows), and no
-  two rows share one.
+  of prompts. No gradients: inputs that require them are refused while a graph is recorded, and dual tensors always. Token
+  locations as in `append_kv`: those outside the pool are skipped (padded rows), and no two rows share one.
 
 `q_weight` and `k_weight` may both be None: rotation alone, in float32 with one rounding (`RoPE.split` rounds after
 every operation, as the reference does). Positions outside the tables leave the normed rows unrotated. D is even and at
@@ -204,6 +204,7 @@ def norm_rope_append(qkv: t.Tensor, positions: t.Tensor, cos_table: t.Tensor, si
     scales = k_scales is None or k_scales.is_contiguous() and v_scales.is_contiguous()
     if not (k_cache.is_contiguous() and v_cache.is_contiguous() and scales):
         raise ValueError(f"{what}: cache tensors must be contiguous")
+    _native.refuse_gradients(qkv, cos_table, sin_table, q_weight, k_weight, what=what)
     device = _native.require_gpu(qkv, positions, cos_table, sin_table, q_weight, k_weight, k_cache, v_cache, k_scales, v_scales,
                                  blocks, offsets, what=what)
     q = _empty(rows, num_q_heads, d, qkv)
