@@ -118,7 +118,7 @@ def _plain(qkv, positions, cos_table, sin_table, num_q_heads, num_kv_heads, d, q
         if w is not None:
             part = part / t.sqrt(part.square().mean(-1, keepdim=True) + eps) * w.float()
         out.append(_turn(part, cos, sin).to(qkv.dtype))
-    return *out, x[:, num_q_heads + num_kv_heads:].to(qkv.dtype)
+    return *out, x[:, num_q_heads + num_kv_heads:].to(qkv.dtype, copy=True)
 
 
 class NormRopeFunction(t.autograd.Function):
