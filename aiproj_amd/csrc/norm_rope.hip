@@ -18,7 +18,7 @@
 // Bound by HBM: 16384 tokens of 32 + 8 heads of 128 in bfloat16 take 73 us forward (403 MB, 5.5 TB/s) and 122 us backward (570 MB,
 // 4.7 TB/s); 65536 tokens of 16 + 4 heads with packed outputs and an e4m3fn cache 190 us (873 MB, 4.6 TB/s). Sums across a row's
 // lanes by DPP, the hardware's reciprocal root and 16-bit roundings in pairs keep the vector ALU below that.
-#include "kvfp8_common.h"
+#include "kvfp8_decode_common.h"
 #include "mfma_tiles.h"
 
 namespace kvfp8 {
@@ -65,10 +65,6 @@ struct NormRopeArgs {
     void* dx;                             // null: not wanted
     float* part;                          // [workgroups][2][head_dim] sums for the weights, null: not wanted
 };
-
-__device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) {
-    return is64 ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t)reinterpret_cast<const int32_t*>(p)[i];
-}
 
 // Elements d0 .. d0 + N - 1 of a row of type DT as they are stored, zeros past D. VEC: the row starts at a multiple of the access
 // and D is a multiple of N.
@@ -232,15 +228,15 @@ norm_rope_kernel(NormRopeArgs a) {
     if (a.q_weight != nullptr && !is_v) load_any<kNrElems, VEC>(r.section == 0 ? a.q_weight : a.k_weight, a.w_dtype, d0, D, w);
     T* const outs = reinterpret_cast<T*>(r.section == 0 ? a.q_out : (is_v ? a.v_out : a.k_out));
     for (int64_t token = r.token; token < a.rows; token += a.step) {
-        const int64_t pos = is_v ? 0 : index_at(a.positions, a.pos64, token);
+        const int64_t pos = is_v ? 0 : load_i(a.positions, a.pos64, token);
         const T* const src = reinterpret_cast<const T*>(a.x) + token * a.row_stride + (int64_t)(r.before + r.first) * D;
         Raw<DT, kNrElems> raw[kHeads];
 #pragma unroll
         for (int u = 0; u < kHeads; ++u) raw[u] = load_raw<DT, kNrElems, VEC>(src + (int64_t)min(u, r.count - 1) * D, d0, D);
         int64_t block = -1, offset = -1;
         if (cached) {
-            block = index_at(a.blocks, a.blocks64, token);
-            offset = index_at(a.offsets, a.offsets64, token);
+            block = load_i(a.blocks, a.blocks64, token);
+            offset = load_i(a.offsets, a.offsets64, token);
         }
         const bool inside = block >= 0 && block < a.num_blocks && offset >= 0 && offset < a.block_size;
         Angles g = {};
@@ -316,7 +312,7 @@ norm_rope_backward_kernel(NormRopeArgs a) {
     if (normed) load_any<kNrElems, VEC>(r.section == 0 ? a.q_weight : a.k_weight, a.w_dtype, d0, D, w);
     const T* const grads = reinterpret_cast<const T*>(r.section == 0 ? a.gq : (is_v ? a.gv : a.gk));
     for (int64_t token = r.token; token < a.rows; token += a.step) {
-        const int64_t pos = is_v ? 0 : index_at(a.positions, a.pos64, token);
+        const int64_t pos = is_v ? 0 : load_i(a.positions, a.pos64, token);
         const T* const src = reinterpret_cast<const T*>(a.x) + token * a.row_stride + (int64_t)(r.before + r.first) * D;
         Raw<DT, kNrElems> rx[kHeads], rg[kHeads];
 #pragma unroll
