@@ -15,8 +15,8 @@
 // token after another: the weights and their gradients' sums stay in registers, the heads of a token share the angles, and their
 // loads are issued together.
 //
-// Bound by HBM: 16384 tokens of 32 + 8 heads of 128 in bfloat16 take 73 us forward (403 MB, 5.5 TB/s) and 122 us backward (570 MB,
-// 4.7 TB/s); 65536 tokens of 16 + 4 heads with packed outputs and an e4m3fn cache 190 us (873 MB, 4.6 TB/s). Sums across a row's
+// Bound by HBM: 16384 tokens of 32 + 8 heads of 128 in bfloat16 take 73 us forward (403 MB, 5.5 TB/s) and 118 us backward (570 MB,
+// 4.8 TB/s); 65536 tokens of 16 + 4 heads with packed outputs and an e4m3fn cache 187 us (873 MB, 4.7 TB/s). Sums across a row's
 // lanes by DPP, the hardware's reciprocal root and 16-bit roundings in pairs keep the vector ALU below that.
 #include "kvfp8_decode_common.h"
 #include "mfma_tiles.h"
@@ -144,7 +144,9 @@ __device__ __forceinline__ float row_sum(float x) {
     return bits_f32(row_fold<LPR>(f32_bits(x), [](uint32_t a, uint32_t b) { return f32_bits(bits_f32(a) + bits_f32(b)); }));
 }
 
-// 1 / sqrt(x): the hardware's estimate (one unit in the last place) but for subnormal numbers, which it takes for zeros.
+// 1 / sqrt(x): the hardware's estimate (one unit in the last place) but for subnormal numbers, which it takes for zeros. A root and a
+// division instead would round twice, half a unit each. It moves a quantized row's scale by as much, and a code only where a value lies
+// that close to a border (none of 524288 codes of normal rows on the CPU, for a root one unit off).
 __device__ __forceinline__ float inverse_root(float x) {
     return x < 1.17549435e-38f ? 1.0f / sqrtf(x) : __builtin_amdgcn_rsqf(x);
 }
@@ -437,7 +439,7 @@ int lanes_of(int head_dim) {
 
 // Heads of a run. With rows enough for every lane of the device and 16-byte accesses of 16-bit elements four, else one. Forward in
 // microseconds with runs of 1 / 4, bfloat16, 32 + 8 heads of 128: 512 rows 5.6 / 5.5 (below: 1.0 less with one), 1024 rows 8.2 / 6.8,
-// 16384 rows 93 / 73; backward of 16384 rows 139 / 117. float32, whose runs of four need twice the registers: 4096 rows 32 / 36, and
+// 16384 rows 93 / 73; backward of 16384 rows 139 / 118. float32, whose runs of four need twice the registers: 4096 rows 32 / 36, and
 // backward 56 / 79.
 constexpr int kNrRun = 4;
 int run_of(int64_t rows, int64_t heads, int dtype, bool vec, int lanes) {

@@ -6,8 +6,10 @@
 // over those tokens t, khat and vhat the cache's rows, dequantized. float32 sums, scores base 2; zeros for a row without
 // tokens.
 //
-// Bound by the cache's bytes up to about 64 pairs (node, q head) of a KV head, each token being read once a KV head, and by
-// the products behind that. tree_generic_kernel takes every cache, head size (up to 512) and page size on the vector ALU.
+// Its floor is the cache's bytes up to about 64 pairs (node, q head) of a KV head, each token being read once a KV head, and the
+// products behind that; the kernels on the matrix cores are bound by the vector ALU beside them. tree_generic_kernel takes every
+// cache, head size (up to 512) and page size on the vector ALU (8 sequences of 16 nodes and 1016 tokens, 32 / 8 heads of 80: 389 us
+// against 32 there): a workgroup reads a sequence's tokens for one row alone.
 #include "tree_attention.h"
 
 namespace kvfp8 {

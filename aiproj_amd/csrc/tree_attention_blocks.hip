@@ -15,18 +15,20 @@
 //                               reads of those rows
 // Operand types as in shared_prefix_narrow.h.
 //
-// Two workgroups share a CU (236 VGPRs, 77 KB of LDS each), so that one computes while the other begins or joins. Microseconds of
-// a call against blocks of 16 pairs (tree_attention_mfma.hip, which also takes 16-bit queries when built for them), and against
-// blocks of 32, 64 and 128 of eight waves, alone on their CU, cache in e4m3fn, head size 128:
-//   sequences, nodes, tokens, q / KV heads           16    8 x 32    8 x 64   8 x 128    4 x 64
+// Two workgroups share a CU (237 VGPRs, 77 KB of LDS each), so that one computes while the other begins or joins. Microseconds of
+// a call when that was chosen, four waves on 64 pairs, against blocks of 16 pairs from registers (as tree_attention_mfma.hip has them
+// for float32 queries; that form for 16-bit ones is gone) and against blocks of 32, 64 and 128 of eight waves, alone on their CU;
+// cache in e4m3fn, head size 128, and last the present kernel, behind later steps:
+//   sequences, nodes, tokens, q / KV heads           16    8 x 32    8 x 64   8 x 128    4 x 64    now
 //   64, 2, 2000, 64 / 8                              88        92       114       139        80
-//   32, 16, 4080, 32 / 8                            184       118        83       116        88
-//   61, 1 to 60, 1 to 3060, 16 / 4                  221       153       144       163       118
-//   8, 64, 32768, 32 / 8                            951       576       419       402       399
-// The vector ALU and the matrix cores bound it where there are rows enough: per step 215 and 16 instructions, of which two waves a
-// SIMD hide little from each other. The waves' priority is higher at the loads and the products (8 sequences of 32768 tokens: 377 us
-// with it, 399 without), and all of a step's operands leave LDS at its begin (393 against 403). With one row block HBM bounds it: 32
-// sequences of 4096 tokens 74 us without the join, 269 MB, 3.6 TB/s.
+//   32, 16, 4080, 32 / 8                            184       118        83       116        88     86
+//   61, 1 to 60, 1 to 3060, 16 / 4 (float16 q)      221       153       144       163       118    104
+//   8, 64, 32768, 32 / 8                            951       576       419       402       399    390
+// The vector ALU and the matrix cores bound it where there are rows enough: per step 225 and 16 instructions, of which two waves a
+// SIMD hide little from each other. Steps since that table: the waves' priority is higher at the loads and the products (8 sequences of
+// 32768 tokens: 399 us without it, 377 with it), and all of a step's operands leave LDS at its begin (403, 393). With one row block
+// the same bounds it before HBM does: 32 sequences of 4096 tokens take 78 us without the join, 269 MB at 3.4 TB/s, where one row a
+// sequence (kvfp8_decode_mfma.hip) takes 48: both tiles' waves read and widen every code, and every workgroup makes the plan.
 #include "joined_state.h"
 #include "shared_prefix_narrow.h"
 #include "tree_attention.h"

@@ -66,7 +66,7 @@ struct NodeProducts {
 };
 
 // Blocks of 16 pairs, for float32 queries: in three bf16 parts, whose operands leave no registers for more pairs. Bound by
-// the six products of a step: 32 sequences of 16 nodes and 4080 tokens, 32 / 8 heads of 128, 217 us (16-bit queries: 87).
+// the six products of a step: 32 sequences of 16 nodes and 4080 tokens, 32 / 8 heads of 128, 217 us (16-bit queries: 86).
 template <int C>
 __global__ void __launch_bounds__(64 * kTreeWaves)
 tree_narrow_kernel(TreeArgs a) {

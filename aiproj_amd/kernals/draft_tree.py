@@ -22,7 +22,8 @@ draft, the nodes above it and itself. The model's choices then say which path ho
 
 Matrix cores: float8_e4m3fn caches of head size 64, 80, 96, 112 or 128 with q of any type, and bf16 or f16 caches of head
 size 64 or 128 with q of their type, pages of 16 tokens and more, 16-byte aligned. Everything else, up to head size 512, goes
-to a vector-ALU kernel.
+to a vector-ALU kernel. Rows x q heads and sequences x max_nodes x q heads are below 2^22 each (65535 nodes of 64 heads; 255
+sequences of up to 256 of them); larger batches are refused, and go in parts.
 
 Nothing is synchronized with the host and no device value is read: trees, lengths and pages may change between replays of a
 captured call. No gradients: queries, keys and values that require them are refused while a graph is recorded, and dual
