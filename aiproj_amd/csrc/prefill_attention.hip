@@ -414,8 +414,8 @@ prefill_attention_kernel(PrefillArgs a) {
 // rows and 2.16e-4 -> 2.54e-4 for peaked ones (f16, D 80).
 // Measured, 16 prompts of 64 to 1984 tokens, 32q/8kv heads, D 80, f16, in two orders of the
 // lengths: 1031 and 1120 us on the general kernel above (which pads every product to 128
-// dims) -> 438 and 418 us (386 and 367 with the exponents of 64 and 128: the reference behind by
-// up to 2^8 and the scale fused into the subtraction, 3.6% of it the latter).
+// dims) -> 438 and 418 us (386 and 367 with the reference behind by up to 2^8, as for 64 and 128,
+// and the scale fused into the subtraction, 3.6% of it the latter).
 //
 // An item is one (sequence, KV head, query block): the eight waves are `gw` q heads
 // x (8 / gw) groups of 32 query rows, and its K/V blocks of 64 keys are staged once
@@ -509,9 +509,10 @@ prefill_fa_kernel(PrefillArgs a, int32_t units, int32_t upx, int32_t per_xcd) {
     constexpr bool kHalf = kD % 32 != 0;             // and one step of 16 dims
     // How far (log2) a row's max may exceed the reference that its probabilities are scaled by.
     // 80, 96 and 112: not at all, so that the largest probability is 1 and packed without error,
-    // as on the general kernel (see above). Their scaled scores are rounded before the reference is
-    // taken off for the same reason: a fused product would leave the reference's rounding in the
-    // exponent, which from scores of some 2^30 on is more than the exponent's range.
+    // as on the general kernel (see above). Scaled scores are rounded before the reference is taken
+    // off: a fused product would leave the reference's rounding in the exponent, which from scores
+    // of some 2^30 on is more than the exponent's range (64 x 1024 tokens, 16q/4kv, D 128, bf16:
+    // 355 us fused, 358 so; D 64 267 both).
     constexpr float kLag = kD == 64 || kD == 128 ? 8.0f : 0.0f;
     // Vector-memory instructions a wave issues: kBlockLoads per K/V block, kQLoads
     // for its Q operands of one item.
@@ -775,7 +776,7 @@ prefill_fa_kernel(PrefillArgs a, int32_t units, int32_t upx, int32_t per_xcd) {
         const bool full = kb * kKeys + kKeys - 1 <= qa && kb * kKeys + kKeys <= L;   // wave-uniform
 #pragma unroll
         for (int qt = 0; qt < kFaTiles; ++qt) {
-            // Raw scores (the scale is applied inside the exponent below), masked in
+            // Raw scores (the scale is applied to the maximum and the exponents below), masked in
             // place so that blocks without a mask keep them in their registers.
             if (!full) {
                 // Keep key kb * 64 + 16 kt + 4 j + jj when it is <= min(row, L - 1).
@@ -811,9 +812,7 @@ prefill_fa_kernel(PrefillArgs a, int32_t units, int32_t upx, int32_t per_xcd) {
         }
         float pr[kFaTiles][16];
         auto prob = [&](int qt, int i) __attribute__((always_inline)) {
-            const float x = sacc[i / 4][qt][i % 4];
-            pr[qt][i] = __builtin_amdgcn_exp2f(kLag > 0.0f ? __builtin_fmaf(x, a.scale_log2, neg_m[qt])
-                                                           : scaled_minus(x, a.scale_log2, neg_m[qt]));
+            pr[qt][i] = __builtin_amdgcn_exp2f(scaled_minus(sacc[i / 4][qt][i % 4], a.scale_log2, neg_m[qt]));
             l[qt] += pr[qt][i];
         };
         auto pack_half = [&](int pp) __attribute__((always_inline)) {
