@@ -794,9 +794,11 @@ prefill_fa_kernel(PrefillArgs a, int32_t units, int32_t upx, int32_t per_xcd) {
             // Lazy rescale (kLag): the accumulators keep a reference max m that is only moved
             // when some row's max grows by more than 2^8 (p <= 256 meanwhile, far
             // inside float32 and bf16 range), so the accumulators are rarely scaled.
+            // The difference is tested: from 2^27 on m + kLag may round to m + 16, and a probability
+            // of 2^16 is past float16's numbers.
             // Each lane tests its own 16 keys; only a rescale needs the row's max over
             // its four lanes.
-            if (__ballot(mx > m[qt] + kLag)) {
+            if (__ballot(mx - m[qt] > kLag)) {
                 const float m_new = fmaxf(m[qt], max_across_rows(mx));
                 const float m_use = m_new == kNegInf ? 0.0f : m_new;
                 // An item's first block finds the accumulators at zero: nothing to scale.

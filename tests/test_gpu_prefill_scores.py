@@ -55,3 +55,18 @@ def test_equal_keys_share_the_weight_at_any_size(form, size):
 def test_equal_keys_of_float16(form, size, top):
     """With an outlier channel of 6e4 in queries and keys scores are 4e8."""
     _equal_keys(F16, *form, size, top)
+
+
+def test_scores_a_step_past_what_the_reference_allows():
+    """A reference at which 2^8 more rounds to 2^16 more: the weights of the scores there are past float16's largest number. Keys 0,
+    128, .. have a score of 134601552 (base 2), keys 64, 192, .. the next float32, 16 above it."""
+    n, d, gen = 250, 64, t.Generator(device="cpu").manual_seed(1)
+    k, v, q = t.zeros(n, 2, d), t.randn(n, 2, d, generator=gen).clamp(-3, 3), t.zeros(n, 8, d)
+    k[::64, :, 0] = 13016.0
+    k[64::128, :, 1] = 1.0
+    q[..., 0], q[..., 1] = 57344.0, 64.0
+    (out, _), (want, weight) = _attend(*(x.to(F16).cuda() for x in (q, k, v)))
+    # The scores are 8 apart (base e), their float32 values 11: the lower ones weigh e^-8 or e^-11, of values up to 3 that are not the
+    # higher ones'. The others are roundings.
+    bound = HALF[F16] * want.abs() + (HALF[F16] + 2.0 ** -12) * weight + 2.0 ** -25 + 2 * 3 * math.exp(-8)
+    assert bool(out.isfinite().all()) and bool(((out.double() - want).abs() <= bound).all())
